@@ -290,6 +290,55 @@ int kbn_moe_route_topk(const void* logits, int logits_bf16, int64_t ld, int64_t 
                        int32_t* out_ids, kbn_stream_t stream);
 
 /*
+ * MXFP4: blocks of 32 values along K, e2m1 codes (two per byte, the even element in the low nibble) and one E8M0 scale byte
+ * b = 2^(b-127) per block.  kb-nano has no 4-bit path; these are the 4-bit counterparts of the 1x128 FP8 entry points above.
+ * K % 32 == 0.
+ *   kbn_quant_mxfp4: x [M,K] bf16, row stride ld_x -> q [M,K/2] bytes, row stride ld_q (a multiple of 4; q 4-byte aligned).
+ *     scale byte of a block with largest magnitude a: 2^ceil(log2(a/6)), at least 2^-127 -- no value is clipped; codes are
+ *     rounded to nearest even.  A block with an infinity or a NaN gets byte 255 and codes 0: it reads back as NaN.
+ *     scale (may be null): row-major bytes [M,K/32], row stride s_row; sf_packed (may be null; one of the two is needed):
+ *     the same bytes in the packed form kbn_mxfp4_gemm_nt reads, kbn_packed_mxfp4_bytes(M, K) bytes, 16-byte aligned;
+ *     words of rows past M in the last 128-row block are left unwritten, blocks past K count as 2^0.
+ *   kbn_silu_mul_quant_mxfp4: in [M, 2*N2] bf16 (gate | up) -> the same outputs for y = bf16(bf16(silu(gate)) * up), [M, N2].
+ *     N2 % 32 == 0.  Enqueues the table fill of kbn_silu_mul_quant_1x128 on first use.
+ *   kbn_dequant_mxfp4: codes and row-major scales -> bf16 [M,K], row stride ld_out.
+ *   kbn_pack_mxfp4_scales: row-major scale bytes [rows,K/32] -> the packed form (rows past the last one: 2^0).
+ * Strides of codes and scales are in bytes.
+ */
+int64_t kbn_packed_mxfp4_bytes(int64_t rows, int64_t K);
+int kbn_quant_mxfp4(const void* x, int64_t M, int64_t K, int64_t ld_x, void* q, int64_t ld_q, void* scale,
+                    int64_t s_row, void* sf_packed, kbn_stream_t stream);
+int kbn_silu_mul_quant_mxfp4(const void* in, int64_t M, int64_t N2, int64_t ld_in, void* q, int64_t ld_q, void* scale,
+                             int64_t s_row, void* sf_packed, kbn_stream_t stream);
+int kbn_dequant_mxfp4(const void* q, int64_t ld_q, const void* scale, int64_t s_row, int64_t M, int64_t K, void* out,
+                      int64_t ld_out, kbn_stream_t stream);
+int kbn_pack_mxfp4_scales(const void* scale, int64_t rows, int64_t K, int64_t s_row, void* packed, kbn_stream_t stream);
+
+/*
+ * The MoE layer behind the router's logits for at most 16 tokens, in two kernels: what kbn_moe_route_topk, the permutation,
+ * the grouped GEMMs with their activation and quantisation, and the weighted sum do for larger batches
+ * (tasks/baseline/L2/qwen3_moe.py:161-188, tasks/baseline/L2/fused_experts.py:208-283).
+ *   x [T,H] bf16 (row stride ld_x, a multiple of 8; 16-byte aligned); logits and the routing arguments as in
+ *   kbn_moe_route_topk, with topk <= 16; H % 128 == 0, I % 128 == 0.
+ *   weight_format 0: FP8, w13 e4m3 [E,2I,H] with fp32 scales [E,2I/128,H/128], w2 e4m3 [E,H,I] with [E,H/128,I/128] (any
+ *     positive scales); 1: MXFP4, codes w13 [E,2I,H/2], w2 [E,H,I/2] with row-major scale bytes [E,2I,H/32], [E,H,I/32].
+ *     All contiguous.
+ *   out [T,H] bf16, row stride ld_out; out_w fp32 [T,topk] and out_ids int32 [T,topk] (both or neither): the routing.
+ * The activations are not quantised (a few tokens cost no bytes): out = bf16(sum_s w_s * W2 (silu(W1 x) * (W3 x))), summed
+ * in fp32 in slot order, tokens and activated rows rounded to 11 bits beside a power of two per row.  A token whose logits
+ * hold a NaN gets NaNs (and ids -1).  workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents
+ * irrelevant; calls that may overlap need one each.  KBN_ERR_UNSUPPORTED when a row of max(H, I) values does not fit the
+ * shared memory of an SM (about 55,000).  Waits inside are bounded and report through kbn_gemm_status.
+ */
+int64_t kbn_moe_few_tokens_workspace_bytes(int64_t T, int64_t topk, int64_t H, int64_t I);
+int kbn_moe_few_tokens(const void* x, int64_t ld_x, int64_t T, const void* logits, int logits_bf16, int64_t ld, int64_t E,
+                       int softmax, const float* bias, int64_t n_group, int64_t topk_group, int64_t topk, int renormalize,
+                       float renorm_floor, float scale, int round_bf16, int weight_format, const void* w13,
+                       const void* w13_s, const void* w2, const void* w2_s, int64_t H, int64_t I, void* out,
+                       int64_t ld_out, float* out_w, int32_t* out_ids, void* workspace, int64_t workspace_bytes,
+                       kbn_stream_t stream);
+
+/*
  * Expert-parallel FP8 MoE layer over the GPUs of one NVLink/NVSwitch box, one process per GPU.
  * Experts are split in contiguous blocks (rank r owns experts [r*E/R, (r+1)*E/R)); tokens stay on
  * their source rank.  Dispatch and combine are peer stores over NVLink issued by this library's

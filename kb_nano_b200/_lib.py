@@ -48,6 +48,14 @@ SIGNATURES = {
     "kbn_moe_pair_experts": (_i32, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr]),
     "kbn_moe_permute": (_i32, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
     "kbn_moe_permute_sf": (_i32, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _ptr]),
+    "kbn_packed_mxfp4_bytes": (_i64, [_i64, _i64]),
+    "kbn_quant_mxfp4": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr]),
+    "kbn_silu_mul_quant_mxfp4": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr]),
+    "kbn_dequant_mxfp4": (_i32, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _ptr]),
+    "kbn_pack_mxfp4_scales": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _ptr]),
+    "kbn_moe_few_tokens_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "kbn_moe_few_tokens": (_i32, [_ptr, _i64, _i64, _ptr, _i32, _i64, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _f32, _f32, _i32, _i32, _ptr, _ptr,
+                                  _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr]),
     "kbn_ep_create": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_ptr)]),
     "kbn_ep_ipc_handle": (_i32, [_ptr, _ptr]),
     "kbn_ep_attach": (_i32, [_ptr, _ptr]),

@@ -1,0 +1,330 @@
+// Weight streaming for a few activation rows: the core of the MoE layer for a few tokens and of the MXFP4 linear layer
+// on at most eight rows.
+//
+// With at most eight rows (tokens) per weight matrix a product is a weight stream, 2 to 16 flop per weight byte, and what
+// counts is that enough weight bytes are in flight on every SM all the time.  One CTA per SM walks a contiguous range of
+// units; a unit is 16 weight rows (two boxes of eight) over the whole K.  A producer warp keeps a ring of 16 KB stages
+// full with 3-D tiled TMA loads (eight rows of a box, up to 16 chunks of 128 K-values each, one instruction per box) and
+// the block scales beside them (4-byte asynchronous copies); sixteen consumer warps split the chunks.
+//
+//   product    mma.sync.m16n8k16, f16 x f16 -> fp32: the 16 weight rows are its M, the tokens its N.  (tcgen05 would spend a
+//              128-row tile on them and needs its operands in fp8 or fp4; at this intensity the legacy instruction is far
+//              from being the bound.)  e4m3 and e2m1 codes are converted to f16 exactly, two per instruction.
+//   tokens     held in shared memory as f16, each row multiplied by a power of two that brings its largest magnitude into
+//              [2^14, 2^15); the power is taken out again after the sum.  bf16 has 8 significant bits and f16 has 11, so a
+//              value is kept exactly down to 2^-32 of the row's largest, and below that to within 2^-40 of it.
+//   scales     FP8: one fp32 factor per 128 x 128 block, applied to each 128-K partial sum.  MXFP4: one power of two per row
+//              and 32 K-values, applied to each 32-K partial sum.  Both in fp32, so any scale works.
+//   K order    a dot product does not care: lane t of a quad takes 16 consecutive K-values of a row per load (FP8) or
+//              eight (MXFP4), and reads the same K-values of its token.
+//   sums       fp32; the warps' partial results meet in shared memory and are added in warp order (bit-reproducible).
+#pragma once
+#include "gemm_common.cuh"
+#include "mxfp4.cuh"
+
+namespace kbn {
+namespace few {
+
+enum WeightFormat : int { kFp8 = 0, kMxfp4 = 1 };
+
+constexpr int kConsumerWarps = 16;
+constexpr int kThreads = 32 * (kConsumerWarps + 1);      // consumers first, then the producer warp
+constexpr int kStageBytes = 16384;                        // two boxes of 8 KB
+constexpr int kMaxGroup = 8;                              // tokens per job: the N of the matrix instruction
+constexpr int kMaxTokens = 16, kMaxTopk = 16, kMaxPairs = kMaxTokens * kMaxTopk;
+constexpr int kMaxStages = 12;
+constexpr int kMinStages = 5;                             // 80 KB in flight per SM: what 6.5 TB/s needs at about 1.5 us
+
+template <int FMT>
+struct Fmt;
+template <>
+struct Fmt<kFp8> {
+    static constexpr int kChunkBytes = 128, kChunks = 8, kScaleBytes = 128, kTokenPad = 16;
+    static constexpr int kArrivals = 8;                   // warps that read a stage
+};
+template <>
+struct Fmt<kMxfp4> {
+    static constexpr int kChunkBytes = 64, kChunks = 16, kScaleBytes = 1024, kTokenPad = 64;
+    static constexpr int kArrivals = 16;
+};
+
+// Where a weight matrix's scales lie.  FP8: fp32 [rows / 128, KC].  MXFP4: one 32-bit word per row and chunk, row-major
+// (packed == 0: word (row, c) at row * KC + c) or in the packed layout of the tensor core.
+struct ScaleSource {
+    const void* base;
+    int32_t packed;
+};
+
+struct Smem {
+    uint8_t* ring;         // stages, 1024-byte aligned
+    uint8_t* scales;       // one area per stage
+    uint8_t* tokens;       // f16 rows, stride token_stride
+    float* red;            // two buffers of 16 warps x 128 partial sums
+    uint64_t* bars;        // full[stages], empty[stages]
+    int32_t stages;
+};
+
+__device__ __forceinline__ void mma_f16_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 bytes -> two packed f16 pairs.  Exact.
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on `bar` once this thread's earlier cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumerWarps) : "memory"); }
+
+// Ring position, advanced one stage at a time.
+struct RingPos {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void advance(uint32_t stages) {
+        if (++slot == stages) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+__device__ __forceinline__ void init_ring(const Smem& s, int arrivals) {
+    for (int i = 0; i < s.stages; ++i) {
+        ptx::mbar_init(ptx::smem_u32(s.bars + i), 1 + 32);                    // the producer's bytes, its 32 lanes' scale copies
+        ptx::mbar_init(ptx::smem_u32(s.bars + s.stages + i), (uint32_t)arrivals);
+    }
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+}
+
+// Producer warp: all stages of one unit.  row_a, row_b: first rows of the two boxes (in rows of the tensor map; a box past
+// the last row is filled with zeros by the TMA).  n_rows: rows the scale array covers.
+template <int FMT>
+__device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const void* tmap, const ScaleSource& sc, int32_t row_a, int32_t row_b,
+                                             int32_t n_rows, int32_t KC, int lane, const WaitCtx& w) {
+    using F = Fmt<FMT>;
+    for (int32_t c0 = 0; c0 < KC; c0 += F::kChunks) {
+        const uint32_t full = ptx::smem_u32(s.bars + pos.slot), empty = ptx::smem_u32(s.bars + s.stages + pos.slot);
+        wait_bar(empty, pos.phase ^ 1u, w);
+        const uint32_t dst = ptx::smem_u32(s.ring) + pos.slot * kStageBytes;
+        if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(full, kStageBytes);
+            tma_load_3d(dst, tmap, 0, row_a, c0, full);
+            tma_load_3d(dst + kStageBytes / 2, tmap, 0, row_b, c0, full);
+        }
+        const uint32_t sdst = ptx::smem_u32(s.scales) + pos.slot * F::kScaleBytes;
+        if (FMT == kFp8) {
+            // lane = 8 * box + chunk
+            const int32_t c = c0 + (lane & 7);
+            if (lane < 16 && c < KC) {
+                const int32_t row = lane < 8 ? row_a : row_b;
+                cp_async4(sdst + lane * 4, static_cast<const float*>(sc.base) + (int64_t)(row >> 7) * KC + c);
+            }
+        } else {
+            // word (chunk, row of 16) at (chunk * 16 + row) * 4: eight words per lane
+            const int32_t r = lane & 15;
+            const int32_t row = min((r < 8 ? row_a : row_b - 8) + r, n_rows - 1);
+            const uint32_t* base = static_cast<const uint32_t*>(sc.base);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int32_t c = c0 + 2 * i + (lane >> 4);
+                if (c < KC)
+                    cp_async4(sdst + (uint32_t)((2 * i + (lane >> 4)) * 16 + r) * 4u,
+                              base + (sc.packed ? (int64_t)mxfp4::packed_word(row, c, KC) : (int64_t)row * KC + c));
+            }
+        }
+        cp_async_arrive(full);
+        pos.advance((uint32_t)s.stages);
+    }
+}
+
+// Consumer warp: its chunks of one unit, added to acc.  acc[0..1]: row g of box 0 with tokens 2t, 2t + 1; acc[2..3]: row g of
+// box 1.  FP8: a stage has work for eight warps; slots with an even number belong to warps 0-7, the others to warps 8-15.
+// A slot must always have the same readers: a warp may only test a barrier for a phase if it has seen the phase before it
+// complete, because the test tells two phases apart by their parity alone.
+template <int FMT>
+__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, uint32_t token_row,
+                                             float (&acc)[4], const WaitCtx& w) {
+    using F = Fmt<FMT>;
+    const int g = lane >> 2, t = lane & 3;
+    const int cw = FMT == kFp8 ? (warp & 7) : warp;
+    for (int32_t c0 = 0; c0 < KC; c0 += F::kChunks) {
+        const RingPos here = pos;
+        pos.advance((uint32_t)s.stages);
+        if (FMT == kFp8 && (here.slot & 1u) != (uint32_t)(warp >> 3)) continue;
+        wait_bar(ptx::smem_u32(s.bars + here.slot), here.phase, w);
+        const int32_t c = c0 + cw;
+        if (c < KC) {
+            const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * 8 + g) * F::kChunkBytes;
+            const uint32_t box1 = box0 + kStageBytes / 2;
+            const uint32_t sdst = ptx::smem_u32(s.scales) + here.slot * F::kScaleBytes;
+            if (FMT == kFp8) {
+                float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t piece = (uint32_t)(t + 4 * j);
+                    const uint4 wa = lds128(box0 + ((piece ^ (uint32_t)g) << 4)), wb = lds128(box1 + ((piece ^ (uint32_t)g) << 4));
+                    const uint32_t ta = token_row + (uint32_t)(c * 128 + (int)piece * 16) * 2u;
+                    const uint4 x0 = lds128(ta), x1 = lds128(ta + 16);
+                    uint32_t a0, a1, a2, a3;
+                    e4m3x4_to_f16(wa.x, a0, a2); e4m3x4_to_f16(wb.x, a1, a3);
+                    mma_f16_m16n8k16(p, a0, a1, a2, a3, x0.x, x0.y);
+                    e4m3x4_to_f16(wa.y, a0, a2); e4m3x4_to_f16(wb.y, a1, a3);
+                    mma_f16_m16n8k16(q, a0, a1, a2, a3, x0.z, x0.w);
+                    e4m3x4_to_f16(wa.z, a0, a2); e4m3x4_to_f16(wb.z, a1, a3);
+                    mma_f16_m16n8k16(p, a0, a1, a2, a3, x1.x, x1.y);
+                    e4m3x4_to_f16(wa.w, a0, a2); e4m3x4_to_f16(wb.w, a1, a3);
+                    mma_f16_m16n8k16(q, a0, a1, a2, a3, x1.z, x1.w);
+                }
+                const float s0 = __uint_as_float(lds32(sdst + cw * 4)), s1 = __uint_as_float(lds32(sdst + 32 + cw * 4));
+                acc[0] = fmaf(p[0] + q[0], s0, acc[0]);
+                acc[1] = fmaf(p[1] + q[1], s0, acc[1]);
+                acc[2] = fmaf(p[2] + q[2], s1, acc[2]);
+                acc[3] = fmaf(p[3] + q[3], s1, acc[3]);
+            } else {
+                const uint32_t sw0 = lds32(sdst + (uint32_t)(cw * 16 + g) * 4u), sw1 = lds32(sdst + (uint32_t)(cw * 16 + 8 + g) * 4u);
+                const uint32_t swz = (uint32_t)(g >> 1) & 3u;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const uint32_t off = (((uint32_t)b ^ swz) << 4) + (uint32_t)t * 4u;
+                    const uint32_t wa = lds32(box0 + off), wb = lds32(box1 + off);
+                    const uint4 x = lds128(token_row + (uint32_t)(c * 128 + b * 32 + t * 8) * 2u);
+                    uint32_t ha[4], hb[4];
+                    mxfp4::unpack_e2m1x8(wa, ha);
+                    mxfp4::unpack_e2m1x8(wb, hb);
+                    float p[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16_m16n8k16(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+                    mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
+                    const float s0 = mxfp4::scale_value((sw0 >> (8 * b)) & 0xffu), s1 = mxfp4::scale_value((sw1 >> (8 * b)) & 0xffu);
+                    acc[0] = fmaf(p[0], s0, acc[0]);
+                    acc[1] = fmaf(p[1], s0, acc[1]);
+                    acc[2] = fmaf(p[2], s1, acc[2]);
+                    acc[3] = fmaf(p[3], s1, acc[3]);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + s.stages + here.slot));
+    }
+}
+
+// Adds up a unit's 16 partial results: element (row of 16) * 8 + token of buffer `buf`.
+__device__ __forceinline__ void store_partials(const Smem& s, int buf, int warp, int lane, const float (&acc)[4]) {
+    float* r = s.red + (buf * kConsumerWarps + warp) * 128;
+    const int g = lane >> 2, t = lane & 3;
+    *reinterpret_cast<float2*>(r + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
+    *reinterpret_cast<float2*>(r + (g + 8) * 8 + 2 * t) = make_float2(acc[2], acc[3]);
+}
+__device__ __forceinline__ float sum_partials(const Smem& s, int buf, int element) {
+    const float* r = s.red + buf * kConsumerWarps * 128 + element;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kConsumerWarps; ++i) v += r[i * 128];
+    return v;
+}
+
+// x * 2^e for |e| up to 254, in two exact steps (one factor alone may leave fp32's range).
+__device__ __forceinline__ float scale_pow2(float x, int e) {
+    const int h = e >> 1;
+    return x * __uint_as_float((uint32_t)(h + 127) << 23) * __uint_as_float((uint32_t)(e - h + 127) << 23);
+}
+// Exponent that brings a row's largest finite magnitude (fp32 bit pattern) into [2^14, 2^15); 0 for an all-zero row.
+__device__ __forceinline__ int token_exponent(uint32_t amax_bits) {
+    if (amax_bits == 0u) return 0;
+    int e = (int)(amax_bits >> 23) - 127;
+    if (amax_bits < 0x00800000u) e = -118 - __clz((int)amax_bits);      // subnormal: 2^(31 - clz - 149)
+    return 14 - e;
+}
+
+// A few f16 rows of K values into shared memory from fp32 or bf16 rows in global memory, normalised as described above, by
+// all consumer threads.  row_ptr(i): row i < n.  expo[i] receives the exponent to take out again.  max_bits: n words.
+// The caller has synchronised the consumers since the last use of the rows; a consumer_sync() must follow.
+template <typename T, typename RowPtr>
+__device__ __forceinline__ void load_tokens(uint8_t* tokens, uint32_t stride, int n, int K, RowPtr row_ptr, uint32_t* max_bits, int* expo, int tid) {
+    const int vecs = K / 8;                       // K % 128 == 0: sixteen consecutive threads share a row
+    const int total = n * vecs;
+    if (tid < n) max_bits[tid] = 0;
+    consumer_sync();
+    auto load = [&](int i, float (&f)[8]) {
+        const int row = i / vecs, v = i - row * vecs;
+        if (sizeof(T) == 2) {
+            const uint4 u = *(reinterpret_cast<const uint4*>(row_ptr(row)) + v);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[2 * j] = bf16_lo(w[j]);
+                f[2 * j + 1] = bf16_hi(w[j]);
+            }
+        } else {
+            const float4* p = reinterpret_cast<const float4*>(row_ptr(row)) + 2 * v;
+            const float4 a = __ldcg(p), b = __ldcg(p + 1);
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+        }
+        return row;
+    };
+    for (int i0 = 0; i0 < total; i0 += 32 * kConsumerWarps) {
+        const int i = i0 + tid;
+        uint32_t m = 0;
+        int row = 0;
+        if (i < total) {
+            float f[8];
+            row = load(i, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
+                if (b < 0x7f800000u) m = max(m, b);       // infinities and NaNs keep their place, the finite values set the scale
+            }
+        }
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((tid & 15) == 0 && i < total) atomicMax(max_bits + row, m);
+    }
+    consumer_sync();
+    for (int i = tid; i < total; i += 32 * kConsumerWarps) {
+        float f[8];
+        const int row = load(i, f);
+        const int e = token_exponent(max_bits[row]);
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 p = __floats2half2_rn(scale_pow2(f[2 * j], e), scale_pow2(f[2 * j + 1], e));
+            h[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        *reinterpret_cast<uint4*>(tokens + (size_t)row * stride + (size_t)(i - row * vecs) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    if (tid < n) expo[tid] = -token_exponent(max_bits[tid]);
+}
+
+// Host: ring depth for `fixed` bytes of other shared memory (0: does not fit).
+constexpr int kSmemMax = 232448;
+
+}  // namespace few
+}  // namespace kbn

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 FP8 = torch.float8_e4m3fn
 
@@ -137,3 +137,74 @@ def fused_experts_fp8(hidden_states: torch.Tensor, w13: torch.Tensor, w2: torch.
 
 
 LAUNCHES_PER_LAYER = 7   # quant, rank, offsets, scatter, GEMM1 (+activation), GEMM2, combine
+
+
+FEW_TOKENS_MAX = 16      # most tokens of a few_tokens_moe call
+
+
+def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
+                   w2_scale: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
+                   topk_group: int = 1, renormalize: bool = True, renorm_floor: float = 0.0, scale: float = 1.0, round_bf16: bool = False,
+                   out: torch.Tensor | None = None, out_w: torch.Tensor | None = None, out_ids: torch.Tensor | None = None) -> torch.Tensor:
+    """The whole MoE layer behind the router for 1 to 16 tokens, in two kernels: routing (the arguments of ops.moe_route_topk), the
+    chosen experts' SwiGLU MLPs, the weighted sum.  Bound by the chosen experts' weights, each read once.
+
+    hidden_states bf16 [T,H], router_logits fp32 or bf16 [T,E].  Experts in FP8 -- w13 e4m3 [E,2I,H] with fp32 scales
+    [E,2I/128,H/128], w2 e4m3 [E,H,I] with [E,H/128,I/128], any positive scales -- or in MXFP4: codes uint8 [E,2I,H/2] and
+    [E,H,I/2] with E8M0 scales uint8 [E,2I,H/32] and [E,H,I/32].  H and I are multiples of 128, top_k at most 16.
+    Returns out bf16 [T,H]; out_w fp32 [T,top_k] and out_ids int32 [T,top_k], given together, receive the routing.
+
+    The activations are not quantised (with a few tokens that saves no bytes), so results differ from fused_experts_fp8 by
+    that pipeline's FP8 rounding of its activations.  Scratch comes from the caching allocator with every call: calls on
+    several streams, and captured graphs, do not share any."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"unsupported scoring function {scoring!r}")
+    if hidden_states.dim() != 2 or hidden_states.dtype != torch.bfloat16 or hidden_states.stride(1) != 1:
+        raise ValueError("hidden_states must be bf16 [T, H], contiguous along H")
+    t, h = hidden_states.shape
+    if router_logits.dim() != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16) or router_logits.shape[0] != t or router_logits.stride(1) != 1:
+        raise ValueError(f"router_logits must be fp32 or bf16 [{t}, E], contiguous along E")
+    if not 0 <= t <= FEW_TOKENS_MAX:
+        raise ValueError(f"few_tokens_moe takes at most {FEW_TOKENS_MAX} tokens, got {t}")
+    e = router_logits.shape[1]
+    if w13.dtype == FP8 and w2.dtype == FP8:
+        fmt, i = 0, w2.shape[-1]
+        want = ((e, 2 * i, h), (e, h, i), (e, (2 * i + 127) // 128, (h + 127) // 128), (e, (h + 127) // 128, (i + 127) // 128))
+        scale_types = (torch.float32,)
+    elif w13.dtype in ops._CODE_DTYPES and w2.dtype in ops._CODE_DTYPES:
+        fmt, i = 1, w2.shape[-1] * 2
+        want = ((e, 2 * i, h // 2), (e, h, i // 2), (e, 2 * i, h // 32), (e, h, i // 32))
+        scale_types = ops._BYTE_SCALE_DTYPES
+    else:
+        raise ValueError(f"w13 and w2 must both be float8_e4m3fn or both MXFP4 codes (uint8), got {w13.dtype} and {w2.dtype}")
+    if h % 128 or i % 128:
+        raise ValueError(f"hidden size {h} and intermediate size {i} must be multiples of 128")
+    for name, x, shape in zip(("w13", "w2", "w13_scale", "w2_scale"), (w13, w2, w13_scale, w2_scale), want):
+        if tuple(x.shape) != shape or not x.is_contiguous() or (name.endswith("scale") and x.dtype not in scale_types):
+            raise ValueError(f"{name} must be contiguous {shape}{'' if not name.endswith('scale') else f' {scale_types[0]}'}, got {x.dtype} {tuple(x.shape)}")
+    if out is None:
+        out = torch.empty(t, h, dtype=torch.bfloat16, device=hidden_states.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (t, h) or out.stride(1) != 1:
+        raise ValueError(f"out must be bf16 [{t}, {h}], contiguous along H")
+    if (out_w is None) != (out_ids is None):
+        raise ValueError("out_w and out_ids come together")
+    if out_w is not None:
+        if out_w.dtype != torch.float32 or tuple(out_w.shape) != (t, top_k) or not out_w.is_contiguous():
+            raise ValueError("out_w must be contiguous float32 [T, top_k]")
+        if out_ids.dtype != torch.int32 or tuple(out_ids.shape) != (t, top_k) or not out_ids.is_contiguous():
+            raise ValueError("out_ids must be contiguous int32 [T, top_k]")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != e or not bias.is_contiguous()):
+        raise ValueError("bias must be contiguous float32 [E]")
+    dev = ops._cuda(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, out, *(x for x in (bias, out_w, out_ids) if x is not None))
+    lib = _lib.load()
+    with ops._on(dev):
+        # allocated on the calling stream's account: the allocator hands it to nobody else before this call's kernels have run
+        nbytes = int(lib.kbn_moe_few_tokens_workspace_bytes(t, top_k, h, i))
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        _lib.check(lib.kbn_moe_few_tokens(
+            hidden_states.data_ptr(), hidden_states.stride(0) if t > 1 else h, t, router_logits.data_ptr(), int(router_logits.dtype == torch.bfloat16),
+            router_logits.stride(0) if t > 1 else e, e, int(scoring == "softmax"), bias.data_ptr() if bias is not None else None, n_group, topk_group,
+            top_k, int(renormalize), renorm_floor, scale, int(round_bf16), fmt, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
+            h, i, out.data_ptr(), out.stride(0) if t > 1 else h, out_w.data_ptr() if out_w is not None else None,
+            out_ids.data_ptr() if out_ids is not None else None, ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream))
+    return out

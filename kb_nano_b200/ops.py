@@ -632,3 +632,97 @@ def requant_weights_ue8m0(w_fp8: torch.Tensor, scale: torch.Tensor, eps: float =
     # the scales changed behind torch's version counter: forget any packed copy made from the old values
     for key in [k_ for k_ in _WEIGHT_SF_CACHE if k_[0] == scale.data_ptr()]:
         _WEIGHT_SF_CACHE.pop(key, None)
+
+
+# ---- MXFP4: blocks of 32 along K, e2m1 codes (two per byte, even element in the low nibble), E8M0 scale bytes --------
+
+MX_BLOCK = 32
+_CODE_DTYPES = (torch.uint8, torch.float4_e2m1fn_x2)
+_BYTE_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def packed_mxfp4_bytes(rows: int, k: int) -> int:
+    """Size of the packed scale buffer of [rows, k] MXFP4 values (what mxfp4_gemm_nt reads)."""
+    return (rows + 127) // 128 * ((k + 127) // 128) * 512
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor; that of a single row is free in torch and is taken as the row's length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check_codes(q: torch.Tensor, m: int, k: int, what: str) -> None:
+    if q.dtype not in _CODE_DTYPES or tuple(q.shape) != (m, k // 2) or q.stride(1) != 1:
+        raise ValueError(f"{what} must be uint8 (or float4_e2m1fn_x2) [{m}, {k // 2}], contiguous along the last dim, got {q.dtype} {tuple(q.shape)}")
+
+
+def _check_byte_scales(s: torch.Tensor, m: int, k: int, what: str) -> None:
+    if s.dtype not in _BYTE_SCALE_DTYPES or tuple(s.shape) != (m, k // MX_BLOCK) or (s.stride(1) != 1 and s.shape[1] > 1):
+        raise ValueError(f"{what} must be uint8 (or float8_e8m0fnu) [{m}, {k // MX_BLOCK}], contiguous along the last dim, got {s.dtype} {tuple(s.shape)}")
+
+
+def _check_packed_mxfp4(buf: torch.Tensor, rows: int, k: int, dev, what: str) -> None:
+    need = packed_mxfp4_bytes(rows, k)
+    if buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.device != dev or buf.numel() < need or buf.data_ptr() % 16:
+        raise ValueError(f"{what} must be a contiguous, 16-byte aligned uint8 buffer on {dev} with at least {need} bytes")
+
+
+def _quant_mxfp4_call(fn: str, x: torch.Tensor, k: int, out_fp4: torch.Tensor, out_scale: torch.Tensor | None, packed_sf: torch.Tensor | None) -> None:
+    m = x.shape[0]
+    dev = _cuda(x, out_fp4, *(t for t in (out_scale, packed_sf) if t is not None))
+    if k % MX_BLOCK:
+        raise ValueError(f"the quantised dimension ({k}) must be a multiple of {MX_BLOCK}")
+    _check_codes(out_fp4, m, k, "out_fp4")
+    if out_scale is None and packed_sf is None:
+        raise ValueError("give out_scale (row-major scales), packed_sf (the GEMM's layout) or both")
+    if out_scale is not None:
+        _check_byte_scales(out_scale, m, k, "out_scale")
+    if packed_sf is not None:
+        _check_packed_mxfp4(packed_sf, m, k, dev, "packed_sf")
+    with _on(dev):
+        _lib.check(getattr(_lib.load(), fn)(x.data_ptr(), m, k, _row_stride(x), out_fp4.data_ptr(), _row_stride(out_fp4),
+                                            out_scale.data_ptr() if out_scale is not None else None,
+                                            _row_stride(out_scale) if out_scale is not None else 0,
+                                            packed_sf.data_ptr() if packed_sf is not None else None, _stream(x)))
+
+
+def quant_mxfp4(x: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor | None = None, packed_sf: torch.Tensor | None = None) -> None:
+    """x bf16 [M,K] -> MXFP4: out_fp4 uint8 [M,K/2] and the E8M0 scales of its blocks of 32, row-major in out_scale uint8
+    [M,K/32] and / or in the packed form of mxfp4_gemm_nt in packed_sf (uint8, packed_mxfp4_bytes(M, K) bytes).  The scale is
+    the smallest power of two that clips nothing; a block with an infinity or a NaN becomes NaN."""
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
+        raise ValueError(f"x must be bf16 [M,K], contiguous along K, got {x.dtype} {tuple(x.shape)}")
+    _quant_mxfp4_call("kbn_quant_mxfp4", x, x.shape[1], out_fp4, out_scale, packed_sf)
+
+
+def silu_mul_quant_mxfp4(inp: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor | None = None, packed_sf: torch.Tensor | None = None) -> None:
+    """inp bf16 [M, 2*N2] (gate | up) -> bf16(bf16(silu(gate)) * up) in MXFP4, [M, N2]; outputs as in quant_mxfp4."""
+    if inp.dim() != 2 or inp.dtype != torch.bfloat16 or inp.stride(1) != 1 or inp.shape[1] % 2:
+        raise ValueError(f"inp must be bf16 [M, 2*N2], contiguous along the last dim, got {inp.dtype} {tuple(inp.shape)}")
+    _quant_mxfp4_call("kbn_silu_mul_quant_mxfp4", inp, inp.shape[1] // 2, out_fp4, out_scale, packed_sf)
+
+
+def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
+    """MXFP4 codes [M,K/2] with row-major scales [M,K/32] -> out bf16 [M,K] (exact within bf16's range)."""
+    dev = _cuda(q, scale, out)
+    if out.dim() != 2 or out.dtype != torch.bfloat16 or out.stride(1) != 1 or out.shape[1] % MX_BLOCK:
+        raise ValueError(f"out must be bf16 [M,K], contiguous along K, K a multiple of {MX_BLOCK}, got {out.dtype} {tuple(out.shape)}")
+    m, k = out.shape
+    _check_codes(q, m, k, "q")
+    _check_byte_scales(scale, m, k, "scale")
+    with _on(dev):
+        _lib.check(_lib.load().kbn_dequant_mxfp4(q.data_ptr(), _row_stride(q), scale.data_ptr(), _row_stride(scale), m, k, out.data_ptr(),
+                                                 _row_stride(out), _stream(out)))
+
+
+def pack_mxfp4_scales(scale: torch.Tensor, k: int) -> torch.Tensor:
+    """Row-major E8M0 scales uint8 [rows, K/32] -> packed uint8 buffer for mxfp4_gemm_nt (done once per weight)."""
+    if scale.dim() != 2 or k % MX_BLOCK:
+        raise ValueError(f"scale must be 2-D and K={k} a multiple of {MX_BLOCK}")
+    dev = _cuda(scale)
+    rows = scale.shape[0]
+    _check_byte_scales(scale, rows, k, "scale")
+    out = torch.empty(packed_mxfp4_bytes(rows, k), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(_lib.load().kbn_pack_mxfp4_scales(scale.data_ptr(), rows, k, _row_stride(scale), out.data_ptr(), _stream(scale)))
+    return out
