@@ -314,6 +314,17 @@ int kbn_dequant_mxfp4(const void* q, int64_t ld_q, const void* scale, int64_t s_
                       int64_t ld_out, kbn_stream_t stream);
 int kbn_pack_mxfp4_scales(const void* scale, int64_t rows, int64_t K, int64_t s_row, void* packed, kbn_stream_t stream);
 
+/* Dense MXFP4 GEMM: C[m,n] = sum_k A[m,k] B[n,k] (+ bias[n], fp32), codes A [M,K/2] and B [N,K/2] contiguous, scales in the
+ * packed form, fp32 accumulation (tcgen05 kind::mxf4), bf16 out with row stride ldc.  bias: bf16 [N] or null.  K % 32 == 0;
+ * operand pointers 16-byte aligned.  The 4-bit counterpart of kbn_fp8_gemm_nt_ue8m0.
+ * kbn_mxfp4_linear: the same on bf16 rows x [M,K] (row stride ld_x), quantised on the way as kbn_quant_mxfp4 does.  a_q
+ * (M*K/2 bytes) and a_sf (kbn_packed_mxfp4_bytes(M, K) bytes) are scratch, 16-byte aligned; up to eight rows with
+ * K % 128 == 0 take one launch that leaves them untouched, if the rows fit the shared memory of an SM. */
+int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const void* B, const void* sfb_packed, const void* bias,
+                      void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, kbn_stream_t stream);
+int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t K, void* a_q, void* a_sf, const void* B,
+                     const void* sfb_packed, const void* bias, void* C, int64_t ldc, int64_t N, kbn_stream_t stream);
+
 /*
  * The MoE layer behind the router's logits for at most 16 tokens, in two kernels: what kbn_moe_route_topk, the permutation,
  * the grouped GEMMs with their activation and quantisation, and the weighted sum do for larger batches

@@ -53,6 +53,8 @@ SIGNATURES = {
     "kbn_silu_mul_quant_mxfp4": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr]),
     "kbn_dequant_mxfp4": (_i32, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _ptr]),
     "kbn_pack_mxfp4_scales": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _ptr]),
+    "kbn_mxfp4_gemm_nt": (_i32, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr]),
+    "kbn_mxfp4_linear": (_i32, [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _ptr]),
     "kbn_moe_few_tokens_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "kbn_moe_few_tokens": (_i32, [_ptr, _i64, _i64, _ptr, _i32, _i64, _i64, _i32, _ptr, _i64, _i64, _i64, _i32, _f32, _f32, _i32, _i32, _ptr, _ptr,
                                   _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr]),

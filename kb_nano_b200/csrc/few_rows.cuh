@@ -21,6 +21,7 @@
 #pragma once
 #include "gemm_common.cuh"
 #include "mxfp4.cuh"
+#include "tensor_map.cuh"
 
 namespace kbn {
 namespace few {
@@ -323,8 +324,25 @@ __device__ __forceinline__ void load_tokens(uint8_t* tokens, uint32_t stride, in
     if (tid < n) expo[tid] = -token_exponent(max_bits[tid]);
 }
 
-// Host: ring depth for `fixed` bytes of other shared memory (0: does not fit).
-constexpr int kSmemMax = 232448;
+constexpr int kSmemMax = 232448;      // shared memory a CTA may ask for
+
+// Weight matrix [rows, K] as (chunk, row, chunk number): one box is eight rows of kChunks chunks, each chunk's eight rows
+// side by side and swizzled, so that a warp reading one chunk of eight rows touches every bank once.
+template <int FMT>
+static int weight_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K) {
+    using F = Fmt<FMT>;
+    TensorMapSpec t;
+    memset(&t, 0, sizeof(t));
+    const uint64_t row_bytes = (uint64_t)(FMT == kFp8 ? K : K / 2);
+    t.base = base;
+    t.rank = 3;
+    t.dims[0] = F::kChunkBytes; t.dims[1] = (uint64_t)rows; t.dims[2] = (uint64_t)(K / 128);
+    t.strides[0] = row_bytes; t.strides[1] = F::kChunkBytes;
+    t.box[0] = F::kChunkBytes; t.box[1] = 8; t.box[2] = F::kChunks;
+    t.swizzle = FMT == kFp8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+    return encode_tensor_map(tm, t);
+}
 
 }  // namespace few
 }  // namespace kbn

@@ -18,7 +18,6 @@
 
 #include "few_rows.cuh"
 #include "moe_route.cuh"
-#include "tensor_map.cuh"
 
 namespace kbn {
 namespace few {
@@ -316,24 +315,6 @@ static bool plan(int64_t K, int want, Plan* p) {
         return true;
     }
     return false;
-}
-
-// Weight matrix [rows, K] as (chunk, row, chunk number): one box is eight rows of kChunks chunks, each chunk's eight rows
-// side by side and swizzled, so that a warp reading one chunk of eight rows touches every bank once.
-template <int FMT>
-static int weight_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K) {
-    using F = Fmt<FMT>;
-    TensorMapSpec t;
-    memset(&t, 0, sizeof(t));
-    const uint64_t row_bytes = (uint64_t)(FMT == kFp8 ? K : K / 2);
-    t.base = base;
-    t.rank = 3;
-    t.dims[0] = F::kChunkBytes; t.dims[1] = (uint64_t)rows; t.dims[2] = (uint64_t)(K / 128);
-    t.strides[0] = row_bytes; t.strides[1] = F::kChunkBytes;
-    t.box[0] = F::kChunkBytes; t.box[1] = 8; t.box[2] = F::kChunks;
-    t.swizzle = FMT == kFp8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
-    return encode_tensor_map(tm, t);
 }
 
 template <typename Kernel>

@@ -726,3 +726,56 @@ def pack_mxfp4_scales(scale: torch.Tensor, k: int) -> torch.Tensor:
     with _on(dev):
         _lib.check(_lib.load().kbn_pack_mxfp4_scales(scale.data_ptr(), rows, k, _row_stride(scale), out.data_ptr(), _stream(scale)))
     return out
+
+
+def _check_mxfp4_weight(b_q: torch.Tensor, b_sf: torch.Tensor, k: int, dev) -> int:
+    n = b_q.shape[0]
+    _check_codes(b_q, n, k, "b_q")
+    if not b_q.is_contiguous():
+        raise ValueError("b_q must be contiguous")
+    _check_packed_mxfp4(b_sf, n, k, dev, "b_sf")
+    return n
+
+
+def _check_out(out: torch.Tensor, m: int, n: int) -> None:
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (m, n) or (out.stride(1) != 1 and n > 1):
+        raise ValueError(f"out must be bf16 [{m}, {n}], contiguous along N")
+
+
+def mxfp4_gemm_nt(a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
+                  bias: torch.Tensor | None = None) -> None:
+    """out bf16 [M,N] = MXFP4 a_q [M,K/2] times MXFP4 b_q [N,K/2], transposed (+ bias, in fp32, before the rounding).  a_sf and
+    b_sf are the packed scales (quant_mxfp4's packed_sf, pack_mxfp4_scales)."""
+    dev = _cuda(a_q, a_sf, b_q, b_sf, out)
+    if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[1] or a_q.shape[1] % 16:
+        raise ValueError(f"a_q and b_q must be [M, K/2] and [N, K/2] with K a multiple of {MX_BLOCK}, got {tuple(a_q.shape)} and {tuple(b_q.shape)}")
+    m, k = a_q.shape[0], a_q.shape[1] * 2
+    _check_codes(a_q, m, k, "a_q")
+    if not a_q.is_contiguous():
+        raise ValueError("a_q must be contiguous")
+    _check_packed_mxfp4(a_sf, m, k, dev, "a_sf")
+    n = _check_mxfp4_weight(b_q, b_sf, k, dev)
+    _check_out(out, m, n)
+    with _on(dev):
+        _lib.check(_lib.load().kbn_mxfp4_gemm_nt(a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(), _bias_ptr(bias, n, dev), out.data_ptr(),
+                                                 _row_stride(out), m, n, k, _stream(out)))
+
+
+def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
+                 bias: torch.Tensor | None = None) -> None:
+    """The MXFP4 linear layer: x bf16 [M,K], quantised as quant_mxfp4 does, times b_q [N,K/2] / b_sf (packed) into out bf16
+    [M,N].  a_q uint8 [M,K/2] and a_sf (packed_mxfp4_bytes(M, K) bytes) are scratch for the quantised rows; up to eight rows
+    are quantised inside the one kernel that multiplies them and leave the scratch untouched."""
+    dev = _cuda(x, a_q, a_sf, b_q, b_sf, out)
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1 or x.shape[1] % MX_BLOCK:
+        raise ValueError(f"x must be bf16 [M,K], contiguous along K, K a multiple of {MX_BLOCK}, got {x.dtype} {tuple(x.shape)}")
+    m, k = x.shape
+    _check_codes(a_q, m, k, "a_q")
+    if not a_q.is_contiguous():
+        raise ValueError("a_q must be contiguous")
+    _check_packed_mxfp4(a_sf, m, k, dev, "a_sf")
+    n = _check_mxfp4_weight(b_q, b_sf, k, dev)
+    _check_out(out, m, n)
+    with _on(dev):
+        _lib.check(_lib.load().kbn_mxfp4_linear(x.data_ptr(), _row_stride(x), m, k, a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(),
+                                                _bias_ptr(bias, n, dev), out.data_ptr(), _row_stride(out), n, _stream(x)))

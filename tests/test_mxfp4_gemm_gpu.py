@@ -1,0 +1,224 @@
+"""The MXFP4 GEMM and linear layer against products in 64 bits: one row to several thousand, ragged N and K, every scheduling
+form (weight stream, split K over a cluster, persistent pairs), bias, extreme scales, strides, graphs, and an MLP."""
+import pytest
+import torch
+
+from tests import mx_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def operand(rows, k, gen, dev, spread=4):
+    q = torch.randint(0, 256, (rows, k // 2), generator=gen, device=dev, dtype=torch.uint8)
+    s = torch.randint(127 - spread, 127 + spread, (rows, k // 32), generator=gen, device=dev, dtype=torch.uint8)
+    return q, s
+
+
+def check(got, a, b, bias=None):
+    """|error| <= half a bf16 step of the result + the fp32 sum's error: (K + 16) * 2^-22 of the sum of magnitudes.  2^-22, four
+    times fp32's half step, because the tensor core adds its products in groups with fewer guard bits than one fp32 add."""
+    want = a @ b.t() + (bias.double() if bias is not None else 0.0)
+    mag = a.abs() @ b.abs().t() + (bias.double().abs() if bias is not None else 0.0)
+    err = want.abs() * 2.0**-8 + mag * (a.shape[1] + 16) * 2.0**-22 + 1e-37
+    d = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert float((d / err).max()) <= 1.0
+
+
+SHAPES = [(1, 8, 32), (1, 1, 128), (3, 24, 160), (9, 17, 64), (16, 256, 256), (77, 2056, 1440), (128, 512, 4096), (129, 300, 544), (200, 4096, 7168),
+          (256, 256, 2048), (512, 4096, 7168), (1000, 7168, 2048), (1023, 1000, 96), (2500, 3000, 416), (4096, 5120, 512)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_gemm(cuda_dev, m, n, k, with_bias):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(m * 7 + n + k)
+    aq, asc = operand(m, k, gen, cuda_dev)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bias = torch.randn(n, generator=gen, device=cuda_dev).to(torch.bfloat16) if with_bias else None
+    out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device=cuda_dev)
+    ops.mxfp4_gemm_nt(aq, ops.pack_mxfp4_scales(asc, k), bq, ops.pack_mxfp4_scales(bsc, k), out, bias)
+    check(out, ref.values(aq, asc), ref.values(bq, bsc), bias)
+    again = torch.empty_like(out)
+    ops.mxfp4_gemm_nt(aq, ops.pack_mxfp4_scales(asc, k), bq, ops.pack_mxfp4_scales(bsc, k), again, bias)
+    assert torch.equal(out, again)
+    assert ops.gemm_status(cuda_dev) == 0
+
+
+def linear(x, bq, bsf, n, bias=None, out=None):
+    from kb_nano_b200 import ops
+    m, k = x.shape
+    aq = torch.empty(m, k // 2, dtype=torch.uint8, device=x.device)
+    asf = torch.empty(ops.packed_mxfp4_bytes(m, k), dtype=torch.uint8, device=x.device)
+    out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device=x.device) if out is None else out
+    ops.mxfp4_linear(x, aq, asf, bq, bsf, out, bias)
+    return out
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 7168), (1, 8, 128), (2, 40, 256), (5, 1, 384), (7, 2056, 1152), (8, 4096, 7168), (8, 24, 8192), (8, 64, 14336), (4, 100, 96),
+                                   (9, 512, 512), (33, 136, 1440), (300, 777, 640)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_linear(cuda_dev, m, n, k, with_bias):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(m + n + k)
+    x = torch.randn(m, k, generator=gen, device=cuda_dev) * torch.exp2(torch.randint(-6, 6, (m, k // 32), generator=gen, device=cuda_dev).float()).repeat_interleave(32, 1)
+    x = x.to(torch.bfloat16)
+    x[0, :32] = 0
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bias = torch.randn(n, generator=gen, device=cuda_dev).to(torch.bfloat16) if with_bias else None
+    out = linear(x, bq, ops.pack_mxfp4_scales(bsc, k), n, bias)
+    check(out, ref.values(*ref.quant(x)), ref.values(bq, bsc), bias)
+    assert ops.gemm_status(cuda_dev) == 0
+
+
+@pytest.mark.parametrize("m", [2, 40])
+def test_scales_at_the_ends_of_the_range(cuda_dev, m):
+    """Tiny activations on huge weights and the reverse: results of ordinary size from scales near both ends."""
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(3)
+    n, k = 48, 256
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    for shift in (-90, 90):
+        x = (torch.randn(m, k, generator=gen, device=cuda_dev) * 2.0**-shift).to(torch.bfloat16)
+        s = (bsc.to(torch.int32) + shift).to(torch.uint8)
+        check(linear(x, bq, ops.pack_mxfp4_scales(s, k), n), ref.values(*ref.quant(x)), ref.values(bq, s))
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_non_finite_rows_and_weights(cuda_dev, m):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(4)
+    n, k = 64, 256
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    x = torch.randn(m, k, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    clean = linear(x, bq, ops.pack_mxfp4_scales(bsc, k), n)
+    x[1, 70] = float("inf")
+    bsc[5, 3] = 255
+    got = linear(x, bq, ops.pack_mxfp4_scales(bsc, k), n)
+    assert torch.isnan(got[1]).all() and torch.isnan(got[:, 5]).all()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[1] = False
+    keep[:, 5] = False
+    assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("m,n", [(3, 72), (40, 72), (300, 1000)])
+def test_strided_rows_in_and_out(cuda_dev, m, n):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(5)
+    k = 256
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bsf = ops.pack_mxfp4_scales(bsc, k)
+    wide = torch.randn(m, k + 13, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    for off in (0, 3, 8):
+        x = wide[:, off:off + k]
+        want = linear(x.contiguous(), bq, bsf, n)
+        big = torch.full((m, n + 9), 7.0, dtype=torch.bfloat16, device=cuda_dev)
+        linear(x, bq, bsf, n, out=big[:, 4:4 + n])
+        assert torch.equal(big[:, 4:4 + n], want) and (big[:, :4] == 7).all() and (big[:, 4 + n:] == 7).all()
+
+
+def test_weights_written_just_before(cuda_dev):
+    """Nothing may be read before the kernel in front has finished: operands, scales and weights made right before the product."""
+    from kb_nano_b200 import ops
+    m, n, k = 40, 4096, 4096
+    gen = torch.Generator(device=cuda_dev).manual_seed(6)
+    for rows in (m, 4):
+        x = torch.randn(rows, k, generator=gen, device=cuda_dev).to(torch.bfloat16)
+        w = torch.randn(2, n, k, generator=gen, device=cuda_dev).to(torch.bfloat16)
+        bq = torch.empty(n, k // 2, dtype=torch.uint8, device=cuda_dev)
+        bsf = torch.empty(ops.packed_mxfp4_bytes(n, k), dtype=torch.uint8, device=cuda_dev)
+        aq = torch.empty(rows, k // 2, dtype=torch.uint8, device=cuda_dev)
+        asf = torch.empty(ops.packed_mxfp4_bytes(rows, k), dtype=torch.uint8, device=cuda_dev)
+        outs = [[], []]
+        for r in range(6):
+            o = torch.empty(rows, n, dtype=torch.bfloat16, device=cuda_dev)
+            ops.quant_mxfp4(x, aq, packed_sf=asf)
+            ops.quant_mxfp4(w[r & 1], bq, packed_sf=bsf)
+            if rows > 8:
+                ops.mxfp4_gemm_nt(aq, asf, bq, bsf, o)
+            else:
+                ops.mxfp4_linear(x, aq, asf, bq, bsf, o)
+            outs[r & 1].append(o)
+        for j in range(2):
+            assert all(torch.equal(o, outs[j][0]) for o in outs[j])
+            check(outs[j][0], ref.values(*ref.quant(x)), ref.values(*ref.quant(w[j])))
+
+
+def test_mlp_of_two_linears_and_the_activation_in_a_graph(cuda_dev):
+    """quantise -> gate|up product -> SiLU*up and quantise -> down product, eager and replayed, on its own stream."""
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(7)
+    h, i = 512, 384
+    w13, s13 = operand(2 * i, h, gen, cuda_dev, spread=2)
+    w2, s2 = operand(h, i, gen, cuda_dev, spread=2)
+    s13 -= 6
+    s2 -= 6
+    p13, p2 = ops.pack_mxfp4_scales(s13, h), ops.pack_mxfp4_scales(s2, i)
+    for m in (1, 8, 100):
+        x = torch.randn(m, h, generator=gen, device=cuda_dev).to(torch.bfloat16)
+        aq, asf = torch.empty(m, h // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(ops.packed_mxfp4_bytes(m, h), dtype=torch.uint8, device=cuda_dev)
+        yq, ysf = torch.empty(m, i // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(ops.packed_mxfp4_bytes(m, i), dtype=torch.uint8, device=cuda_dev)
+        ys = torch.empty(m, i // 32, dtype=torch.uint8, device=cuda_dev)
+        gu, out = torch.empty(m, 2 * i, dtype=torch.bfloat16, device=cuda_dev), torch.empty(m, h, dtype=torch.bfloat16, device=cuda_dev)
+
+        def mlp():
+            ops.mxfp4_linear(x, aq, asf, w13, p13, gu)
+            ops.silu_mul_quant_mxfp4(gu, yq, ys, ysf)
+            ops.mxfp4_gemm_nt(yq, ysf, w2, p2, out)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            mlp()
+        torch.cuda.current_stream().wait_stream(side)
+        check(gu, ref.values(*ref.quant(x)), ref.values(w13, s13))
+        g, u = gu.double().chunk(2, dim=1)
+        cw, sw = ref.quant(ref.bf16_round(ref.bf16_round(g * torch.sigmoid(g)) * u))
+        assert torch.equal(yq, cw) and torch.equal(ys, sw)
+        check(out, ref.values(yq, ys), ref.values(w2, s2))
+        want = out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            mlp()
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_no_rows_or_columns(cuda_dev):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(8)
+    bq, bsc = operand(16, 64, gen, cuda_dev)
+    assert linear(torch.empty(0, 64, dtype=torch.bfloat16, device=cuda_dev), bq, ops.pack_mxfp4_scales(bsc, 64), 16).shape == (0, 16)
+    assert linear(torch.ones(3, 64, dtype=torch.bfloat16, device=cuda_dev), bq[:0], ops.pack_mxfp4_scales(bsc[:0], 64), 0).shape == (3, 0)
+
+
+def test_refusals(cuda_dev):
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(9)
+    m, n, k = 4, 16, 64
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda_dev)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bsf = ops.pack_mxfp4_scales(bsc, k)
+    aq, asf = torch.empty(m, k // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(ops.packed_mxfp4_bytes(m, k), dtype=torch.uint8, device=cuda_dev)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=cuda_dev)
+    with pytest.raises(ValueError, match="bf16"):
+        ops.mxfp4_linear(x.half(), aq, asf, bq, bsf, out)
+    with pytest.raises(ValueError, match="b_q"):
+        ops.mxfp4_linear(x, aq, asf, bq[:, :16], bsf, out)
+    with pytest.raises(ValueError, match="b_sf"):
+        ops.mxfp4_linear(x, aq, asf, bq, bsf[:-16], out)
+    with pytest.raises(ValueError, match="a_sf"):
+        ops.mxfp4_linear(x, aq, asf[16:], bq, bsf, out)
+    with pytest.raises(ValueError, match="out must be"):
+        ops.mxfp4_linear(x, aq, asf, bq, bsf, out.float())
+    with pytest.raises(ValueError, match="bias"):
+        ops.mxfp4_linear(x, aq, asf, bq, bsf, out, torch.zeros(n, device=cuda_dev))
+    with pytest.raises(ValueError, match="multiple of 32"):
+        ops.mxfp4_gemm_nt(aq[:, :24].contiguous(), asf, bq[:, :24].contiguous(), bsf, out)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ops.mxfp4_gemm_nt(aq.cpu(), asf, bq, bsf, out)
