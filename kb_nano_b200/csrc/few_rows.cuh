@@ -17,7 +17,9 @@
 //              and 32 K-values, applied to each 32-K partial sum.  Both in fp32, so any scale works.
 //   K order    a dot product does not care: lane t of a quad takes 16 consecutive K-values of a row per load (FP8) or
 //              eight (MXFP4), and reads the same K-values of its token.
-//   sums       fp32; the warps' partial results meet in shared memory and are added in warp order (bit-reproducible).
+//   sums       fp32; the warps' partial results meet in shared memory, where two finisher warps (one per buffer, every other
+//              unit) add them in warp order (bit-reproducible) and do what the unit's results need, so that no consumer
+//              waits for a store, a fence or another consumer.
 #pragma once
 #include "gemm_common.cuh"
 #include "mxfp4.cuh"
@@ -28,8 +30,9 @@ namespace few {
 
 enum WeightFormat : int { kFp8 = 0, kMxfp4 = 1 };
 
-constexpr int kConsumerWarps = 16;
-constexpr int kThreads = 32 * (kConsumerWarps + 1);      // consumers first, then the producer warp
+constexpr int kConsumerWarps = 16, kFinishers = 2;
+constexpr int kProducerWarp = kConsumerWarps, kFirstFinisher = kConsumerWarps + 1;
+constexpr int kThreads = 32 * (kConsumerWarps + 1 + kFinishers);
 constexpr int kStageBytes = 16384;                        // two boxes of 8 KB
 constexpr int kMaxGroup = 8;                              // tokens per job: the N of the matrix instruction
 constexpr int kMaxTokens = 16, kMaxTopk = 16, kMaxPairs = kMaxTokens * kMaxTopk;
@@ -60,8 +63,8 @@ struct Smem {
     uint8_t* ring;         // stages, 1024-byte aligned
     uint8_t* scales;       // one area per stage
     uint8_t* tokens;       // f16 rows, stride token_stride
-    float* red;            // two buffers of 16 warps x 128 partial sums
-    uint64_t* bars;        // full[stages], empty[stages]
+    float* red;            // one buffer of 16 warps x 128 partial sums per finisher
+    uint64_t* bars;        // full[stages], empty[stages], partials full[kFinishers], partials empty[kFinishers]
     int32_t stages;
 };
 
@@ -120,6 +123,10 @@ __device__ __forceinline__ void init_ring(const Smem& s, int arrivals) {
     for (int i = 0; i < s.stages; ++i) {
         ptx::mbar_init(ptx::smem_u32(s.bars + i), 1 + 32);                    // the producer's bytes, its 32 lanes' scale copies
         ptx::mbar_init(ptx::smem_u32(s.bars + s.stages + i), (uint32_t)arrivals);
+    }
+    for (int i = 0; i < kFinishers; ++i) {
+        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + i), kConsumerWarps);
+        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + i), 1);
     }
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
@@ -236,19 +243,30 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
     }
 }
 
-// Adds up a unit's 16 partial results: element (row of 16) * 8 + token of buffer `buf`.
-__device__ __forceinline__ void store_partials(const Smem& s, int buf, int warp, int lane, const float (&acc)[4]) {
+// Consumer warp: its partial sums of the CTA's u-th unit to the finisher u % kFinishers; element (row of 16) * 8 + token.
+__device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, int lane, const float (&acc)[4], const WaitCtx& w) {
+    const int buf = (int)(u % kFinishers);
+    wait_bar(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf), (uint32_t)(u / kFinishers & 1) ^ 1u, w);
     float* r = s.red + (buf * kConsumerWarps + warp) * 128;
     const int g = lane >> 2, t = lane & 3;
     *reinterpret_cast<float2*>(r + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
     *reinterpret_cast<float2*>(r + (g + 8) * 8 + 2 * t) = make_float2(acc[2], acc[3]);
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + buf));
 }
-__device__ __forceinline__ float sum_partials(const Smem& s, int buf, int element) {
-    const float* r = s.red + buf * kConsumerWarps * 128 + element;
-    float v = 0.f;
+// Finisher warp u % kFinishers: the sums of the CTA's u-th unit.  Lane l receives row l / 2, tokens 4 (l % 2) .. + 3.
+__device__ __forceinline__ void take_over(const Smem& s, int64_t u, int lane, float (&v)[4], const WaitCtx& w) {
+    const int buf = (int)(u % kFinishers);
+    wait_bar(ptx::smem_u32(s.bars + 2 * s.stages + buf), (uint32_t)(u / kFinishers & 1), w);
+    const float4* r = reinterpret_cast<const float4*>(s.red + buf * kConsumerWarps * 128) + lane;
+    v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kConsumerWarps; ++i) v += r[i * 128];
-    return v;
+    for (int i = 0; i < kConsumerWarps; ++i) {
+        const float4 p = r[i * 32];
+        v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+    }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf));
 }
 
 // x * 2^e for |e| up to 254, in two exact steps (one factor alone may leave fp32's range).
@@ -266,7 +284,7 @@ __device__ __forceinline__ int token_exponent(uint32_t amax_bits) {
 
 // A few f16 rows of K values into shared memory from fp32 or bf16 rows in global memory, normalised as described above, by
 // all consumer threads.  row_ptr(i): row i < n.  expo[i] receives the exponent to take out again.  max_bits: n words.
-// The caller has synchronised the consumers since the last use of the rows; a consumer_sync() must follow.
+// Begins with a barrier of the consumers (all have read the rows that are replaced); a consumer_sync() must follow.
 template <typename T, typename RowPtr>
 __device__ __forceinline__ void load_tokens(uint8_t* tokens, uint32_t stride, int n, int K, RowPtr row_ptr, uint32_t* max_bits, int* expo, int tid) {
     const int vecs = K / 8;                       // K % 128 == 0: sixteen consecutive threads share a row

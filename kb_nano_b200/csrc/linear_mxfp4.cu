@@ -12,7 +12,7 @@
 namespace kbn {
 namespace few {
 
-constexpr int kRedBytes = 2 * kConsumerWarps * 128 * 4;
+constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
 constexpr int kLinearFixed = 1024 + kRedBytes + 256 + 128;      // alignment, partial sums, barriers, row exponents and flag
 
 struct LinearArgs {
@@ -112,29 +112,33 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
 
     const int32_t units = (a.N + 15) / 16, KC = a.K / 128;
     const int32_t u0 = (int32_t)((int64_t)units * blockIdx.x / gridDim.x), u1 = (int32_t)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
-    RingPos pos;
-    if (warp == kConsumerWarps) {
+    if (warp == kProducerWarp) {
         const WaitCtx w{abort_flag, a.status, 17};
+        RingPos pos;
         for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4>(s, pos, &tm, a.s, 16 * u, 16 * u + 8, a.N, KC, lane, w);
-    } else {
+    } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
+        RingPos pos;
         quantise_tokens(s.tokens, (uint32_t)a.token_stride, a, vec != 0, b_max, tid);
         consumer_sync();
         const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, a.M - 1) * (uint32_t)a.token_stride;
         for (int32_t u = u0; u < u1; ++u) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             consume_unit<kMxfp4>(s, pos, KC, warp, lane, token_row, acc, w);
-            const int buf = (u - u0) & 1;
-            store_partials(s, buf, warp, lane, acc);
-            consumer_sync();
-            const int j = tid - 128 * ((u - u0) & 3);      // four warps finish the unit, in turn
-            if (j >= 0 && j < 128) {
-                const int tok = j >> 4, r = j & 15, n = 16 * u + r;
-                if (tok < a.M && n < a.N) {
-                    float v = scale_pow2(sum_partials(s, buf, r * 8 + tok), (int)b_max[tok] - 127 - 13);
-                    if (a.bias != nullptr) v += __bfloat162float(a.bias[n]);
-                    a.C[(int64_t)tok * a.ldc + n] = __float2bfloat16_rn(v);
-                }
+            hand_over(s, u - u0, warp, lane, acc, w);
+        }
+    } else {
+        const WaitCtx w{abort_flag, a.status, 21};
+        for (int32_t u = u0 + warp - kFirstFinisher; u < u1; u += kFinishers) {
+            float v[4];
+            take_over(s, u - u0, lane, v, w);          // the row exponents were there before the first partial sum
+            const int n = 16 * u + (lane >> 1), tok0 = 4 * (lane & 1);
+            if (n < a.N) {
+                const float bias = a.bias != nullptr ? __bfloat162float(a.bias[n]) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (tok0 + i < a.M)
+                        a.C[(int64_t)(tok0 + i) * a.ldc + n] = __float2bfloat16_rn(scale_pow2(v[i], (int)b_max[tok0 + i] - 127 - 13) + bias);
             }
         }
     }

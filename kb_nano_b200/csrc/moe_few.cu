@@ -53,13 +53,13 @@ struct Scratch {                   // small shared-memory state beside the ring
     int32_t id[kMaxPairs];
     int32_t leader[kMaxPairs];
     uint32_t max_bits[kMaxGroup];
-    int expo[kMaxGroup];
+    int expo[2][kMaxGroup];        // by the job's parity: a finisher may be a unit or two behind the consumers
     int abort_flag;
 };
 
 __host__ __device__ constexpr int scratch_bytes() { return (int)((sizeof(Scratch) + 127) / 128 * 128); }
-constexpr int kRedBytes = 2 * kConsumerWarps * 128 * 4;
-constexpr int kBarBytes = 2 * kMaxStages * 8;
+constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
+constexpr int kBarBytes = (2 * kMaxStages + 2 * kFinishers) * 8;
 
 template <int FMT>
 __device__ __forceinline__ Smem carve(uint8_t* raw, int stages, int group, int token_stride, Scratch** scratch) {
@@ -169,23 +169,24 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
     const int32_t blocks = a.I / 8, KC = a.H / 128;
     const int64_t units = (int64_t)sc.jobs.n_jobs * blocks;
     const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    RingPos pos;
-    if (warp == kConsumerWarps) {
+    int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+    if (warp == kProducerWarp) {
         const WaitCtx w{&sc.abort_flag, a.status, 8};
-        int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+        RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * 2 * a.I + 8 * rb;
             produce_unit<FMT>(s, pos, &tm, a.s13, row, row + a.I, 2 * a.I * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
-    } else {
+    } else if (warp < kConsumerWarps) {
         const WaitCtx w{&sc.abort_flag, a.status, 9};
-        int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks), loaded = -1;
+        RingPos pos;
+        int32_t loaded = -1;
         for (int64_t u = u0; u < u1; ++u) {
             const int count = sc.jobs.count[job];
             if (job != loaded) {
                 load_tokens<__nv_bfloat16>(s.tokens, (uint32_t)a.token_stride, count, a.H,
-                                           [&](int i) { return a.x + (int64_t)(sc.jobs.pair[job][i] / a.topk) * a.ld_x; }, sc.max_bits, sc.expo, tid);
+                                           [&](int i) { return a.x + (int64_t)(sc.jobs.pair[job][i] / a.topk) * a.ld_x; }, sc.max_bits, sc.expo[job & 1], tid);
                 consumer_sync();
                 loaded = job;
             }
@@ -193,20 +194,45 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
             const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, count - 1) * (uint32_t)a.token_stride;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             consume_unit<FMT>(s, pos, KC, warp, lane, token_row, acc, w);
-            const int buf = (int)((u - u0) & 1);
-            store_partials(s, buf, warp, lane, acc);
-            consumer_sync();
-            const int j = tid - 64 * (int)((u - u0) & 7);      // two warps finish the unit, in turn
-            if (j >= 0 && j < 64 && (j >> 3) < count) {
-                const int tok = j >> 3, r = j & 7, e = sc.expo[tok];
-                const float g = scale_pow2(sum_partials(s, buf, r * 8 + tok), e), up = scale_pow2(sum_partials(s, buf, (r + 8) * 8 + tok), e);
-                a.y[(int64_t)sc.jobs.pair[job][tok] * a.I + 8 * rb + r] = __fdiv_rn(g, 1.0f + expf(-g)) * up;
+            hand_over(s, u - u0, warp, lane, acc, w);
+            if (++rb == blocks) rb = 0, ++job;
+        }
+    } else {
+        const WaitCtx w{&sc.abort_flag, a.status, 19};
+        for (int64_t u = u0; u < u1; ++u) {
+            if ((u - u0) % kFinishers == warp - kFirstFinisher) {
+                float v[4];
+                take_over(s, u - u0, lane, v, w);
+                const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float other = __shfl_down_sync(0xffffffffu, v[i], 16);      // rows 8-15 are the up projection's
+                    if (lane < 16 && tok0 + i < count) {
+                        const int e = sc.expo[job & 1][tok0 + i];
+                        const float g = scale_pow2(v[i], e), up = scale_pow2(other, e);
+                        a.y[(int64_t)sc.jobs.pair[job][tok0 + i] * a.I + 8 * rb + (lane >> 1)] = __fdiv_rn(g, 1.0f + expf(-g)) * up;
+                    }
+                }
             }
             if (++rb == blocks) rb = 0, ++job;
         }
     }
     drain_after_abort(&sc.abort_flag);
 }
+
+// out[:, 16 rb .. + 15]: each token's rows with their router weights, in slot order, by one warp.
+__device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, int rb, int lane) {
+    const int col = 16 * rb + (lane & 15);
+    for (int t = lane >> 4; t < a.T; t += 2) {
+        float v = 0.f;
+        const float* rp = a.rows + (int64_t)t * a.topk * a.H + col;
+#pragma unroll 8
+        for (int k = 0; k < a.topk; ++k) v = fmaf(weight[t * a.topk + k], __ldcg(rp + (int64_t)k * a.H), v);
+        a.out[(int64_t)t * a.ld_out + col] = __float2bfloat16_rn(v);
+    }
+}
+
+constexpr int kCountBatch = 4;
 
 template <int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -239,53 +265,56 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
     }
     const int64_t units = (int64_t)n_jobs * blocks;
     const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    RingPos pos;
-    if (warp == kConsumerWarps) {
+    int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+    if (warp == kProducerWarp) {
         const WaitCtx w{&sc.abort_flag, a.status, 10};
-        int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+        RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * a.H + 16 * rb;
             produce_unit<FMT>(s, pos, &tm, a.s2, row, row + 8, a.H * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
-    } else {
+    } else if (warp < kConsumerWarps) {
         const WaitCtx w{&sc.abort_flag, a.status, 11};
-        int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks), loaded = -1;
+        RingPos pos;
+        int32_t loaded = -1;
         for (int64_t u = u0; u < u1; ++u) {
             const int count = sc.jobs.count[job];
             if (job != loaded) {
                 load_tokens<float>(s.tokens, (uint32_t)a.token_stride, count, a.I,
-                                   [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I; }, sc.max_bits, sc.expo, tid);
+                                   [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I; }, sc.max_bits, sc.expo[job & 1], tid);
                 consumer_sync();
                 loaded = job;
             }
             const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, count - 1) * (uint32_t)a.token_stride;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             consume_unit<FMT>(s, pos, KC, warp, lane, token_row, acc, w);
-            const int buf = (int)((u - u0) & 1);
-            store_partials(s, buf, warp, lane, acc);
-            consumer_sync();
-            const int j = tid - 128 * (int)((u - u0) & 3);     // four warps finish the unit, in turn
-            if (j >= 0 && j < 128) {
-                const int tok = j >> 4, r = j & 15;
-                if (tok < count)
-                    a.rows[(int64_t)sc.jobs.pair[job][tok] * a.H + 16 * rb + r] = scale_pow2(sum_partials(s, buf, r * 8 + tok), sc.expo[tok]);
-                // the warp that completes the column block (four warps of every job) adds the rows up
+            hand_over(s, u - u0, warp, lane, acc, w);
+            if (++rb == blocks) rb = 0, ++job;
+        }
+    } else {
+        const WaitCtx w{&sc.abort_flag, a.status, 20};
+        int pending = 0, mine = 0;            // column blocks stored but not yet counted; lane i holds the i-th
+        for (int64_t u = u0; u < u1; ++u) {
+            if ((u - u0) % kFinishers == warp - kFirstFinisher) {
+                float v[4];
+                take_over(s, u - u0, lane, v, w);
+                const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (tok0 + i < count)
+                        a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + 16 * rb + (lane >> 1)] = scale_pow2(v[i], sc.expo[job & 1][tok0 + i]);
+                if (lane == pending) mine = rb;
+                ++pending;
+            }
+            // One fence and one round of counting for several units.  Who completes a column block (every job once) adds it up.
+            if (pending == kCountBatch || (pending > 0 && u + kFinishers >= u1)) {
                 __threadfence();
                 __syncwarp();
-                int last = 0;
-                if (lane == 0) last = atomicAdd(a.counters + rb, 1) == 4 * n_jobs - 1;
-                if (__shfl_sync(0xffffffffu, last, 0)) {
-                    __threadfence();
-                    const int col = 16 * rb + (lane & 15);
-                    for (int t = lane >> 4; t < a.T; t += 2) {
-                        float v = 0.f;
-                        const float* rp = a.rows + (int64_t)t * a.topk * a.H + col;
-#pragma unroll 8
-                        for (int k = 0; k < a.topk; ++k) v = fmaf(sc.jobs.weight[t * a.topk + k], __ldcg(rp + (int64_t)k * a.H), v);
-                        a.out[(int64_t)t * a.ld_out + col] = __float2bfloat16_rn(v);
-                    }
-                }
+                unsigned last = __ballot_sync(0xffffffffu, lane < pending && atomicAdd(a.counters + mine, 1) == n_jobs - 1);
+                if (last) __threadfence();
+                for (; last; last &= last - 1) add_up(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
+                pending = 0;
             }
             if (++rb == blocks) rb = 0, ++job;
         }
