@@ -10,9 +10,10 @@
 //   product    mma.sync.m16n8k16, f16 x f16 -> fp32: the 16 weight rows are its M, the tokens its N.  (tcgen05 would spend a
 //              128-row tile on them and needs its operands in fp8 or fp4; at this intensity the legacy instruction is far
 //              from being the bound.)  e4m3 and e2m1 codes are converted to f16 exactly, two per instruction.
-//   tokens     held in shared memory as f16, each row multiplied by a power of two that brings its largest magnitude into
-//              [2^14, 2^15); the power is taken out again after the sum.  bf16 has 8 significant bits and f16 has 11, so a
-//              value is kept exactly down to 2^-32 of the row's largest, and below that to within 2^-40 of it.
+//   tokens     held in shared memory as f16, each 128 K-values of a row multiplied by a power of two that brings their
+//              largest magnitude into [2^14, 2^15); the power is taken out of the chunk's partial sum.  bf16 has 8 significant
+//              bits and f16 has 11, so a value is kept exactly down to 2^-32 of its chunk's largest, and below that to within
+//              2^-40 of it.  One power per chunk, not per row, so that a row is converted in one pass, without a barrier.
 //   scales     FP8: one fp32 factor per 128 x 128 block, applied to each 128-K partial sum.  MXFP4: one power of two per row
 //              and 32 K-values, applied to each 32-K partial sum.  Both in fp32, so any scale works.
 //   K order    a dot product does not care: lane t of a quad takes 16 consecutive K-values of a row per load (FP8) or
@@ -53,16 +54,16 @@ struct Fmt<kMxfp4> {
 };
 
 // Where a weight matrix's scales lie.  FP8: fp32 [rows / 128, KC].  MXFP4: one 32-bit word per row and chunk, row-major
-// (packed == 0: word (row, c) at row * KC + c) or in the packed layout of the tensor core.
+// (word (row, c) at row * KC + c) or, PACKED, in the packed layout of the tensor core.
 struct ScaleSource {
     const void* base;
-    int32_t packed;
 };
 
 struct Smem {
     uint8_t* ring;         // stages, 1024-byte aligned
     uint8_t* scales;       // one area per stage
     uint8_t* tokens;       // f16 rows, stride token_stride
+    float* token_scales;   // [rows, K / 128]: what a chunk's partial sum is multiplied by
     float* red;            // one buffer of 16 warps x 128 partial sums per finisher
     uint64_t* bars;        // full[stages], empty[stages], partials full[kFinishers], partials empty[kFinishers]
     int32_t stages;
@@ -134,7 +135,7 @@ __device__ __forceinline__ void init_ring(const Smem& s, int arrivals) {
 
 // Producer warp: all stages of one unit.  row_a, row_b: first rows of the two boxes (in rows of the tensor map; a box past
 // the last row is filled with zeros by the TMA).  n_rows: rows the scale array covers.
-template <int FMT>
+template <int FMT, bool PACKED = false>
 __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const void* tmap, const ScaleSource& sc, int32_t row_a, int32_t row_b,
                                              int32_t n_rows, int32_t KC, int lane, const WaitCtx& w) {
     using F = Fmt<FMT>;
@@ -156,21 +157,30 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
                 cp_async4(sdst + lane * 4, static_cast<const float*>(sc.base) + (int64_t)(row >> 7) * KC + c);
             }
         } else {
-            // word (chunk, row of 16) at (chunk * 16 + row) * 4: eight words per lane
-            const int32_t r = lane & 15;
+            // word (chunk, row of 16) at (chunk * 16 + row) * 4: eight words per lane, two chunks apart
+            const int32_t r = lane & 15, c = c0 + (lane >> 4);
             const int32_t row = min((r < 8 ? row_a : row_b - 8) + r, n_rows - 1);
-            const uint32_t* base = static_cast<const uint32_t*>(sc.base);
+            const uint32_t* src = static_cast<const uint32_t*>(sc.base) + (PACKED ? (int64_t)mxfp4::packed_word(row, c, KC) : (int64_t)row * KC + c);
+            const uint32_t sl = sdst + (uint32_t)lane * 4u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int32_t c = c0 + 2 * i + (lane >> 4);
-                if (c < KC)
-                    cp_async4(sdst + (uint32_t)((2 * i + (lane >> 4)) * 16 + r) * 4u,
-                              base + (sc.packed ? (int64_t)mxfp4::packed_word(row, c, KC) : (int64_t)row * KC + c));
-            }
+            for (int i = 0; i < 8; ++i)
+                if (c + 2 * i < KC) cp_async4(sl + i * 128, src + i * (PACKED ? 256 : 2));
         }
         cp_async_arrive(full);
         pos.advance((uint32_t)s.stages);
     }
+}
+
+// What a consumer lane reads of the tokens: the f16 row of column g, the chunk scales of columns 2t and 2t + 1 (shared-memory
+// addresses).  Columns without a token repeat the last one's; nothing reads their results.
+struct TokenColumns {
+    uint32_t row, scale0, scale1;
+};
+template <typename RowOf>
+__device__ __forceinline__ TokenColumns token_columns(const Smem& s, uint32_t stride, int32_t KC, int count, int lane, RowOf row_of) {
+    const int g = min(lane >> 2, count - 1), t0 = min(2 * (lane & 3), count - 1), t1 = min(2 * (lane & 3) + 1, count - 1);
+    return TokenColumns{ptx::smem_u32(s.tokens) + (uint32_t)row_of(g) * stride, ptx::smem_u32(s.token_scales) + (uint32_t)(row_of(t0) * KC) * 4u,
+                        ptx::smem_u32(s.token_scales) + (uint32_t)(row_of(t1) * KC) * 4u};
 }
 
 // Consumer warp: its chunks of one unit, added to acc.  acc[0..1]: row g of box 0 with tokens 2t, 2t + 1; acc[2..3]: row g of
@@ -178,8 +188,8 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
 // A slot must always have the same readers: a warp may only test a barrier for a phase if it has seen the phase before it
 // complete, because the test tells two phases apart by their parity alone.
 template <int FMT>
-__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, uint32_t token_row,
-                                             float (&acc)[4], const WaitCtx& w) {
+__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, const TokenColumns& tc, float (&acc)[4],
+                                             const WaitCtx& w) {
     using F = Fmt<FMT>;
     const int g = lane >> 2, t = lane & 3;
     const int cw = FMT == kFp8 ? (warp & 7) : warp;
@@ -193,13 +203,14 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
             const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * 8 + g) * F::kChunkBytes;
             const uint32_t box1 = box0 + kStageBytes / 2;
             const uint32_t sdst = ptx::smem_u32(s.scales) + here.slot * F::kScaleBytes;
+            const float x0s = __uint_as_float(lds32(tc.scale0 + (uint32_t)c * 4u)), x1s = __uint_as_float(lds32(tc.scale1 + (uint32_t)c * 4u));
             if (FMT == kFp8) {
                 float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t piece = (uint32_t)(t + 4 * j);
                     const uint4 wa = lds128(box0 + ((piece ^ (uint32_t)g) << 4)), wb = lds128(box1 + ((piece ^ (uint32_t)g) << 4));
-                    const uint32_t ta = token_row + (uint32_t)(c * 128 + (int)piece * 16) * 2u;
+                    const uint32_t ta = tc.row + (uint32_t)(c * 128 + (int)piece * 16) * 2u;
                     const uint4 x0 = lds128(ta), x1 = lds128(ta + 16);
                     uint32_t a0, a1, a2, a3;
                     e4m3x4_to_f16(wa.x, a0, a2); e4m3x4_to_f16(wb.x, a1, a3);
@@ -212,30 +223,36 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
                     mma_f16_m16n8k16(q, a0, a1, a2, a3, x1.z, x1.w);
                 }
                 const float s0 = __uint_as_float(lds32(sdst + cw * 4)), s1 = __uint_as_float(lds32(sdst + 32 + cw * 4));
-                acc[0] = fmaf(p[0] + q[0], s0, acc[0]);
-                acc[1] = fmaf(p[1] + q[1], s0, acc[1]);
-                acc[2] = fmaf(p[2] + q[2], s1, acc[2]);
-                acc[3] = fmaf(p[3] + q[3], s1, acc[3]);
+                acc[0] = fmaf((p[0] + q[0]) * x0s, s0, acc[0]);
+                acc[1] = fmaf((p[1] + q[1]) * x1s, s0, acc[1]);
+                acc[2] = fmaf((p[2] + q[2]) * x0s, s1, acc[2]);
+                acc[3] = fmaf((p[3] + q[3]) * x1s, s1, acc[3]);
             } else {
                 const uint32_t sw0 = lds32(sdst + (uint32_t)(cw * 16 + g) * 4u), sw1 = lds32(sdst + (uint32_t)(cw * 16 + 8 + g) * 4u);
                 const uint32_t swz = (uint32_t)(g >> 1) & 3u;
+                const uint32_t e0[2] = {mxfp4::scale_bf16x2(sw0), mxfp4::scale_bf16x2(sw0 >> 16)}, e1[2] = {mxfp4::scale_bf16x2(sw1), mxfp4::scale_bf16x2(sw1 >> 16)};
+                float q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const uint32_t off = (((uint32_t)b ^ swz) << 4) + (uint32_t)t * 4u;
                     const uint32_t wa = lds32(box0 + off), wb = lds32(box1 + off);
-                    const uint4 x = lds128(token_row + (uint32_t)(c * 128 + b * 32 + t * 8) * 2u);
+                    const uint4 x = lds128(tc.row + (uint32_t)(c * 128 + b * 32 + t * 8) * 2u);
                     uint32_t ha[4], hb[4];
                     mxfp4::unpack_e2m1x8(wa, ha);
                     mxfp4::unpack_e2m1x8(wb, hb);
                     float p[4] = {0.f, 0.f, 0.f, 0.f};
                     mma_f16_m16n8k16(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
                     mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
-                    const float s0 = mxfp4::scale_value((sw0 >> (8 * b)) & 0xffu), s1 = mxfp4::scale_value((sw1 >> (8 * b)) & 0xffu);
-                    acc[0] = fmaf(p[0], s0, acc[0]);
-                    acc[1] = fmaf(p[1], s0, acc[1]);
-                    acc[2] = fmaf(p[2], s1, acc[2]);
-                    acc[3] = fmaf(p[3], s1, acc[3]);
+                    const float s0 = b & 1 ? bf16_hi(e0[b >> 1]) : bf16_lo(e0[b >> 1]), s1 = b & 1 ? bf16_hi(e1[b >> 1]) : bf16_lo(e1[b >> 1]);
+                    q[0] = fmaf(p[0], s0, q[0]);
+                    q[1] = fmaf(p[1], s0, q[1]);
+                    q[2] = fmaf(p[2], s1, q[2]);
+                    q[3] = fmaf(p[3], s1, q[3]);
                 }
+                acc[0] = fmaf(q[0], x0s, acc[0]);
+                acc[1] = fmaf(q[1], x1s, acc[1]);
+                acc[2] = fmaf(q[2], x0s, acc[2]);
+                acc[3] = fmaf(q[3], x1s, acc[3]);
             }
         }
         __syncwarp();
@@ -274,7 +291,7 @@ __device__ __forceinline__ float scale_pow2(float x, int e) {
     const int h = e >> 1;
     return x * __uint_as_float((uint32_t)(h + 127) << 23) * __uint_as_float((uint32_t)(e - h + 127) << 23);
 }
-// Exponent that brings a row's largest finite magnitude (fp32 bit pattern) into [2^14, 2^15); 0 for an all-zero row.
+// Exponent that brings the largest finite magnitude (fp32 bit pattern) of some values into [2^14, 2^15); 0 if all are zero.
 __device__ __forceinline__ int token_exponent(uint32_t amax_bits) {
     if (amax_bits == 0u) return 0;
     int e = (int)(amax_bits >> 23) - 127;
@@ -282,64 +299,62 @@ __device__ __forceinline__ int token_exponent(uint32_t amax_bits) {
     return 14 - e;
 }
 
-// A few f16 rows of K values into shared memory from fp32 or bf16 rows in global memory, normalised as described above, by
-// all consumer threads.  row_ptr(i): row i < n.  expo[i] receives the exponent to take out again.  max_bits: n words.
-// Begins with a barrier of the consumers (all have read the rows that are replaced); a consumer_sync() must follow.
-template <typename T, typename RowPtr>
-__device__ __forceinline__ void load_tokens(uint8_t* tokens, uint32_t stride, int n, int K, RowPtr row_ptr, uint32_t* max_bits, int* expo, int tid) {
-    const int vecs = K / 8;                       // K % 128 == 0: sixteen consecutive threads share a row
-    const int total = n * vecs;
-    if (tid < n) max_bits[tid] = 0;
-    consumer_sync();
-    auto load = [&](int i, float (&f)[8]) {
-        const int row = i / vecs, v = i - row * vecs;
-        if (sizeof(T) == 2) {
-            const uint4 u = *(reinterpret_cast<const uint4*>(row_ptr(row)) + v);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Rows of K values -> f16 rows and chunk scales in shared memory, normalised as described above, by NT threads.  T: fp32 or
+// bf16.  row_ptr(i): row i < n, 16-byte aligned.  No barrier inside: the caller sees to it that nobody reads the rows that
+// are replaced, and publishes the new ones.  BATCH loads are under way at once in every thread.
+template <typename T, int NT, typename RowPtr>
+__device__ __forceinline__ void load_tokens(const Smem& s, uint32_t stride, int n, int K, RowPtr row_ptr, int tid) {
+    constexpr int W = sizeof(T) / 2;              // 16-byte loads per eight values
+    constexpr int BATCH = 8 / W;
+    const uint32_t vecs = (uint32_t)K / 8u;       // K % 128 == 0: sixteen consecutive threads share a chunk of a row
+    const uint32_t total = (uint32_t)n * vecs;
+    const uint32_t magic = 0xffffffffu / vecs + 1u;      // i / vecs == umulhi(i, magic): i * vecs < 2^32 here
+    for (uint32_t i0 = 0; i0 < total; i0 += BATCH * NT) {
+        uint4 u[BATCH][W];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const uint32_t i = i0 + (uint32_t)(k * NT + tid), row = __umulhi(i, magic);
+            if (i < total) {
+                const uint4* p = reinterpret_cast<const uint4*>(row_ptr((int)row)) + (size_t)(i - row * vecs) * W;
+#pragma unroll
+                for (int j = 0; j < W; ++j) u[k][j] = __ldcg(p + j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) u[k][j] = make_uint4(0, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const uint32_t i = i0 + (uint32_t)(k * NT + tid), row = __umulhi(i, magic), v = i - row * vecs;
+            if (i0 + (uint32_t)(k * NT) >= total) break;      // whole warps
+            float f[8];
+            const uint32_t w[4] = {u[k][0].x, u[k][0].y, u[k][0].z, u[k][0].w}, w2[4] = {u[k][W - 1].x, u[k][W - 1].y, u[k][W - 1].z, u[k][W - 1].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f[2 * j] = bf16_lo(w[j]);
-                f[2 * j + 1] = bf16_hi(w[j]);
+                f[W == 1 ? 2 * j : j] = W == 1 ? bf16_lo(w[j]) : __uint_as_float(w[j]);
+                f[W == 1 ? 2 * j + 1 : j + 4] = W == 1 ? bf16_hi(w[j]) : __uint_as_float(w2[j]);
             }
-        } else {
-            const float4* p = reinterpret_cast<const float4*>(row_ptr(row)) + 2 * v;
-            const float4 a = __ldcg(p), b = __ldcg(p + 1);
-            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-        }
-        return row;
-    };
-    for (int i0 = 0; i0 < total; i0 += 32 * kConsumerWarps) {
-        const int i = i0 + tid;
-        uint32_t m = 0;
-        int row = 0;
-        if (i < total) {
-            float f[8];
-            row = load(i, f);
+            uint32_t m = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t b = __float_as_uint(f[j]) & 0x7fffffffu;
-                if (b < 0x7f800000u) m = max(m, b);       // infinities and NaNs keep their place, the finite values set the scale
+                m = max(m, b < 0x7f800000u ? b : 0u);         // infinities and NaNs keep their place, the finite values set the scale
+            }
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (i < total) {
+                const int e = token_exponent(m);
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __half2 p = __floats2half2_rn(scale_pow2(f[2 * j], e), scale_pow2(f[2 * j + 1], e));
+                    h[j] = *reinterpret_cast<const uint32_t*>(&p);
+                }
+                *reinterpret_cast<uint4*>(s.tokens + (size_t)row * stride + (size_t)v * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                if ((tid & 15) == 0) s.token_scales[row * (vecs >> 4) + (v >> 4)] = scale_pow2(1.0f, -e);
             }
         }
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if ((tid & 15) == 0 && i < total) atomicMax(max_bits + row, m);
     }
-    consumer_sync();
-    for (int i = tid; i < total; i += 32 * kConsumerWarps) {
-        float f[8];
-        const int row = load(i, f);
-        const int e = token_exponent(max_bits[row]);
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __half2 p = __floats2half2_rn(scale_pow2(f[2 * j], e), scale_pow2(f[2 * j + 1], e));
-            h[j] = *reinterpret_cast<const uint32_t*>(&p);
-        }
-        *reinterpret_cast<uint4*>(tokens + (size_t)row * stride + (size_t)(i - row * vecs) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-    }
-    if (tid < n) expo[tid] = -token_exponent(max_bits[tid]);
 }
 
 constexpr int kSmemMax = 232448;      // shared memory a CTA may ask for

@@ -2,8 +2,8 @@
 //
 // At most eight rows (a decode step): one launch.  Every CTA quantises the rows itself -- a few thousand values, under a
 // microsecond -- into f16 rows in shared memory and streams its share of the weight rows (few_rows.cuh).  The values are
-// the ones the quantiser would have stored: a code times 2^(b - b_max), b_max the row's largest scale byte, is exact in f16
-// down to 2^-36 of the row's largest block, and the power is taken out after the sum.
+// the ones the quantiser would have stored: a code times 2^(b - b_max), b_max the largest of the scale bytes of 128 values, is
+// exact in f16 down to 2^-36 of the largest block, and the power is taken out of the 128 values' partial sum.
 // More rows, or K no multiple of 128: the quantiser and the tensor-core GEMM.
 #include <algorithm>
 
@@ -13,7 +13,7 @@ namespace kbn {
 namespace few {
 
 constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
-constexpr int kLinearFixed = 1024 + kRedBytes + 256 + 128;      // alignment, partial sums, barriers, row exponents and flag
+constexpr int kLinearFixed = 1024 + kRedBytes + 256 + 128;      // alignment, partial sums, barriers, flag
 
 struct LinearArgs {
     const __nv_bfloat16* x;
@@ -26,58 +26,55 @@ struct LinearArgs {
     int32_t M, N, K, stages, token_stride;
 };
 
-// x rows -> MXFP4 values as f16, by all consumer threads; b_max[i]: row i's largest scale byte.  VEC: 16-byte loads.
-__device__ __forceinline__ void quantise_tokens(uint8_t* tokens, uint32_t stride, const LinearArgs& a, bool vec, uint32_t* b_max, int tid) {
-    const int vecs = a.K / 8, total = a.M * vecs;      // K % 128 == 0: sixteen consecutive threads share a row, four a block
-    auto load = [&](int i, uint32_t (&w)[4]) {
-        const int row = i / vecs, v = i - row * vecs;
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)row * a.ld_x + (int64_t)v * 8;
-        if (vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        } else {
+// x rows -> MXFP4 values as f16 and their chunk scales, by all consumer threads.
+__device__ __forceinline__ void quantise_tokens(const Smem& s, const LinearArgs& a, bool vec, int tid) {
+    constexpr int NT = 32 * kConsumerWarps, BATCH = 4;
+    const uint32_t vecs = (uint32_t)a.K / 8u, total = (uint32_t)a.M * vecs;      // sixteen consecutive threads share a chunk, four a block
+    const uint32_t magic = 0xffffffffu / vecs + 1u;      // i / vecs == umulhi(i, magic): i * vecs < 2^32 here
+    for (uint32_t i0 = 0; i0 < total; i0 += BATCH * NT) {
+        uint32_t w[BATCH][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = (uint32_t)p[2 * j] | ((uint32_t)p[2 * j + 1] << 16);
-        }
-        return row;
-    };
-    auto block_byte = [&](const uint32_t (&w)[4]) {
-        uint32_t m = mxfp4::max_u16x2(mxfp4::max_u16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), mxfp4::max_u16x2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-        m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        return mxfp4::scale_byte(max(m & 0xffffu, m >> 16));
-    };
-    if (tid < a.M) b_max[tid] = 0;
-    consumer_sync();
-    for (int i0 = 0; i0 < total; i0 += 32 * kConsumerWarps) {
-        const int i = i0 + tid;
-        uint32_t w[4] = {0, 0, 0, 0};
-        const int row = i < total ? load(i, w) : 0;
-        const uint32_t b = block_byte(w);
-        uint32_t m = b == 255u ? 0u : b;
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        if ((tid & 15) == 0 && i < total) atomicMax(b_max + row, m);
-    }
-    consumer_sync();
-    for (int i0 = 0; i0 < total; i0 += 32 * kConsumerWarps) {
-        const int i = i0 + tid;
-        uint32_t w[4] = {0, 0, 0, 0};
-        const int row = i < total ? load(i, w) : 0;
-        const uint32_t b = block_byte(w);
-        uint32_t h[4];
-        mxfp4::unpack_e2m1x8(mxfp4::quant8(w, mxfp4::inv_scale(b), b == 255u), h);
-        if (i < total) {
-            // 2^(b - b_max + 13): the largest code, 6, becomes 49152
-            const int e = max((int)b - (int)b_max[row] + 13, -126);
-            const float f = b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(e + 127) << 23);
+        for (int k = 0; k < BATCH; ++k) {
+            const uint32_t i = i0 + (uint32_t)(k * NT + tid), row = __umulhi(i, magic);
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)row * a.ld_x + (size_t)(i - row * vecs) * 8;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __half2 c = *reinterpret_cast<const __half2*>(&h[j]);
-                const __half2 r = __floats2half2_rn(__low2float(c) * f, __high2float(c) * f);
-                h[j] = *reinterpret_cast<const uint32_t*>(&r);
+            for (int j = 0; j < 4; ++j) w[k][j] = 0;
+            if (i < total) {
+                if (vec) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(p);
+                    w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[k][j] = (uint32_t)p[2 * j] | ((uint32_t)p[2 * j + 1] << 16);
+                }
             }
-            *reinterpret_cast<uint4*>(tokens + (size_t)row * stride + (size_t)(i - row * vecs) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const uint32_t i = i0 + (uint32_t)(k * NT + tid), row = __umulhi(i, magic), v = i - row * vecs;
+            if (i0 + (uint32_t)(k * NT) >= total) break;      // whole warps
+            uint32_t m = mxfp4::max_u16x2(mxfp4::max_u16x2(w[k][0] & 0x7fff7fffu, w[k][1] & 0x7fff7fffu),
+                                          mxfp4::max_u16x2(w[k][2] & 0x7fff7fffu, w[k][3] & 0x7fff7fffu));
+            m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const uint32_t b = mxfp4::scale_byte(max(m & 0xffffu, m >> 16));
+            int top = b == 255u ? 0 : (int)b;
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            uint32_t h[4];
+            mxfp4::unpack_e2m1x8(mxfp4::quant8(w[k], mxfp4::inv_scale(b), b == 255u), h);
+            if (i < total) {
+                // 2^(b - top + 13): the largest code, 6, becomes 49152
+                const float f = b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(max((int)b - top + 13, -126) + 127) << 23);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __half2 c = *reinterpret_cast<const __half2*>(&h[j]);
+                    const __half2 r = __floats2half2_rn(__low2float(c) * f, __high2float(c) * f);
+                    h[j] = *reinterpret_cast<const uint32_t*>(&r);
+                }
+                *reinterpret_cast<uint4*>(s.tokens + (size_t)row * (uint32_t)a.token_stride + (size_t)v * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                if ((tid & 15) == 0) s.token_scales[row * (vecs >> 4) + (v >> 4)] = scale_pow2(1.0f, top - 127 - 13);
+            }
         }
     }
 }
@@ -95,10 +92,10 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     p += kRedBytes;
     s.bars = reinterpret_cast<uint64_t*>(p);
     p += 256;
-    uint32_t* b_max = reinterpret_cast<uint32_t*>(p);
-    int* abort_flag = reinterpret_cast<int*>(p) + kMaxGroup;
+    int* abort_flag = reinterpret_cast<int*>(p);
     p += 128;
     s.tokens = p;
+    s.token_scales = reinterpret_cast<float*>(p + (size_t)a.M * a.token_stride);
     s.stages = a.stages;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -115,30 +112,30 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     if (warp == kProducerWarp) {
         const WaitCtx w{abort_flag, a.status, 17};
         RingPos pos;
-        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4>(s, pos, &tm, a.s, 16 * u, 16 * u + 8, a.N, KC, lane, w);
+        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, a.s, 16 * u, 16 * u + 8, a.N, KC, lane, w);
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
         RingPos pos;
-        quantise_tokens(s.tokens, (uint32_t)a.token_stride, a, vec != 0, b_max, tid);
+        quantise_tokens(s, a, vec != 0, tid);
         consumer_sync();
-        const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, a.M - 1) * (uint32_t)a.token_stride;
+        const TokenColumns columns = token_columns(s, (uint32_t)a.token_stride, KC, a.M, lane, [](int col) { return col; });
         for (int32_t u = u0; u < u1; ++u) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            consume_unit<kMxfp4>(s, pos, KC, warp, lane, token_row, acc, w);
+            consume_unit<kMxfp4>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
         }
     } else {
         const WaitCtx w{abort_flag, a.status, 21};
         for (int32_t u = u0 + warp - kFirstFinisher; u < u1; u += kFinishers) {
             float v[4];
-            take_over(s, u - u0, lane, v, w);          // the row exponents were there before the first partial sum
+            take_over(s, u - u0, lane, v, w);
             const int n = 16 * u + (lane >> 1), tok0 = 4 * (lane & 1);
             if (n < a.N) {
                 const float bias = a.bias != nullptr ? __bfloat162float(a.bias[n]) : 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (tok0 + i < a.M)
-                        a.C[(int64_t)(tok0 + i) * a.ldc + n] = __float2bfloat16_rn(scale_pow2(v[i], (int)b_max[tok0 + i] - 127 - 13) + bias);
+                        a.C[(int64_t)(tok0 + i) * a.ldc + n] = __float2bfloat16_rn(v[i] + bias);
             }
         }
     }
@@ -151,7 +148,7 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     LinearArgs a{};
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ld_x = ld_x;
-    a.s = ScaleSource{sfb_packed, 1};
+    a.s = ScaleSource{sfb_packed};
     a.bias = static_cast<const __nv_bfloat16*>(bias);
     a.C = static_cast<__nv_bfloat16*>(C);
     a.ldc = ldc;
@@ -166,7 +163,7 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     KBN_CUDA(cudaFuncSetAttribute(mxfp4_linear_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
     const int64_t units = (N + 15) / 16;
     const unsigned grid = (unsigned)std::min<int64_t>(units, sm_count());
-    const size_t smem = (size_t)(kLinearFixed + M * a.token_stride + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));
+    const size_t smem = (size_t)(kLinearFixed + M * (a.token_stride + K / 32) + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));
     const int vec = (ld_x % 8 == 0 || M == 1) && aligned16(x);
     KBN_CUDA(launch_pdl(mxfp4_linear_few_kernel, dim3(grid), dim3(kThreads), smem, st, tm, a, vec));
     KBN_CHECK_LAUNCH();
@@ -188,8 +185,8 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
     KBN_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1u) == 0 && (reinterpret_cast<uintptr_t>(C) & 1u) == 0 && ((ld_x >= K && ldc >= N) || M == 1), KBN_ERR_ARG,
                 "kbn_mxfp4_linear: odd pointer or a row stride too small");
     // The weight stream serves up to eight rows, as long as their f16 values leave room for the ring.
-    if (M <= kMaxGroup && K % 128 == 0 && K < (1ll << 24) && N < (1ll << 27)) {
-        const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad);
+    if (M <= kMaxGroup && K % 128 == 0 && K < (1ll << 17) && N < (1ll << 27)) {
+        const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad + K / 32);
         const int64_t stages = std::min<int64_t>(left / (kStageBytes + Fmt<kMxfp4>::kScaleBytes), kMaxStages);
         if (stages >= kMinStages) return linear_few(x, ld_x, M, K, B, sfb_packed, bias, C, ldc, N, (int)stages, static_cast<cudaStream_t>(stream));
     }

@@ -10,7 +10,7 @@
 // grouped GEMMs, activation and reduction (tasks/baseline/L2/qwen3_moe.py:161-188, tasks/baseline/L2/fused_experts.py:208-283).
 // The activations are not quantised here: with a few tokens that saves no bytes (the weights are everything), so the result
 // is closer to the real-number one than the W8A8 pipeline's.  Roundings: the tokens and the activated rows to 11 bits
-// beside their row's power of two (few_rows.cuh), the result to bf16; everything between is fp32.
+// beside a power of two per 128 values (few_rows.cuh), the result to bf16; everything between is fp32.
 //
 // Bound: the chosen experts' weights, once.  A CTA's range of units is contiguous over (job, row block), so the tokens of
 // a job are loaded into shared memory once or twice per CTA and the ring keeps filling meanwhile.
@@ -45,15 +45,14 @@ struct MoeArgs {
     float* out_w;                  // may be null
     int32_t* out_ids;
     int32_t* status;
-    int32_t stages, token_stride;
+    int32_t stages, token_stride, token_rows;
 };
 
+constexpr int kMaxExperts = 32 * kRouteMaxPerLane;
 struct Scratch {                   // small shared-memory state beside the ring
     Jobs jobs;
     int32_t id[kMaxPairs];
-    int32_t leader[kMaxPairs];
-    uint32_t max_bits[kMaxGroup];
-    int expo[2][kMaxGroup];        // by the job's parity: a finisher may be a unit or two behind the consumers
+    int16_t taken[kMaxExperts], open_job[kMaxExperts];      // by expert: pairs so far, the job that takes the next one
     int abort_flag;
 };
 
@@ -62,7 +61,7 @@ constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
 constexpr int kBarBytes = (2 * kMaxStages + 2 * kFinishers) * 8;
 
 template <int FMT>
-__device__ __forceinline__ Smem carve(uint8_t* raw, int stages, int group, int token_stride, Scratch** scratch) {
+__device__ __forceinline__ Smem carve(uint8_t* raw, int stages, int rows, int token_stride, Scratch** scratch) {
     Smem s;
     uint8_t* p = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
     s.ring = p;
@@ -76,46 +75,45 @@ __device__ __forceinline__ Smem carve(uint8_t* raw, int stages, int group, int t
     s.bars = reinterpret_cast<uint64_t*>(p);
     p += kBarBytes;
     s.tokens = p;
+    s.token_scales = reinterpret_cast<float*>(p + (size_t)rows * token_stride);
     s.stages = stages;
-    (void)group;
-    (void)token_stride;
     return s;
 }
 
-// Pairs -> jobs.  A job is up to `group` pairs of one expert, in pair order; jobs are numbered by their first pair.  All
-// threads of the block take part (blockDim >= pairs).
-__device__ __forceinline__ void build_jobs(Scratch& sc, int pairs, int E, int group, int tid) {
-    int before = 0, leader = -1;
-    const int e = tid < pairs ? sc.id[tid] : -1;
-    const bool valid = e >= 0 && e < E;
-    if (valid) {
-        for (int q = 0; q < tid; ++q)
-            if (sc.id[q] == e) {
-                if (before % group == 0) leader = q;
-                ++before;
+// Pairs -> jobs, by one warp.  A job is up to `group` pairs of one expert, in pair order; jobs are numbered by their first
+// pair.  sc.taken is all zero.  One step per token: its experts are distinct, as a rule; where one occurs twice (equal
+// choices of a router that has run out of experts) the later slot waits for a step of its own.
+__device__ __forceinline__ void build_jobs(Scratch& sc, int T, int topk, int group, int lane) {
+    int n = 0;
+    for (int t = 0; t < T; ++t) {
+        const int p = t * topk + lane;
+        const int e = lane < topk ? sc.id[p] : -1;
+        unsigned todo = __ballot_sync(0xffffffffu, e >= 0);
+        const unsigned same = __match_any_sync(0xffffffffu, e);
+        while (todo) {
+            const bool now = ((todo >> lane) & 1u) && __ffs((int)(same & todo)) - 1 == lane;
+            const int k = now ? sc.taken[e] : 1;
+            const bool opens = now && k == 0;
+            const unsigned opening = __ballot_sync(0xffffffffu, opens);
+            if (now) {
+                const int job = opens ? n + __popc(opening & ((1u << lane) - 1u)) : sc.open_job[e];
+                if (opens) {
+                    sc.open_job[e] = (int16_t)job;
+                    sc.jobs.expert[job] = e;
+                }
+                sc.jobs.pair[job][k] = (int16_t)p;
+                sc.jobs.count[job] = k + 1;
+                sc.taken[e] = (int16_t)(k + 1 == group ? 0 : k + 1);
             }
-        if (before % group == 0) leader = tid;
-    }
-    if (tid < pairs) sc.leader[tid] = leader;
-    __syncthreads();
-    if (valid) {
-        int job = 0;
-        for (int q = 0; q < leader; ++q) job += sc.leader[q] == q;
-        sc.jobs.pair[job][before % group] = (int16_t)tid;
-        if (leader == tid) {
-            int n = 0;
-            for (int q = tid; q < pairs; ++q) n += sc.leader[q] == tid;
-            sc.jobs.expert[job] = e;
-            sc.jobs.count[job] = n;
+            n += __popc(opening);
+            todo &= ~__ballot_sync(0xffffffffu, now);
+            __syncwarp();
         }
     }
-    if (tid == 0) {
-        int n = 0;
-        for (int q = 0; q < pairs; ++q) n += sc.leader[q] == q;
-        sc.jobs.n_jobs = n;
-    }
-    __syncthreads();
+    if (lane == 0) sc.jobs.n_jobs = n;
+    __syncwarp();
 }
+constexpr int kJobsBarrier = 3;
 
 // A copy that was asked for may still be on its way when a bounded wait has run out: give it time to land before the
 // shared memory is given back.
@@ -129,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, const int logits_bf16, const MoeArgs a) {
     extern __shared__ uint8_t raw[];
     Scratch* scp;
-    const Smem s = carve<FMT>(raw, a.stages, a.group, a.token_stride, &scp);
+    const Smem s = carve<FMT>(raw, a.stages, a.token_rows, a.token_stride, &scp);
     Scratch& sc = *scp;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -137,33 +135,48 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
         sc.abort_flag = 0;
         ptx::prefetch_tensormap(&tm);
     }
+    for (int i = tid; i < a.E; i += kThreads) sc.taken[i] = 0;
     __syncthreads();
     ptx::grid_dependency_wait();          // the logits, the tokens and the weights are final from here on
     ptx::launch_dependents();
 
-    const int pairs = a.T * a.topk;
-    if (warp < a.T) {
-        float w;
+    // Where all tokens fit they stay in shared memory for every job; with at most eight, half of the consumers fetch them
+    // while the other half routes.
+    const bool resident = a.T <= a.token_rows;
+    const bool at_once = resident && a.T <= kConsumerWarps / 2;
+    const int router = at_once ? warp - kConsumerWarps / 2 : warp;
+    auto token = [&](int i) { return a.x + (int64_t)i * a.ld_x; };
+    if (warp < kConsumerWarps && router >= 0 && router < a.T) {
+        float logit[PER], w;
         int id;
-        if (logits_bf16) route_token<PER, true>(ra, warp, lane, w, id);
-        else route_token<PER, false>(ra, warp, lane, w, id);
+        load_logits<PER>(ra, logits_bf16 != 0, router, lane, logit);
+        route_logits<PER>(ra, lane, logit, w, id);
         if (lane < a.topk) {
             const bool ok = id >= 0 && id < a.E;
-            sc.id[warp * a.topk + lane] = ok ? id : -1;
-            sc.jobs.weight[warp * a.topk + lane] = ok ? w : __uint_as_float(0x7fc00000u);
+            sc.id[router * a.topk + lane] = ok ? id : -1;
+            sc.jobs.weight[router * a.topk + lane] = ok ? w : __uint_as_float(0x7fc00000u);
             if (blockIdx.x == 0 && a.out_w != nullptr) {
-                a.out_w[warp * a.topk + lane] = w;
-                a.out_ids[warp * a.topk + lane] = ok ? id : -1;
+                a.out_w[router * a.topk + lane] = w;
+                a.out_ids[router * a.topk + lane] = ok ? id : -1;
             }
         }
     }
+    if (at_once && warp < kConsumerWarps / 2) load_tokens<__nv_bfloat16, 16 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
     __syncthreads();
-    build_jobs(sc, pairs, a.E, a.group, tid);
-    if (blockIdx.x == 0) {                // for the second kernel
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(&sc.jobs);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(a.jobs);
-        for (int i = tid; i < (int)(sizeof(Jobs) / 4); i += kThreads) dst[i] = src[i];
-        for (int i = tid; i < a.H / 16; i += kThreads) a.counters[i] = 0;
+    // The producer groups the pairs and starts on the weights at once; the others join as soon as the jobs are there.
+    if (warp == kProducerWarp) {
+        build_jobs(sc, a.T, a.topk, a.group, lane);
+        asm volatile("bar.arrive %0, %1;" ::"n"(kJobsBarrier), "n"(kThreads) : "memory");
+    } else {
+        if (resident && !at_once && warp < kConsumerWarps) load_tokens<__nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
+        asm volatile("bar.sync %0, %1;" ::"n"(kJobsBarrier), "n"(kThreads) : "memory");
+        if (blockIdx.x == 0) {            // for the second kernel
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(&sc.jobs);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(a.jobs);
+            const int i0 = tid - (warp > kProducerWarp ? 32 : 0);      // the producer is not here
+            for (int i = i0; i < (int)(sizeof(Jobs) / 4); i += kThreads - 32) dst[i] = src[i];
+            for (int i = i0; i < a.H / 16; i += kThreads - 32) a.counters[i] = 0;
+        }
     }
 
     const int32_t blocks = a.I / 8, KC = a.H / 128;
@@ -182,18 +195,21 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
         const WaitCtx w{&sc.abort_flag, a.status, 9};
         RingPos pos;
         int32_t loaded = -1;
+        TokenColumns columns{};
         for (int64_t u = u0; u < u1; ++u) {
             const int count = sc.jobs.count[job];
             if (job != loaded) {
-                load_tokens<__nv_bfloat16>(s.tokens, (uint32_t)a.token_stride, count, a.H,
-                                           [&](int i) { return a.x + (int64_t)(sc.jobs.pair[job][i] / a.topk) * a.ld_x; }, sc.max_bits, sc.expo[job & 1], tid);
-                consumer_sync();
+                if (!resident) {
+                    consumer_sync();          // everybody is done with the last job's tokens
+                    load_tokens<__nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, a.H,
+                                                                    [&](int i) { return token(sc.jobs.pair[job][i] / a.topk); }, tid);
+                    consumer_sync();
+                }
                 loaded = job;
+                columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [&](int col) { return resident ? sc.jobs.pair[job][col] / a.topk : col; });
             }
-            // columns without a token compute the last token's again; nothing reads them
-            const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, count - 1) * (uint32_t)a.token_stride;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            consume_unit<FMT>(s, pos, KC, warp, lane, token_row, acc, w);
+            consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
             if (++rb == blocks) rb = 0, ++job;
         }
@@ -208,9 +224,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
                 for (int i = 0; i < 4; ++i) {
                     const float other = __shfl_down_sync(0xffffffffu, v[i], 16);      // rows 8-15 are the up projection's
                     if (lane < 16 && tok0 + i < count) {
-                        const int e = sc.expo[job & 1][tok0 + i];
-                        const float g = scale_pow2(v[i], e), up = scale_pow2(other, e);
-                        a.y[(int64_t)sc.jobs.pair[job][tok0 + i] * a.I + 8 * rb + (lane >> 1)] = __fdiv_rn(g, 1.0f + expf(-g)) * up;
+                        a.y[(int64_t)sc.jobs.pair[job][tok0 + i] * a.I + 8 * rb + (lane >> 1)] = __fdiv_rn(v[i], 1.0f + expf(-v[i])) * other;
                     }
                 }
             }
@@ -233,13 +247,14 @@ __device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, in
 }
 
 constexpr int kCountBatch = 4;
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 
 template <int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
 few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
     extern __shared__ uint8_t raw[];
     Scratch* scp;
-    const Smem s = carve<FMT>(raw, a.stages, a.group, a.token_stride, &scp);
+    const Smem s = carve<FMT>(raw, a.stages, a.token_rows, a.token_stride, &scp);
     Scratch& sc = *scp;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -278,17 +293,18 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
         const WaitCtx w{&sc.abort_flag, a.status, 11};
         RingPos pos;
         int32_t loaded = -1;
+        TokenColumns columns{};
         for (int64_t u = u0; u < u1; ++u) {
             const int count = sc.jobs.count[job];
             if (job != loaded) {
-                load_tokens<float>(s.tokens, (uint32_t)a.token_stride, count, a.I,
-                                   [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I; }, sc.max_bits, sc.expo[job & 1], tid);
+                consumer_sync();
+                load_tokens<float, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, a.I, [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I; }, tid);
                 consumer_sync();
                 loaded = job;
+                columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [](int col) { return col; });
             }
-            const uint32_t token_row = ptx::smem_u32(s.tokens) + (uint32_t)min(lane >> 2, count - 1) * (uint32_t)a.token_stride;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            consume_unit<FMT>(s, pos, KC, warp, lane, token_row, acc, w);
+            consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
             if (++rb == blocks) rb = 0, ++job;
         }
@@ -303,16 +319,16 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (tok0 + i < count)
-                        a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + 16 * rb + (lane >> 1)] = scale_pow2(v[i], sc.expo[job & 1][tok0 + i]);
+                        a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + 16 * rb + (lane >> 1)] = v[i];
                 if (lane == pending) mine = rb;
                 ++pending;
             }
             // One fence and one round of counting for several units.  Who completes a column block (every job once) adds it up.
             if (pending == kCountBatch || (pending > 0 && u + kFinishers >= u1)) {
-                __threadfence();
+                fence_gpu();
                 __syncwarp();
                 unsigned last = __ballot_sync(0xffffffffu, lane < pending && atomicAdd(a.counters + mine, 1) == n_jobs - 1);
-                if (last) __threadfence();
+                if (last) fence_gpu();
                 for (; last; last &= last - 1) add_up(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
                 pending = 0;
             }
@@ -325,22 +341,22 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
 // ---- host ----------------------------------------------------------------------------------------
 
 struct Plan {
-    int group, stages, token_stride;
+    int rows, stages, token_stride;
     size_t smem;
 };
 
-// Largest group of tokens (up to `want`) whose rows of K values leave room for a ring of at least kMinStages.
+// As many token rows of K values (with their chunk scales), up to `want`, as leave room for a ring of at least kMinStages.
 template <int FMT>
 static bool plan(int64_t K, int want, Plan* p) {
-    const int64_t stride = K * 2 + Fmt<FMT>::kTokenPad, per_stage = kStageBytes + Fmt<FMT>::kScaleBytes;
+    const int64_t stride = K * 2 + Fmt<FMT>::kTokenPad, row = stride + K / 32, per_stage = kStageBytes + Fmt<FMT>::kScaleBytes;
     const int64_t fixed = 1024 + kRedBytes + scratch_bytes() + kBarBytes;
-    for (int g = std::min(want, kMaxGroup); g >= 1; --g) {
-        const int64_t left = kSmemMax - fixed - g * stride;
+    for (int g = want; g >= 1; --g) {
+        const int64_t left = kSmemMax - fixed - g * row;
         if (left < kMinStages * per_stage) continue;
-        p->group = g;
+        p->rows = g;
         p->token_stride = (int)stride;
         p->stages = (int)std::min<int64_t>(left / per_stage, kMaxStages);
-        p->smem = (size_t)(fixed + g * stride + p->stages * per_stage);
+        p->smem = (size_t)(fixed + g * row + p->stages * per_stage);
         return true;
     }
     return false;
@@ -368,11 +384,16 @@ static WorkspaceLayout workspace_layout(int64_t T, int64_t topk, int64_t H, int6
 
 template <int FMT>
 static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& ra, int logits_bf16, cudaStream_t st) {
+    // One grouping of the pairs for both kernels: as many rows as either can hold.  The first keeps all tokens if it can.
     Plan p1, p2;
-    KBN_REQUIRE(plan<FMT>(std::max(a.H, a.I), a.T, &p1), KBN_ERR_UNSUPPORTED,
+    const int most = std::min(a.T, kMaxGroup);
+    KBN_REQUIRE(plan<FMT>(a.H, most, &p1) && plan<FMT>(a.I, most, &p2), KBN_ERR_UNSUPPORTED,
                 "kbn_moe_few_tokens: a row of %d values does not fit the shared memory", std::max(a.H, a.I));
-    a.group = p1.group;                    // one grouping for both kernels
-    KBN_REQUIRE(plan<FMT>(a.H, a.group, &p1) && plan<FMT>(a.I, a.group, &p2), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
+    a.group = std::min(p1.rows, p2.rows);
+    Plan all;
+    KBN_REQUIRE(plan<FMT>(a.H, a.T, &all) && plan<FMT>(a.I, a.group, &p2), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
+    if (all.rows < a.T) plan<FMT>(a.H, a.group, &all);
+    p1 = all;
     CUtensorMap t13, t2;
     int rc = weight_map<FMT>(&t13, w13, (int64_t)a.E * 2 * a.I, a.H);
     if (rc != KBN_OK) return rc;
@@ -387,10 +408,12 @@ static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& 
     if (rc != KBN_OK) return rc;
     const unsigned grid = (unsigned)sm_count();
     a.stages = p1.stages;
+    a.token_rows = p1.rows;
     a.token_stride = p1.token_stride;
     KBN_CUDA(launch_pdl(up_kernel, dim3(grid), dim3(kThreads), p1.smem, st, t13, ra, logits_bf16, a));
     KBN_CHECK_LAUNCH();
     a.stages = p2.stages;
+    a.token_rows = p2.rows;
     a.token_stride = p2.token_stride;
     KBN_CUDA(launch_pdl(few_down_kernel<FMT>, dim3(grid), dim3(kThreads), p2.smem, st, t2, a));
     KBN_CHECK_LAUNCH();
@@ -438,8 +461,8 @@ extern "C" int kbn_moe_few_tokens(const void* x, int64_t ld_x, int64_t T, const 
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ld_x = ld_x;
     a.T = (int32_t)T; a.topk = (int32_t)topk; a.H = (int32_t)H; a.I = (int32_t)I; a.E = (int32_t)E;
-    a.s13 = ScaleSource{w13_s, 0};
-    a.s2 = ScaleSource{w2_s, 0};
+    a.s13 = ScaleSource{w13_s};
+    a.s2 = ScaleSource{w2_s};
     a.jobs = reinterpret_cast<Jobs*>(ws + wl.jobs);
     a.counters = reinterpret_cast<int32_t*>(ws + wl.counters);
     a.y = reinterpret_cast<float*>(ws + wl.y);

@@ -36,6 +36,17 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
     return __uint_as_float(b == 0u ? 0x00400000u : (b == 255u ? 0x7fc00000u : b << 23));
 }
 
+// Two E8M0 bytes (the low half of w) -> two packed bf16 values, with the subnormal and the NaN.  Exact.
+__device__ __forceinline__ uint32_t scale_bf16x2(uint32_t w) {
+    uint32_t d;
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %1;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %0, a;\n\t}"
+        : "=r"(d)
+        : "r"(w));
+    return d;
+}
+
 // Two fp32 values -> one byte of two e2m1 codes (lo in the low nibble), round to nearest even, saturating at +-6.
 __device__ __forceinline__ uint32_t pack_e2m1x2(float lo, float hi) {
     uint32_t d;
