@@ -5,7 +5,8 @@
 // counts is that enough weight bytes are in flight on every SM all the time.  One CTA per SM walks a contiguous range of
 // units; a unit is 16 weight rows (two boxes of eight) over the whole K.  A producer warp keeps a ring of 16 KB stages
 // full with 3-D tiled TMA loads (eight rows of a box, up to 16 chunks of 128 K-values each, one instruction per box) and
-// the block scales beside them (4-byte asynchronous copies); sixteen consumer warps split the chunks.
+// the block scales beside them (tiled loads too where their rows allow it, else 4-byte asynchronous copies, which cost the
+// one producer warp about as many instructions as everything else); sixteen consumer warps split the chunks.
 //
 //   product    mma.sync.m16n8k16, f16 x f16 -> fp32: the 16 weight rows are its M, the tokens its N.  (tcgen05 would spend a
 //              128-row tile on them and needs its operands in fp8 or fp4; at this intensity the legacy instruction is far
@@ -44,7 +45,7 @@ template <int FMT>
 struct Fmt;
 template <>
 struct Fmt<kFp8> {
-    static constexpr int kChunkBytes = 128, kChunks = 8, kScaleBytes = 128, kTokenPad = 16;
+    static constexpr int kChunkBytes = 128, kChunks = 8, kScaleBytes = 512, kTokenPad = 16;
     static constexpr int kArrivals = 8;                   // warps that read a stage
 };
 template <>
@@ -55,9 +56,15 @@ struct Fmt<kMxfp4> {
 
 // Where a weight matrix's scales lie.  FP8: fp32 [rows / 128, KC].  MXFP4: one 32-bit word per row and chunk, row-major
 // (word (row, c) at row * KC + c) or, PACKED, in the packed layout of the tensor core.
+// MXFP4 row-major scales with 16-byte row strides (K % 512 == 0) also have a tensor map (boxes of eight rows x 64 bytes,
+// 64-byte swizzle).  In the ring a stage's word (row of 16, chunk) is always where that box puts it, see scale_word().
 struct ScaleSource {
     const void* base;
+    const CUtensorMap* map;      // null: asynchronous copies
 };
+__device__ __forceinline__ uint32_t scale_word(int row, int chunk) {      // byte offset; no bank conflicts over eight rows
+    return (uint32_t)(row * 64 + ((((chunk >> 2) ^ (row >> 1)) & 3) << 4) + (chunk & 3) * 4);
+}
 
 struct Smem {
     uint8_t* ring;         // stages, 1024-byte aligned
@@ -74,6 +81,13 @@ __device__ __forceinline__ void mma_f16_m16n8k16(float (&d)[4], uint32_t a0, uin
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with a zero C operand, so that a fresh partial sum costs no register moves.
+__device__ __forceinline__ void mma_f16_m16n8k16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Four e4m3 bytes -> two packed f16 pairs.  Exact.
 __device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -109,6 +123,20 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumerWarps) : "memory"); }
 
+// Bounded wait of a warp on one of this file's barriers.  The hint lets the hardware keep the warp suspended for longer than
+// its default, so that waiting warps take fewer issue slots from working ones.
+__device__ __forceinline__ void wait_ring(uint32_t bar, uint32_t parity, const WaitCtx& w) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (!ok) wait_bar(bar, parity, w);
+}
+
 // Ring position, advanced one stage at a time.
 struct RingPos {
     uint32_t slot = 0, phase = 0;
@@ -141,14 +169,19 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
     using F = Fmt<FMT>;
     for (int32_t c0 = 0; c0 < KC; c0 += F::kChunks) {
         const uint32_t full = ptx::smem_u32(s.bars + pos.slot), empty = ptx::smem_u32(s.bars + s.stages + pos.slot);
-        wait_bar(empty, pos.phase ^ 1u, w);
+        wait_ring(empty, pos.phase ^ 1u, w);
         const uint32_t dst = ptx::smem_u32(s.ring) + pos.slot * kStageBytes;
+        const uint32_t sdst = ptx::smem_u32(s.scales) + pos.slot * F::kScaleBytes;
+        const bool tiled = FMT == kMxfp4 && !PACKED && sc.map != nullptr;
         if (lane == 0) {
-            ptx::mbar_arrive_expect_tx(full, kStageBytes);
+            ptx::mbar_arrive_expect_tx(full, tiled ? kStageBytes + F::kScaleBytes : kStageBytes);
             tma_load_3d(dst, tmap, 0, row_a, c0, full);
             tma_load_3d(dst + kStageBytes / 2, tmap, 0, row_b, c0, full);
+            if (tiled) {
+                ptx::tma_load_2d(sdst, sc.map, c0 * 4, row_a, full);
+                ptx::tma_load_2d(sdst + F::kScaleBytes / 2, sc.map, c0 * 4, row_b, full);
+            }
         }
-        const uint32_t sdst = ptx::smem_u32(s.scales) + pos.slot * F::kScaleBytes;
         if (FMT == kFp8) {
             // lane = 8 * box + chunk
             const int32_t c = c0 + (lane & 7);
@@ -156,15 +189,14 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
                 const int32_t row = lane < 8 ? row_a : row_b;
                 cp_async4(sdst + lane * 4, static_cast<const float*>(sc.base) + (int64_t)(row >> 7) * KC + c);
             }
-        } else {
-            // word (chunk, row of 16) at (chunk * 16 + row) * 4: eight words per lane, two chunks apart
+        } else if (!tiled) {
+            // eight words per lane, two chunks apart
             const int32_t r = lane & 15, c = c0 + (lane >> 4);
             const int32_t row = min((r < 8 ? row_a : row_b - 8) + r, n_rows - 1);
             const uint32_t* src = static_cast<const uint32_t*>(sc.base) + (PACKED ? (int64_t)mxfp4::packed_word(row, c, KC) : (int64_t)row * KC + c);
-            const uint32_t sl = sdst + (uint32_t)lane * 4u;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c + 2 * i < KC) cp_async4(sl + i * 128, src + i * (PACKED ? 256 : 2));
+                if (c + 2 * i < KC) cp_async4(sdst + scale_word(r, (lane >> 4) + 2 * i), src + i * (PACKED ? 256 : 2));
         }
         cp_async_arrive(full);
         pos.advance((uint32_t)s.stages);
@@ -197,7 +229,7 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
         const RingPos here = pos;
         pos.advance((uint32_t)s.stages);
         if (FMT == kFp8 && (here.slot & 1u) != (uint32_t)(warp >> 3)) continue;
-        wait_bar(ptx::smem_u32(s.bars + here.slot), here.phase, w);
+        wait_ring(ptx::smem_u32(s.bars + here.slot), here.phase, w);
         const int32_t c = c0 + cw;
         if (c < KC) {
             const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * 8 + g) * F::kChunkBytes;
@@ -205,7 +237,7 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
             const uint32_t sdst = ptx::smem_u32(s.scales) + here.slot * F::kScaleBytes;
             const float x0s = __uint_as_float(lds32(tc.scale0 + (uint32_t)c * 4u)), x1s = __uint_as_float(lds32(tc.scale1 + (uint32_t)c * 4u));
             if (FMT == kFp8) {
-                float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
+                float p[4], q[4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t piece = (uint32_t)(t + 4 * j);
@@ -214,9 +246,11 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
                     const uint4 x0 = lds128(ta), x1 = lds128(ta + 16);
                     uint32_t a0, a1, a2, a3;
                     e4m3x4_to_f16(wa.x, a0, a2); e4m3x4_to_f16(wb.x, a1, a3);
-                    mma_f16_m16n8k16(p, a0, a1, a2, a3, x0.x, x0.y);
+                    if (j == 0) mma_f16_m16n8k16_first(p, a0, a1, a2, a3, x0.x, x0.y);
+                    else mma_f16_m16n8k16(p, a0, a1, a2, a3, x0.x, x0.y);
                     e4m3x4_to_f16(wa.y, a0, a2); e4m3x4_to_f16(wb.y, a1, a3);
-                    mma_f16_m16n8k16(q, a0, a1, a2, a3, x0.z, x0.w);
+                    if (j == 0) mma_f16_m16n8k16_first(q, a0, a1, a2, a3, x0.z, x0.w);
+                    else mma_f16_m16n8k16(q, a0, a1, a2, a3, x0.z, x0.w);
                     e4m3x4_to_f16(wa.z, a0, a2); e4m3x4_to_f16(wb.z, a1, a3);
                     mma_f16_m16n8k16(p, a0, a1, a2, a3, x1.x, x1.y);
                     e4m3x4_to_f16(wa.w, a0, a2); e4m3x4_to_f16(wb.w, a1, a3);
@@ -228,26 +262,28 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
                 acc[2] = fmaf((p[2] + q[2]) * x0s, s1, acc[2]);
                 acc[3] = fmaf((p[3] + q[3]) * x1s, s1, acc[3]);
             } else {
-                const uint32_t sw0 = lds32(sdst + (uint32_t)(cw * 16 + g) * 4u), sw1 = lds32(sdst + (uint32_t)(cw * 16 + 8 + g) * 4u);
+                const uint32_t sw0 = lds32(sdst + scale_word(g, cw)), sw1 = lds32(sdst + scale_word(g, cw) + 512);      // rows g and g + 8
                 const uint32_t swz = (uint32_t)(g >> 1) & 3u;
                 const uint32_t e0[2] = {mxfp4::scale_bf16x2(sw0), mxfp4::scale_bf16x2(sw0 >> 16)}, e1[2] = {mxfp4::scale_bf16x2(sw1), mxfp4::scale_bf16x2(sw1 >> 16)};
-                float q[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint32_t w0 = box0 + (swz << 4) + (uint32_t)t * 4u;      // 16-byte piece b of the row at w0 ^ 16 b
+                const uint32_t xa = tc.row + (uint32_t)(c * 128 + t * 8) * 2u;
+                float q[4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const uint32_t off = (((uint32_t)b ^ swz) << 4) + (uint32_t)t * 4u;
-                    const uint32_t wa = lds32(box0 + off), wb = lds32(box1 + off);
-                    const uint4 x = lds128(tc.row + (uint32_t)(c * 128 + b * 32 + t * 8) * 2u);
+                    const uint32_t wb_at = w0 ^ (uint32_t)(16 * b);
+                    const uint32_t wa = lds32(wb_at), wb = lds32(wb_at + kStageBytes / 2);
+                    const uint4 x = lds128(xa + 64 * b);
                     uint32_t ha[4], hb[4];
                     mxfp4::unpack_e2m1x8(wa, ha);
                     mxfp4::unpack_e2m1x8(wb, hb);
-                    float p[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16_m16n8k16(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+                    float p[4];
+                    mma_f16_m16n8k16_first(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
                     mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
                     const float s0 = b & 1 ? bf16_hi(e0[b >> 1]) : bf16_lo(e0[b >> 1]), s1 = b & 1 ? bf16_hi(e1[b >> 1]) : bf16_lo(e1[b >> 1]);
-                    q[0] = fmaf(p[0], s0, q[0]);
-                    q[1] = fmaf(p[1], s0, q[1]);
-                    q[2] = fmaf(p[2], s1, q[2]);
-                    q[3] = fmaf(p[3], s1, q[3]);
+                    q[0] = b == 0 ? p[0] * s0 : fmaf(p[0], s0, q[0]);
+                    q[1] = b == 0 ? p[1] * s0 : fmaf(p[1], s0, q[1]);
+                    q[2] = b == 0 ? p[2] * s1 : fmaf(p[2], s1, q[2]);
+                    q[3] = b == 0 ? p[3] * s1 : fmaf(p[3], s1, q[3]);
                 }
                 acc[0] = fmaf(q[0], x0s, acc[0]);
                 acc[1] = fmaf(q[1], x1s, acc[1]);
@@ -263,7 +299,7 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
 // Consumer warp: its partial sums of the CTA's u-th unit to the finisher u % kFinishers; element (row of 16) * 8 + token.
 __device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, int lane, const float (&acc)[4], const WaitCtx& w) {
     const int buf = (int)(u % kFinishers);
-    wait_bar(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf), (uint32_t)(u / kFinishers & 1) ^ 1u, w);
+    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf), (uint32_t)(u / kFinishers & 1) ^ 1u, w);
     float* r = s.red + (buf * kConsumerWarps + warp) * 128;
     const int g = lane >> 2, t = lane & 3;
     *reinterpret_cast<float2*>(r + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
@@ -274,7 +310,7 @@ __device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, in
 // Finisher warp u % kFinishers: the sums of the CTA's u-th unit.  Lane l receives row l / 2, tokens 4 (l % 2) .. + 3.
 __device__ __forceinline__ void take_over(const Smem& s, int64_t u, int lane, float (&v)[4], const WaitCtx& w) {
     const int buf = (int)(u % kFinishers);
-    wait_bar(ptx::smem_u32(s.bars + 2 * s.stages + buf), (uint32_t)(u / kFinishers & 1), w);
+    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + buf), (uint32_t)(u / kFinishers & 1), w);
     const float4* r = reinterpret_cast<const float4*>(s.red + buf * kConsumerWarps * 128) + lane;
     v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll
@@ -359,6 +395,18 @@ __device__ __forceinline__ void load_tokens(const Smem& s, uint32_t stride, int 
 
 constexpr int kSmemMax = 232448;      // shared memory a CTA may ask for
 
+// Lets a kernel use all of an SM's shared memory; asked of the driver once per kernel and device.
+template <typename Kernel>
+static int allow_smem(Kernel kernel, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    KBN_CUDA(cudaGetDevice(&dev));
+    KBN_REQUIRE(dev >= 0 && dev < 64, KBN_ERR_UNSUPPORTED, "device ordinal %d out of range", dev);
+    if (done.load(std::memory_order_acquire) >> dev & 1u) return KBN_OK;
+    KBN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    done.fetch_or(1ull << dev, std::memory_order_release);
+    return KBN_OK;
+}
+
 // Weight matrix [rows, K] as (chunk, row, chunk number): one box is eight rows of kChunks chunks, each chunk's eight rows
 // side by side and swizzled, so that a warp reading one chunk of eight rows touches every bank once.
 template <int FMT>
@@ -374,6 +422,20 @@ static int weight_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K
     t.box[0] = F::kChunkBytes; t.box[1] = 8; t.box[2] = F::kChunks;
     t.swizzle = FMT == kFp8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+    return encode_tensor_map(tm, t);
+}
+
+// Row-major MXFP4 scales [rows, K / 32]; only with K % 512 == 0.
+static int scale_rows_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K) {
+    TensorMapSpec t;
+    memset(&t, 0, sizeof(t));
+    t.base = base;
+    t.rank = 2;
+    t.dims[0] = (uint64_t)(K / 32); t.dims[1] = (uint64_t)rows; t.dims[2] = 1;
+    t.strides[0] = (uint64_t)(K / 32);
+    t.box[0] = 64; t.box[1] = 8; t.box[2] = 1;
+    t.swizzle = CU_TENSOR_MAP_SWIZZLE_64B;
+    t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
     return encode_tensor_map(tm, t);
 }
 

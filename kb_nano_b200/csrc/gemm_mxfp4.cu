@@ -15,6 +15,8 @@
 //   few tiles   (a few hundred rows or fewer) one tile per cluster of 2 S CTAs, whose S pairs split K.  Each pair owns 256 / S
 //               columns and receives the other pairs' partial sums of them as one bulk copy each through the cluster's shared
 //               memory; partials are added in slice order, so results are reproducible.
+#include <algorithm>
+
 #include "gemm_common.cuh"
 #include "mxfp4.cuh"
 #include "tensor_map.cuh"
@@ -22,17 +24,28 @@
 namespace kbn {
 namespace mxfp4 {
 
-constexpr int kTileM = 256, kTileN = 256;
-constexpr int kStages = 6;                                    // K-steps of 256 values in the ring
-constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;      // this CTA's rows of A and of B, one K-step
-constexpr int kOperandBytes = kABytes + kBBytes;
-constexpr int kSfBytes = 3 * 1024;                            // own A row block, both B row blocks, two 128-K blocks each
-constexpr uint32_t kTxPair = 2u * (kOperandBytes + kSfBytes);
+constexpr int kTileM = 256;
+constexpr int kABytes = 128 * 128;                             // this CTA's rows of A, one K-step of 256 values
 constexpr int kEpiWarps = 8;
 constexpr int kGemmThreads = 32 * (2 + kEpiWarps);
-constexpr int kGemmSmem = kStages * (kOperandBytes + kSfBytes) + 1024 + 256;
-constexpr int kTmemColumns = 512, kColSfa = 256, kColSfb = 264;      // scale columns: 4 per row block and 128-K block
+constexpr int kStagingBytes = kEpiWarps * 32 * 128;            // 32 rows x 64 bf16 columns per epilogue warp
+constexpr int kTmemColumns = 512, kColScales = 256;            // accumulators in columns 0-255, scales behind them
 constexpr int kGroupM = 8;                                     // tile rows that run side by side, for reuse of B in L2
+
+// BN: tile columns, 256 or 128.
+template <int BN>
+struct Cfg {
+    static constexpr int kBBytes = BN / 2 * 128;               // this CTA's half of the tile's rows of B
+    static constexpr int kOperandBytes = kABytes + kBBytes;
+    static constexpr int kSfBlocks = 1 + BN / 128;             // row blocks whose scales a step needs: A's own, all of B's
+    static constexpr int kSfBytes = kSfBlocks * 1024;          // two 128-K blocks each
+    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr uint32_t kTxPair = 2u * (kOperandBytes + kSfBytes);
+    static constexpr int kAccs = 256 / BN;                     // accumulators: a 128-column tile is drained under the next one
+    static constexpr int kSmem = kStages * (kOperandBytes + kSfBytes) + kStagingBytes + 1024 + 256;
+    static constexpr int kExchange = 2 * 3 * 128 * (BN / 4) * 4;      // split K: partial sums sent and received, S = 4
+    static_assert(kExchange <= kStages * (kOperandBytes + kSfBytes) + kStagingBytes && kSmem <= 232448, "shared memory");
+};
 
 struct GemmArgs {
     const __nv_bfloat16* bias;
@@ -41,6 +54,7 @@ struct GemmArgs {
     int32_t* status;
     int32_t M, N, kblocks, steps;      // kblocks: 128-K blocks (scales), steps: 256-K steps
     int32_t m_tiles, n_tiles, S;
+    int32_t tiled_out;                 // the output's rows allow tiled stores
 };
 
 // Instruction descriptor, kind::mxf4: A = B = e2m1 K-major, UE8M0 scales, K = 64 dense.
@@ -53,14 +67,43 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t m, uint32_t n, uint32
            | ((m >> 7) << 27)    // M / 128
            | (sf_id << 29);      // scale bytes of A
 }
+// The issuing warps run their loops whole, every lane with the same values, and elect one lane inside each instruction.  With
+// one lane branched off instead, the operands cannot stay in uniform registers and each tcgen05 or TMA instruction cost its
+// issuer about 70 cycles: more, over a step, than the tensor cores need for it (8192 x 7168 x 7168: 259 -> 197 us).
+#define KBN_ELECT "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
 __device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-        : "memory");
+    asm volatile(KBN_ELECT
+                 ".reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+                 : "memory");
 }
+__device__ __forceinline__ void copy_scales_pair(uint32_t dst_tmem, uint64_t src_desc) {
+    asm volatile(KBN_ELECT "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(dst_tmem), "l"(src_desc) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t cta_mask) {
+    asm volatile(KBN_ELECT "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                 ::"r"(bar), "h"(cta_mask) : "memory");
+}
+__device__ __forceinline__ void load_pair(uint32_t dst, const void* tmap, int32_t x, int32_t y, uint32_t bar_cluster) {
+    asm volatile(KBN_ELECT
+                 "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+    asm volatile(KBN_ELECT "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Tiled store of a box from shared memory; completion by bulk groups of the elected lane.
+__device__ __forceinline__ void store_box(const void* tmap, int32_t x, int32_t y, uint32_t src) {
+    asm volatile(KBN_ELECT
+                 "@e cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t"
+                 "@e cp.async.bulk.commit_group;\n\t}"
+                 ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void stores_have_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar_cluster) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
@@ -85,13 +128,28 @@ __device__ __forceinline__ void tile_of(int32_t t, const GemmArgs& p, int32_t& m
     n_tile = in / size;
 }
 
-// 32 accumulator columns of one row (+ bias) -> bf16.
-__device__ __forceinline__ void store_row(float (&f)[32], const GemmArgs& p, int32_t row, int32_t n0) {
-    if (p.bias != nullptr) {
+// + bias, 32 columns.
+__device__ __forceinline__ void add_bias(float (&f)[32], const GemmArgs& p, int32_t n0) {
+    if (p.bias == nullptr) return;
+    if (n0 + 32 <= p.N && (reinterpret_cast<uintptr_t>(p.bias + n0) & 15u) == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint4 b = *reinterpret_cast<const uint4*>(p.bias + n0 + 8 * j);
+            const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[8 * j + 2 * i] += bf16_lo(w[i]);
+                f[8 * j + 2 * i + 1] += bf16_hi(w[i]);
+            }
+        }
+    } else {
 #pragma unroll
         for (int q = 0; q < 32; ++q)
             if (n0 + q < p.N) f[q] += __bfloat162float(p.bias[n0 + q]);
     }
+}
+// 32 columns of one row -> bf16, straight to global memory.
+__device__ __forceinline__ void store_row(const float (&f)[32], const GemmArgs& p, int32_t row, int32_t n0) {
     __nv_bfloat16* c = p.C + (int64_t)row * p.ldc + n0;
     const bool vec = (reinterpret_cast<uintptr_t>(c) & 15u) == 0;
 #pragma unroll
@@ -108,20 +166,30 @@ __device__ __forceinline__ void store_row(float (&f)[32], const GemmArgs& p, int
         }
     }
 }
+// 32 columns of one row -> bf16 in a warp's staging rows (64 columns, 128 bytes, swizzled as the tensor map expects).
+__device__ __forceinline__ void stage_row(const float (&f)[32], uint32_t staging, int row, int half) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        ptx::st_shared_v4(staging + (uint32_t)row * 128u + (uint32_t)(((4 * half + j) ^ (row & 7)) << 4), pack_bf16x2(f[8 * j + 0], f[8 * j + 1]),
+                          pack_bf16x2(f[8 * j + 2], f[8 * j + 3]), pack_bf16x2(f[8 * j + 4], f[8 * j + 5]), pack_bf16x2(f[8 * j + 6], f[8 * j + 7]));
+}
 
-template <bool SPLIT>
+template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSfa,
-                  const __grid_constant__ CUtensorMap tmSfb, const GemmArgs p) {
+                  const __grid_constant__ CUtensorMap tmSfb, const __grid_constant__ CUtensorMap tmC, const GemmArgs p) {
+    using F = Cfg<BN>;
+    constexpr int kStages = F::kStages, kOperandBytes = F::kOperandBytes, kSfBytes = F::kSfBytes;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~(uintptr_t)1023u);
     uint8_t* sf = smem + (size_t)kStages * kOperandBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sf + (size_t)kStages * kSfBytes);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 3);
+    uint8_t* staging = sf + (size_t)kStages * kSfBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStagingBytes);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t bar_full = ptx::smem_u32(bars), bar_empty = ptx::smem_u32(bars + kStages);
-    const uint32_t bar_tfull = ptx::smem_u32(bars + 2 * kStages), bar_tempty = bar_tfull + 8, bar_xchg = bar_tfull + 16;
+    const uint32_t bar_tfull = ptx::smem_u32(bars + 2 * kStages), bar_tempty = bar_tfull + 16, bar_xchg = bar_tfull + 32;      // two accumulators each
     const uint32_t tiles_smem = ptx::smem_u32(smem), sf_smem = ptx::smem_u32(sf);
 
     const uint32_t rank = ptx::cluster_ctarank();
@@ -133,10 +201,12 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             ptx::mbar_init(bar_full + 8 * s, 1);         // armed by the even CTA for both CTAs' copies
             ptx::mbar_init(bar_empty + 8 * s, 1);        // one commit, delivered to both
         }
-        ptx::mbar_init(bar_tfull, 1);
-        ptx::mbar_init(bar_tempty, 2 * kEpiWarps);       // used in the even CTA: the epilogue warps of both
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(bar_tfull + 8 * i, 1);
+            ptx::mbar_init(bar_tempty + 8 * i, 2 * kEpiWarps);       // used in the even CTA: the epilogue warps of both
+        }
         ptx::mbar_init(bar_xchg, 1);
-        if (SPLIT) ptx::mbar_arrive_expect_tx(bar_xchg, (uint32_t)(p.S - 1) * (uint32_t)(128 * (kTileN / p.S) * 4));
+        if (SPLIT) ptx::mbar_arrive_expect_tx(bar_xchg, (uint32_t)(p.S - 1) * (uint32_t)(128 * (BN / p.S) * 4));
         *abort_flag = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
@@ -144,6 +214,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         ptx::prefetch_tensormap(&tmB);
         ptx::prefetch_tensormap(&tmSfa);
         ptx::prefetch_tensormap(&tmSfb);
+        if (p.tiled_out) ptx::prefetch_tensormap(&tmC);
     }
     if (warp == 1) {
         ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), kTmemColumns);
@@ -153,7 +224,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     __syncthreads();
     ptx::cluster_sync();              // the partner's barriers exist before anything is sent to them
     ptx::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Everything this kernel reads, the weights too, may have been written by the kernel before it.
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
@@ -165,103 +236,120 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     const int32_t k0 = (int32_t)ks * per_slice, k1 = min(p.steps, k0 + per_slice);      // not empty: the host sees to it
 
     if (warp == 0) {
-        if (lane == 0) {
-            const WaitCtx w{abort_flag, p.status, 12};
-            uint32_t slot = 0, phase = 0;
-            bool ok = true;
-            for (int32_t t = cluster; ok && t < tiles; t += stride) {
-                int32_t mt, nt;
-                tile_of(t, p, mt, nt);
-                const int32_t row_a = mt * kTileM + (int32_t)pr * 128, row_b = nt * kTileN + (int32_t)pr * 128;
-                const int32_t sfa_row = (row_a >> 7) * p.kblocks, sfb_row = (nt * 2) * p.kblocks;
-                for (int32_t k = k0; k < k1; ++k) {
-                    if (!wait_bar(bar_empty + 8 * slot, phase ^ 1u, w)) { ok = false; break; }
-                    if (pr == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * slot, kTxPair);
-                    const uint32_t bar = ptx::mapa(bar_full + 8 * slot, leader);
-                    const uint32_t dst = tiles_smem + slot * kOperandBytes, sdst = sf_smem + slot * kSfBytes;
-                    ptx::tma_load_2d_pair(dst, &tmA, k * 128, row_a, bar);
-                    ptx::tma_load_2d_pair(dst + kABytes, &tmB, k * 128, row_b, bar);
-                    // scales: the packed array as rows of 256 bytes, two per 512-byte block
-                    ptx::tma_load_2d_pair(sdst, &tmSfa, 0, 2 * (sfa_row + 2 * k), bar);
-                    ptx::tma_load_2d_pair(sdst + 1024, &tmSfb, 0, 2 * (sfb_row + 2 * k), bar);
-                    ptx::tma_load_2d_pair(sdst + 2048, &tmSfb, 0, 2 * (sfb_row + p.kblocks + 2 * k), bar);
-                    if (++slot == kStages) slot = 0, phase ^= 1u;
-                }
+        const WaitCtx w{abort_flag, p.status, 12};
+        uint32_t slot = 0, phase = 0;
+        bool ok = true;
+        for (int32_t t = cluster; ok && t < tiles; t += stride) {
+            int32_t mt, nt;
+            tile_of(t, p, mt, nt);
+            const int32_t row_a = mt * kTileM + (int32_t)pr * 128, row_b = nt * BN + (int32_t)pr * (BN / 2);
+            const int32_t sfa_row = (row_a >> 7) * p.kblocks, sfb_row = nt * (BN / 128) * p.kblocks;
+            for (int32_t k = k0; k < k1; ++k) {
+                ok = __all_sync(0xffffffffu, wait_bar(bar_empty + 8 * slot, phase ^ 1u, w));
+                if (!ok) break;
+                if (pr == 0) expect_bytes(bar_full + 8 * slot, F::kTxPair);
+                const uint32_t bar = ptx::mapa(bar_full + 8 * slot, leader);
+                const uint32_t dst = tiles_smem + slot * kOperandBytes, sdst = sf_smem + slot * kSfBytes;
+                load_pair(dst, &tmA, k * 128, row_a, bar);
+                load_pair(dst + kABytes, &tmB, k * 128, row_b, bar);
+                // scales: the packed array as rows of 256 bytes, two per 512-byte block
+                load_pair(sdst, &tmSfa, 0, 2 * (sfa_row + 2 * k), bar);
+#pragma unroll
+                for (int b = 0; b < BN / 128; ++b) load_pair(sdst + 1024 * (1 + b), &tmSfb, 0, 2 * (sfb_row + b * p.kblocks + 2 * k), bar);
+                if (++slot == kStages) slot = 0, phase ^= 1u;
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && pr == 0) {
+        if (pr == 0) {
             const WaitCtx w{abort_flag, p.status, 13};
-            uint32_t slot = 0, phase = 0, acc_phase = 0;
+            uint32_t slot = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
-            for (int32_t t = cluster; ok && t < tiles; t += stride, acc_phase ^= 1u) {
-                if (!SPLIT) {                 // the accumulator has been drained (passes at once for the first tile)
+            for (int32_t t = cluster; ok && t < tiles; t += stride) {
+                if (!SPLIT) {                 // the accumulator has been drained (passes at once while it is fresh)
                     const long long t0 = clock64();
-                    while (!try_wait_cluster(bar_tempty, acc_phase ^ 1u)) {
-                        if (*abort_flag) { ok = false; break; }
-                        if (clock64() - t0 > kWaitLimitCycles) {
+                    while (!__all_sync(0xffffffffu, try_wait_cluster(bar_tempty + 8 * acc, acc_phase ^ 1u))) {
+                        ok = __all_sync(0xffffffffu, *abort_flag == 0 && clock64() - t0 <= kWaitLimitCycles);
+                        if (!ok) {
                             *abort_flag = 1;
-                            atomicCAS(p.status, 0, w.code | (int)(blockIdx.x << 8));
-                            ok = false;
+                            if (lane == 0) atomicCAS(p.status, 0, w.code | (int)(blockIdx.x << 8));
                             break;
                         }
                     }
                     if (!ok) break;
                     ptx::tc_fence_after();
                 }
+                const uint32_t d = tmem + acc * BN;
                 for (int32_t k = k0; k < k1; ++k) {
-                    if (!wait_bar(bar_full + 8 * slot, phase, w)) { ok = false; break; }
+                    ok = __all_sync(0xffffffffu, wait_bar(bar_full + 8 * slot, phase, w));
+                    if (!ok) break;
                     ptx::tc_fence_after();
                     const uint32_t a = tiles_smem + slot * kOperandBytes, s = sf_smem + slot * kSfBytes;
                     const uint64_t a_desc = ptx::umma_desc_k_sw128(a), b_desc = ptx::umma_desc_k_sw128(a + kABytes);
                     const int halves = min(2, p.kblocks - 2 * k);      // the last step may hold one 128-K block only
                     for (int h = 0; h < halves; ++h) {
-                        const uint32_t sfa = tmem + kColSfa + 4 * h, sfb = tmem + kColSfb + 8 * h;
-                        ptx::tmem_cp_32x128b_warpx4_pair(sfa, ptx::umma_desc_sf(s + 512 * h));
-                        ptx::tmem_cp_32x128b_warpx4_pair(sfb, ptx::umma_desc_sf(s + 1024 + 512 * h));
-                        ptx::tmem_cp_32x128b_warpx4_pair(sfb + 4, ptx::umma_desc_sf(s + 2048 + 512 * h));
-                        mma_mxf4_pair(tmem, a_desc + 4 * h, b_desc + 4 * h, idesc_mxf4(kTileM, kTileN, 0), sfa, sfb, (k > k0 || h > 0) ? 1u : 0u);
-                        mma_mxf4_pair(tmem, a_desc + 4 * h + 2, b_desc + 4 * h + 2, idesc_mxf4(kTileM, kTileN, 2), sfa, sfb, 1u);
+                        const uint32_t sfa = tmem + kColScales + 16 * h, sfb = sfa + 4;
+#pragma unroll
+                        for (int b = 0; b < F::kSfBlocks; ++b) copy_scales_pair(sfa + 4 * b, ptx::umma_desc_sf(s + 1024 * b + 512 * h));
+                        mma_mxf4_pair(d, a_desc + 4 * h, b_desc + 4 * h, idesc_mxf4(kTileM, BN, 0), sfa, sfb, (k > k0 || h > 0) ? 1u : 0u);
+                        mma_mxf4_pair(d, a_desc + 4 * h + 2, b_desc + 4 * h + 2, idesc_mxf4(kTileM, BN, 2), sfa, sfb, 1u);
                     }
-                    ptx::mma_commit_pair(bar_empty + 8 * slot, pair_mask);
+                    commit_pair(bar_empty + 8 * slot, pair_mask);
                     if (++slot == kStages) slot = 0, phase ^= 1u;
                 }
-                if (ok) ptx::mma_commit_pair(bar_tfull, pair_mask);
+                if (ok) commit_pair(bar_tfull + 8 * acc, pair_mask);
+                if (++acc == F::kAccs) acc = 0, acc_phase ^= 1u;
             }
         }
     } else if (!SPLIT) {
         const WaitCtx w{abort_flag, p.status, 14};
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t release = ptx::mapa(bar_tempty, leader);
-        uint32_t phase = 0;
-        for (int32_t t = cluster; t < tiles; t += stride, phase ^= 1u) {
-            if (!wait_bar(bar_tfull, phase, w)) break;
-            __syncwarp();
+        const uint32_t mine = ptx::smem_u32(staging) + (uint32_t)(warp - 2) * (32 * 128);
+        uint32_t acc = 0, phase = 0;
+        constexpr int kCols = BN / 2, kChunks = kCols / 32;      // of this warp
+        for (int32_t t = cluster; t < tiles; t += stride) {
+            if (!__all_sync(0xffffffffu, wait_bar(bar_tfull + 8 * acc, phase, w))) break;
             ptx::tc_fence_after();
             int32_t mt, nt;
             tile_of(t, p, mt, nt);
-            uint32_t r[4][32];
+            uint32_t r[kChunks][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + half * 128 + c * 32, r[c]);
+            for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + half * kCols + c * 32, r[c]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) ptx::tmem_ld_wait(r[c]);
+            for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_wait(r[c]);
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_cluster(release);
-            const int32_t row = mt * kTileM + (int32_t)pr * 128 + quarter * 32 + lane;
-            if (row < p.M && *abort_flag == 0) {
+            if (lane == 0) arrive_cluster(ptx::mapa(bar_tempty + 8 * acc, leader));
+            if (++acc == F::kAccs) acc = 0, phase ^= 1u;
+            const int32_t row0 = mt * kTileM + (int32_t)pr * 128 + quarter * 32;
+            if (row0 >= p.M || *abort_flag != 0) continue;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float f[32];
+            for (int c = 0; c < kChunks; ++c) {
+                const int32_t n0 = nt * BN + half * kCols + c * 32;
+                float f[32];
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(r[c][q]);
-                    store_row(f, p, row, nt * kTileN + half * 128 + c * 32);
+                for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(r[c][q]);
+                add_bias(f, p, n0);
+                if (p.tiled_out) {
+                    if ((c & 1) == 0) {
+                        stores_have_read();      // nothing to wait for in lanes that stored nothing
+                        __syncwarp();
+                    }
+                    stage_row(f, mine, lane, c & 1);
+                    if ((c & 1) == 1 && n0 - 32 < p.N) {
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        store_box(&tmC, (n0 - 32) * 2, row0, mine);
+                    }
+                } else if (row0 + lane < p.M) {
+                    store_row(f, p, row0 + lane, n0);
                 }
             }
         }
+        stores_have_read();              // the shared memory may go once they have
     } else {
         const WaitCtx w{abort_flag, p.status, 15};
         wait_bar(bar_tfull, 0u, w);
+        __syncwarp();
         ptx::tc_fence_after();
     }
 
@@ -272,7 +360,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         const int32_t live = max(0, min(p.M - row0, 128));
         __syncwarp();
         ptx::cluster_sync();              // every CTA of the cluster is done with its stages: they may be overwritten
-        const int W = kTileN / p.S;
+        const int W = BN / p.S;
         const uint32_t slot_bytes = (uint32_t)(128 * W * 4), units = (uint32_t)W / 4u;
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int r_in_tile = quarter * 32 + lane;
@@ -281,7 +369,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         // lane per row stores without bank conflicts; one bulk copy per owner
         if (warp >= 2) {
 #pragma unroll 1
-            for (int cc = half; cc < kTileN / 32; cc += 2) {
+            for (int cc = half; cc < BN / 32; cc += 2) {
                 const uint32_t o = (uint32_t)(32 * cc / W);
                 if (o == ks) continue;
                 uint32_t r[32];
@@ -311,7 +399,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             __syncwarp();
             if (quarter * 32 < live) {
 #pragma unroll 1
-                for (int cc = half; cc < kTileN / 32; cc += 2) {
+                for (int cc = half; cc < BN / 32; cc += 2) {
                     if ((uint32_t)(32 * cc / W) != ks) continue;
                     uint32_t r[32];
                     ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + 32 * cc, r);
@@ -335,7 +423,8 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                                 f[4 * i + 0] += v.x; f[4 * i + 1] += v.y; f[4 * i + 2] += v.z; f[4 * i + 3] += v.w;
                             }
                         }
-                        store_row(f, p, row0 + r_in_tile, nt * kTileN + 32 * cc);
+                        add_bias(f, p, nt * BN + 32 * cc);
+                        store_row(f, p, row0 + r_in_tile, nt * BN + 32 * cc);
                     }
                 }
             }
@@ -356,15 +445,15 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// Codes [rows, K]: boxes of 128 rows x 256 values (128 bytes, 128-byte swizzle).
-static int code_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K, bool weights) {
+// Codes [rows, K]: boxes of box_rows x 256 values (128 bytes, 128-byte swizzle).
+static int code_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K, int box_rows, bool weights) {
     TensorMapSpec t;
     memset(&t, 0, sizeof(t));
     t.base = base;
     t.rank = 2;
     t.dims[0] = (uint64_t)(K / 2); t.dims[1] = (uint64_t)rows; t.dims[2] = 1;
     t.strides[0] = (uint64_t)(K / 2);
-    t.box[0] = 128; t.box[1] = 128; t.box[2] = 1;
+    t.box[0] = 128; t.box[1] = (uint32_t)box_rows; t.box[2] = 1;
     t.swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
     t.promo = weights ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
     return encode_tensor_map(tm, t);
@@ -383,7 +472,21 @@ static int scale_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t kb
     return encode_tensor_map(tm, t);
 }
 
-template <bool SPLIT>
+// Output [M, N] bf16, row stride ldc: boxes of 32 rows x 64 columns.
+static int out_map(CUtensorMap* tm, const void* base, int64_t M, int64_t N, int64_t ldc) {
+    TensorMapSpec t;
+    memset(&t, 0, sizeof(t));
+    t.base = base;
+    t.rank = 2;
+    t.dims[0] = (uint64_t)N * 2; t.dims[1] = (uint64_t)M; t.dims[2] = 1;
+    t.strides[0] = (uint64_t)ldc * 2;
+    t.box[0] = 128; t.box[1] = 32; t.box[2] = 1;
+    t.swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
+    t.promo = CU_TENSOR_MAP_L2_PROMOTION_NONE;
+    return encode_tensor_map(tm, t);
+}
+
+template <int BN, bool SPLIT>
 static int max_clusters(int size) {
     static int cache[64][9] = {};
     int dev = 0;
@@ -392,7 +495,7 @@ static int max_clusters(int size) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(size * 16));
         cfg.blockDim = dim3(kGemmThreads);
-        cfg.dynamicSmemBytes = kGemmSmem;
+        cfg.dynamicSmemBytes = Cfg<BN>::kSmem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned)size;
@@ -400,8 +503,8 @@ static int max_clusters(int size) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (cudaFuncSetAttribute(mxfp4_gemm_kernel<SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&n, mxfp4_gemm_kernel<SPLIT>, &cfg) != cudaSuccess) {
+        if (cudaFuncSetAttribute(mxfp4_gemm_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::kSmem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, mxfp4_gemm_kernel<BN, SPLIT>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             n = 0;
         }
@@ -410,36 +513,40 @@ static int max_clusters(int size) {
     return cache[dev][size] > 0 ? cache[dev][size] : 0;
 }
 
-// K-slices for a problem with too few tiles for one pair each: the most that are resident at once and leave every slice a
-// step; 1: persistent pairs.
-static int plan_split(const GemmArgs& p) {
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    for (int S = 4; S >= 2; S /= 2) {
-        const int per = (p.steps + S - 1) / S;
-        if (2 * S * tiles > sm_count() || (S - 1) * per >= p.steps) continue;
-        if (tiles <= max_clusters<true>(2 * S)) return S;
-    }
-    return 1;
-}
-
-template <bool SPLIT>
-static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const GemmArgs& p, unsigned grid, cudaStream_t st) {
+template <int BN, bool SPLIT>
+static int launch(const void* A, const void* sfa, const void* B, const void* sfb, int64_t K, const GemmArgs& p, unsigned clusters, cudaStream_t st) {
+    CUtensorMap a, b, sa, sb, c;
+    int rc;
+    if ((rc = code_map(&a, A, p.M, K, 128, false)) != KBN_OK || (rc = code_map(&b, B, p.N, K, BN / 2, true)) != KBN_OK ||
+        (rc = scale_map(&sa, sfa, p.M, p.kblocks)) != KBN_OK || (rc = scale_map(&sb, sfb, p.N, p.kblocks)) != KBN_OK)
+        return rc;
+    c = a;                               // never read without tiled_out
+    if (p.tiled_out && (rc = out_map(&c, p.C, p.M, p.N, p.ldc)) != KBN_OK) return rc;
+    const unsigned size = SPLIT ? 2u * (unsigned)p.S : 2u;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(clusters * size);
     cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = kGemmSmem;
+    cfg.dynamicSmemBytes = Cfg<BN>::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)(SPLIT ? 2 * p.S : 2);
+    attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    KBN_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<SPLIT>, a, b, sa, sb, p));
+    KBN_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BN, SPLIT>, a, b, sa, sb, c, p));
     KBN_CHECK_LAUNCH();
     return KBN_OK;
+}
+
+template <int BN>
+static int launch_persistent(const void* A, const void* sfa, const void* B, const void* sfb, int64_t K, const GemmArgs& p, cudaStream_t st) {
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const int pairs = max_clusters<BN, false>(2);
+    KBN_REQUIRE(pairs > 0, KBN_ERR_UNSUPPORTED, "kbn_mxfp4_gemm_nt: no CTA pair fits this device");
+    return launch<BN, false>(A, sfa, B, sfb, K, p, (unsigned)std::min<int64_t>(tiles, pairs), st);
 }
 
 }  // namespace mxfp4
@@ -467,18 +574,25 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const vo
     p.kblocks = (int32_t)kblocks;
     p.steps = (int32_t)((kblocks + 1) / 2);
     p.m_tiles = (int32_t)((M + kTileM - 1) / kTileM);
-    p.n_tiles = (int32_t)((N + kTileN - 1) / kTileN);
     int rc = gemm_status_ptr(&p.status);
     if (rc != KBN_OK) return rc;
-    CUtensorMap a, b, sa, sb;
-    if ((rc = code_map(&a, A, M, K, false)) != KBN_OK || (rc = code_map(&b, B, N, K, true)) != KBN_OK || (rc = scale_map(&sa, sfa_packed, M, kblocks)) != KBN_OK ||
-        (rc = scale_map(&sb, sfb_packed, N, kblocks)) != KBN_OK)
-        return rc;
-    p.S = plan_split(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    if (p.S > 1) return launch<true>(a, b, sa, sb, p, (unsigned)(tiles * 2 * p.S), st);
-    const int pairs = max_clusters<false>(2);
-    KBN_REQUIRE(pairs > 0, KBN_ERR_UNSUPPORTED, "kbn_mxfp4_gemm_nt: no CTA pair fits this device");
-    return launch<false>(a, b, sa, sb, p, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), st);
+    if (M == 1) p.ldc = (N + 7) / 8 * 8;      // the stride of a single row is free
+    p.tiled_out = aligned16(C) && p.ldc % 8 == 0;
+    const int64_t wide = p.m_tiles * ((N + 255) / 256), narrow = p.m_tiles * ((N + 127) / 128);
+    // Few tiles: K split over the cluster, the most slices that are resident at once and leave each a step.
+    p.n_tiles = (int32_t)((N + 255) / 256);
+    for (int S = 4; S >= 2; S /= 2) {
+        const int per = (p.steps + S - 1) / S;
+        if (2 * S * wide > sm_count() || (S - 1) * per >= p.steps || wide > max_clusters<256, true>(2 * S)) continue;
+        p.S = S;
+        return launch<256, true>(A, sfa_packed, B, sfb_packed, K, p, (unsigned)wide, st);
+    }
+    const int64_t pairs = sm_count() / 2;
+    // 128 columns a tile while every pair then has one tile at most; more rounds of them cost 0.75 of a round of wide ones each.
+    if (narrow <= pairs) {
+        p.n_tiles = (int32_t)((N + 127) / 128);
+        return launch_persistent<128>(A, sfa_packed, B, sfb_packed, K, p, st);
+    }
+    return launch_persistent<256>(A, sfa_packed, B, sfb_packed, K, p, st);
 }

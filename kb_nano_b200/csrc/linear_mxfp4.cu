@@ -18,7 +18,7 @@ constexpr int kLinearFixed = 1024 + kRedBytes + 256 + 128;      // alignment, pa
 struct LinearArgs {
     const __nv_bfloat16* x;
     int64_t ld_x;
-    ScaleSource s;
+    const void* sfb;               // packed weight scales
     const __nv_bfloat16* bias;
     __nv_bfloat16* C;
     int64_t ldc;
@@ -112,7 +112,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     if (warp == kProducerWarp) {
         const WaitCtx w{abort_flag, a.status, 17};
         RingPos pos;
-        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, a.s, 16 * u, 16 * u + 8, a.N, KC, lane, w);
+        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, 16 * u, 16 * u + 8, a.N, KC, lane, w);
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
         RingPos pos;
@@ -148,7 +148,7 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     LinearArgs a{};
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ld_x = ld_x;
-    a.s = ScaleSource{sfb_packed};
+    a.sfb = sfb_packed;
     a.bias = static_cast<const __nv_bfloat16*>(bias);
     a.C = static_cast<__nv_bfloat16*>(C);
     a.ldc = ldc;
@@ -160,7 +160,9 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     CUtensorMap tm;
     rc = weight_map<kMxfp4>(&tm, B, N, K);
     if (rc != KBN_OK) return rc;
-    KBN_CUDA(cudaFuncSetAttribute(mxfp4_linear_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    static std::atomic<uint64_t> allowed{0};
+    rc = allow_smem(mxfp4_linear_few_kernel, allowed);
+    if (rc != KBN_OK) return rc;
     const int64_t units = (N + 15) / 16;
     const unsigned grid = (unsigned)std::min<int64_t>(units, sm_count());
     const size_t smem = (size_t)(kLinearFixed + M * (a.token_stride + K / 32) + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));

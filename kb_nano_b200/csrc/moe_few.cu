@@ -35,7 +35,8 @@ struct MoeArgs {
     const __nv_bfloat16* x;
     int64_t ld_x;
     int32_t T, topk, H, I, E, group;
-    ScaleSource s13, s2;
+    const void *s13, *s2;          // weight scales
+    int32_t tiled13, tiled2;       // their loads are tiled (MXFP4, K % 512 == 0)
     float* y;                      // [pairs, I]
     float* rows;                   // [pairs, H]
     Jobs* jobs;
@@ -124,7 +125,7 @@ __device__ __forceinline__ void drain_after_abort(const volatile int* abort_flag
 
 template <int FMT, int PER>
 __global__ void __launch_bounds__(kThreads, 1)
-few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, const int logits_bf16, const MoeArgs a) {
+few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_scales, const RouteArgs ra, const int logits_bf16, const MoeArgs a) {
     extern __shared__ uint8_t raw[];
     Scratch* scp;
     const Smem s = carve<FMT>(raw, a.stages, a.token_rows, a.token_stride, &scp);
@@ -188,7 +189,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const RouteArgs ra, c
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * 2 * a.I + 8 * rb;
-            produce_unit<FMT>(s, pos, &tm, a.s13, row, row + a.I, 2 * a.I * a.E, KC, lane, w);
+            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s13, a.tiled13 ? &tm_scales : nullptr}, row, row + a.I, 2 * a.I * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
     } else if (warp < kConsumerWarps) {
@@ -251,7 +252,7 @@ __device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" 
 
 template <int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
-few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
+few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_scales, const MoeArgs a) {
     extern __shared__ uint8_t raw[];
     Scratch* scp;
     const Smem s = carve<FMT>(raw, a.stages, a.token_rows, a.token_stride, &scp);
@@ -286,7 +287,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const MoeArgs a) {
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * a.H + 16 * rb;
-            produce_unit<FMT>(s, pos, &tm, a.s2, row, row + 8, a.H * a.E, KC, lane, w);
+            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + 8, a.H * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
     } else if (warp < kConsumerWarps) {
@@ -362,12 +363,6 @@ static bool plan(int64_t K, int want, Plan* p) {
     return false;
 }
 
-template <typename Kernel>
-static int allow_smem(Kernel kernel) {
-    KBN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
-    return KBN_OK;
-}
-
 struct WorkspaceLayout {
     int64_t jobs, counters, y, rows, total;
 };
@@ -399,23 +394,30 @@ static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& 
     if (rc != KBN_OK) return rc;
     rc = weight_map<FMT>(&t2, w2, (int64_t)a.E * a.H, a.I);
     if (rc != KBN_OK) return rc;
+    // FP8: never read; the kernels take a map all the same
+    CUtensorMap t13s = t13, t2s = t2;
+    a.tiled13 = FMT == kMxfp4 && a.H % 512 == 0 && aligned16(a.s13);
+    a.tiled2 = FMT == kMxfp4 && a.I % 512 == 0 && aligned16(a.s2);
+    if (a.tiled13 && (rc = scale_rows_map(&t13s, a.s13, (int64_t)a.E * 2 * a.I, a.H)) != KBN_OK) return rc;
+    if (a.tiled2 && (rc = scale_rows_map(&t2s, a.s2, (int64_t)a.E * a.H, a.I)) != KBN_OK) return rc;
     rc = gemm_status_ptr(&a.status);
     if (rc != KBN_OK) return rc;
     auto up_kernel = a.E <= 256 ? few_gate_up_kernel<FMT, 8> : few_gate_up_kernel<FMT, 32>;
-    rc = allow_smem(up_kernel);
+    static std::atomic<uint64_t> up_small{0}, up_large{0}, down{0};
+    rc = allow_smem(up_kernel, a.E <= 256 ? up_small : up_large);
     if (rc != KBN_OK) return rc;
-    rc = allow_smem(few_down_kernel<FMT>);
+    rc = allow_smem(few_down_kernel<FMT>, down);
     if (rc != KBN_OK) return rc;
     const unsigned grid = (unsigned)sm_count();
     a.stages = p1.stages;
     a.token_rows = p1.rows;
     a.token_stride = p1.token_stride;
-    KBN_CUDA(launch_pdl(up_kernel, dim3(grid), dim3(kThreads), p1.smem, st, t13, ra, logits_bf16, a));
+    KBN_CUDA(launch_pdl(up_kernel, dim3(grid), dim3(kThreads), p1.smem, st, t13, t13s, ra, logits_bf16, a));
     KBN_CHECK_LAUNCH();
     a.stages = p2.stages;
     a.token_rows = p2.rows;
     a.token_stride = p2.token_stride;
-    KBN_CUDA(launch_pdl(few_down_kernel<FMT>, dim3(grid), dim3(kThreads), p2.smem, st, t2, a));
+    KBN_CUDA(launch_pdl(few_down_kernel<FMT>, dim3(grid), dim3(kThreads), p2.smem, st, t2, t2s, a));
     KBN_CHECK_LAUNCH();
     return KBN_OK;
 }
@@ -461,8 +463,8 @@ extern "C" int kbn_moe_few_tokens(const void* x, int64_t ld_x, int64_t T, const 
     a.x = static_cast<const __nv_bfloat16*>(x);
     a.ld_x = ld_x;
     a.T = (int32_t)T; a.topk = (int32_t)topk; a.H = (int32_t)H; a.I = (int32_t)I; a.E = (int32_t)E;
-    a.s13 = ScaleSource{w13_s};
-    a.s2 = ScaleSource{w2_s};
+    a.s13 = w13_s;
+    a.s2 = w2_s;
     a.jobs = reinterpret_cast<Jobs*>(ws + wl.jobs);
     a.counters = reinterpret_cast<int32_t*>(ws + wl.counters);
     a.y = reinterpret_cast<float*>(ws + wl.y);

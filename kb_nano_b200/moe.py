@@ -162,49 +162,54 @@ def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13
     if hidden_states.dim() != 2 or hidden_states.dtype != torch.bfloat16 or hidden_states.stride(1) != 1:
         raise ValueError("hidden_states must be bf16 [T, H], contiguous along H")
     t, h = hidden_states.shape
-    if router_logits.dim() != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16) or router_logits.shape[0] != t or router_logits.stride(1) != 1:
+    if router_logits.dim() != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16) or router_logits.size(0) != t or router_logits.stride(1) != 1:
         raise ValueError(f"router_logits must be fp32 or bf16 [{t}, E], contiguous along E")
-    if not 0 <= t <= FEW_TOKENS_MAX:
+    if t > FEW_TOKENS_MAX:
         raise ValueError(f"few_tokens_moe takes at most {FEW_TOKENS_MAX} tokens, got {t}")
-    e = router_logits.shape[1]
+    e = router_logits.size(1)
     if w13.dtype == FP8 and w2.dtype == FP8:
-        fmt, i = 0, w2.shape[-1]
-        want = ((e, 2 * i, h), (e, h, i), (e, (2 * i + 127) // 128, (h + 127) // 128), (e, (h + 127) // 128, (i + 127) // 128))
-        scale_types = (torch.float32,)
+        fmt, i = 0, w2.size(-1)
+        h_in, i_in, rows13, rows2, h_sc, i_sc, scale_types = h, i, (2 * i + 127) // 128, (h + 127) // 128, (h + 127) // 128, (i + 127) // 128, (torch.float32,)
     elif w13.dtype in ops._CODE_DTYPES and w2.dtype in ops._CODE_DTYPES:
-        fmt, i = 1, w2.shape[-1] * 2
-        want = ((e, 2 * i, h // 2), (e, h, i // 2), (e, 2 * i, h // 32), (e, h, i // 32))
-        scale_types = ops._BYTE_SCALE_DTYPES
+        fmt, i = 1, w2.size(-1) * 2
+        h_in, i_in, rows13, rows2, h_sc, i_sc, scale_types = h // 2, i // 2, 2 * i, h, h // 32, i // 32, ops._BYTE_SCALE_DTYPES
     else:
         raise ValueError(f"w13 and w2 must both be float8_e4m3fn or both MXFP4 codes (uint8), got {w13.dtype} and {w2.dtype}")
     if h % 128 or i % 128:
         raise ValueError(f"hidden size {h} and intermediate size {i} must be multiples of 128")
-    for name, x, shape in zip(("w13", "w2", "w13_scale", "w2_scale"), (w13, w2, w13_scale, w2_scale), want):
-        if tuple(x.shape) != shape or not x.is_contiguous() or (name.endswith("scale") and x.dtype not in scale_types):
-            raise ValueError(f"{name} must be contiguous {shape}{'' if not name.endswith('scale') else f' {scale_types[0]}'}, got {x.dtype} {tuple(x.shape)}")
+    if w13.shape != (e, 2 * i, h_in) or not w13.is_contiguous():
+        raise ValueError(f"w13 must be contiguous {(e, 2 * i, h_in)}, got {tuple(w13.shape)}")
+    if w2.shape != (e, h, i_in) or not w2.is_contiguous():
+        raise ValueError(f"w2 must be contiguous {(e, h, i_in)}, got {tuple(w2.shape)}")
+    if w13_scale.shape != (e, rows13, h_sc) or not w13_scale.is_contiguous() or w13_scale.dtype not in scale_types:
+        raise ValueError(f"w13_scale must be contiguous {scale_types[0]} {(e, rows13, h_sc)}, got {w13_scale.dtype} {tuple(w13_scale.shape)}")
+    if w2_scale.shape != (e, rows2, i_sc) or not w2_scale.is_contiguous() or w2_scale.dtype not in scale_types:
+        raise ValueError(f"w2_scale must be contiguous {scale_types[0]} {(e, rows2, i_sc)}, got {w2_scale.dtype} {tuple(w2_scale.shape)}")
     if out is None:
         out = torch.empty(t, h, dtype=torch.bfloat16, device=hidden_states.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (t, h) or out.stride(1) != 1:
+    elif out.dtype != torch.bfloat16 or out.shape != (t, h) or out.stride(1) != 1:
         raise ValueError(f"out must be bf16 [{t}, {h}], contiguous along H")
-    if (out_w is None) != (out_ids is None):
-        raise ValueError("out_w and out_ids come together")
-    if out_w is not None:
-        if out_w.dtype != torch.float32 or tuple(out_w.shape) != (t, top_k) or not out_w.is_contiguous():
+    index = ops._gpu(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, out)
+    w_ptr = ids_ptr = bias_ptr = None
+    if out_w is not None or out_ids is not None:
+        if out_w is None or out_ids is None:
+            raise ValueError("out_w and out_ids come together")
+        if out_w.dtype != torch.float32 or out_w.shape != (t, top_k) or not out_w.is_contiguous():
             raise ValueError("out_w must be contiguous float32 [T, top_k]")
-        if out_ids.dtype != torch.int32 or tuple(out_ids.shape) != (t, top_k) or not out_ids.is_contiguous():
+        if out_ids.dtype != torch.int32 or out_ids.shape != (t, top_k) or not out_ids.is_contiguous():
             raise ValueError("out_ids must be contiguous int32 [T, top_k]")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != e or not bias.is_contiguous()):
-        raise ValueError("bias must be contiguous float32 [E]")
-    dev = ops._cuda(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, out, *(x for x in (bias, out_w, out_ids) if x is not None))
+        ops._gpu(out, out_w, out_ids)
+        w_ptr, ids_ptr = out_w.data_ptr(), out_ids.data_ptr()
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.numel() != e or not bias.is_contiguous():
+            raise ValueError("bias must be contiguous float32 [E]")
+        ops._gpu(out, bias)
+        bias_ptr = bias.data_ptr()
     lib = _lib.load()
-    with ops._on(dev):
-        # allocated on the calling stream's account: the allocator hands it to nobody else before this call's kernels have run
-        nbytes = int(lib.kbn_moe_few_tokens_workspace_bytes(t, top_k, h, i))
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        _lib.check(lib.kbn_moe_few_tokens(
-            hidden_states.data_ptr(), hidden_states.stride(0) if t > 1 else h, t, router_logits.data_ptr(), int(router_logits.dtype == torch.bfloat16),
-            router_logits.stride(0) if t > 1 else e, e, int(scoring == "softmax"), bias.data_ptr() if bias is not None else None, n_group, topk_group,
-            top_k, int(renormalize), renorm_floor, scale, int(round_bf16), fmt, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
-            h, i, out.data_ptr(), out.stride(0) if t > 1 else h, out_w.data_ptr() if out_w is not None else None,
-            out_ids.data_ptr() if out_ids is not None else None, ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream))
+    # allocated on the calling stream's account: the allocator hands it to nobody else before this call's kernels have run
+    ws = torch.empty(lib.kbn_moe_few_tokens_workspace_bytes(t, top_k, h, i), dtype=torch.uint8, device=hidden_states.device)
+    ops._call(index, lib.kbn_moe_few_tokens, hidden_states.data_ptr(), hidden_states.stride(0) if t > 1 else h, t, router_logits.data_ptr(),
+              router_logits.dtype == torch.bfloat16, router_logits.stride(0) if t > 1 else e, e, scoring == "softmax", bias_ptr, n_group, topk_group, top_k,
+              bool(renormalize), renorm_floor, scale, bool(round_bf16), fmt, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), h, i,
+              out.data_ptr(), out.stride(0) if t > 1 else h, w_ptr, ids_ptr, ws.data_ptr(), ws.numel())
     return out

@@ -16,8 +16,14 @@ FP8 = torch.float8_e4m3fn
 GROUP = 128
 
 
+# The handle of a device's current stream without building a torch.cuda.Stream around it (2.3 us against 0.1).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # only called with a CUDA tensor at hand
+
+
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.get_device())
 
 
 def _cuda(*tensors: torch.Tensor) -> torch.device:
@@ -646,119 +652,148 @@ def packed_mxfp4_bytes(rows: int, k: int) -> int:
     return (rows + 127) // 128 * ((k + 127) // 128) * 512
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor; that of a single row is free in torch and is taken as the row's length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _gpu(*tensors: torch.Tensor) -> int:
+    """Index of the one GPU all tensors are on (the checks of _cuda, cheaper: small calls are bound by the host)."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            _cuda(*tensors)
+    return index
 
 
-def _check_codes(q: torch.Tensor, m: int, k: int, what: str) -> None:
-    if q.dtype not in _CODE_DTYPES or tuple(q.shape) != (m, k // 2) or q.stride(1) != 1:
-        raise ValueError(f"{what} must be uint8 (or float4_e2m1fn_x2) [{m}, {k // 2}], contiguous along the last dim, got {q.dtype} {tuple(q.shape)}")
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, current stream of GPU `index`), with that GPU current."""
+    if index == _current_device():
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code:
+        _lib.check(code)
 
 
-def _check_byte_scales(s: torch.Tensor, m: int, k: int, what: str) -> None:
-    if s.dtype not in _BYTE_SCALE_DTYPES or tuple(s.shape) != (m, k // MX_BLOCK) or (s.stride(1) != 1 and s.shape[1] > 1):
-        raise ValueError(f"{what} must be uint8 (or float8_e8m0fnu) [{m}, {k // MX_BLOCK}], contiguous along the last dim, got {s.dtype} {tuple(s.shape)}")
+# The three checks below return the tensor's row stride; that of a single row is free in torch and is taken as its length.
+
+def _bf16_rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a bf16 matrix with contiguous rows."""
+    if t.dtype != torch.bfloat16 or t.dim() != 2:
+        raise ValueError(f"{what} must be a bf16 matrix, got {t.dtype} {tuple(t.shape)}")
+    m, n = t.shape
+    ld, step = t.stride()
+    if step != 1 and n > 1:
+        raise ValueError(f"{what} must be contiguous along the last dim, got strides {t.stride()}")
+    return m, n, ld if m > 1 else n
 
 
-def _check_packed_mxfp4(buf: torch.Tensor, rows: int, k: int, dev, what: str) -> None:
-    need = packed_mxfp4_bytes(rows, k)
-    if buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.device != dev or buf.numel() < need or buf.data_ptr() % 16:
-        raise ValueError(f"{what} must be a contiguous, 16-byte aligned uint8 buffer on {dev} with at least {need} bytes")
+def _check_codes(q: torch.Tensor, m: int, k: int, what: str) -> int:
+    if q.dtype in _CODE_DTYPES and q.shape == (m, k // 2):
+        ld, step = q.stride()
+        if step == 1:
+            return ld if m > 1 else k // 2
+    raise ValueError(f"{what} must be uint8 (or float4_e2m1fn_x2) [{m}, {k // 2}], contiguous along the last dim, got {q.dtype} {tuple(q.shape)}")
 
 
-def _quant_mxfp4_call(fn: str, x: torch.Tensor, k: int, out_fp4: torch.Tensor, out_scale: torch.Tensor | None, packed_sf: torch.Tensor | None) -> None:
-    m = x.shape[0]
-    dev = _cuda(x, out_fp4, *(t for t in (out_scale, packed_sf) if t is not None))
+def _check_byte_scales(s: torch.Tensor, m: int, k: int, what: str) -> int:
+    if s.dtype in _BYTE_SCALE_DTYPES and s.shape == (m, k // MX_BLOCK):
+        ld, step = s.stride()
+        if step == 1 or k == MX_BLOCK:
+            return ld if m > 1 else k // MX_BLOCK
+    raise ValueError(f"{what} must be uint8 (or float8_e8m0fnu) [{m}, {k // MX_BLOCK}], contiguous along the last dim, got {s.dtype} {tuple(s.shape)}")
+
+
+def _check_packed_mxfp4(buf: torch.Tensor, rows: int, k: int, what: str) -> int:
+    """Address of a packed scale buffer of [rows, k] values."""
+    ptr = buf.data_ptr()
+    if ptr & 15 or buf.dtype != torch.uint8 or buf.numel() < packed_mxfp4_bytes(rows, k) or not buf.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous, 16-byte aligned uint8 buffer with at least {packed_mxfp4_bytes(rows, k)} bytes")
+    return ptr
+
+
+def _quant_mxfp4_call(fn, x: torch.Tensor, m: int, k: int, ld: int, out_fp4: torch.Tensor, out_scale: torch.Tensor | None,
+                      packed_sf: torch.Tensor | None) -> None:
     if k % MX_BLOCK:
         raise ValueError(f"the quantised dimension ({k}) must be a multiple of {MX_BLOCK}")
-    _check_codes(out_fp4, m, k, "out_fp4")
-    if out_scale is None and packed_sf is None:
-        raise ValueError("give out_scale (row-major scales), packed_sf (the GEMM's layout) or both")
+    ld_q = _check_codes(out_fp4, m, k, "out_fp4")
+    scale_ptr, scale_stride, packed_ptr, index = None, 0, None, x.get_device()
+    if index < 0 or out_fp4.get_device() != index:
+        _cuda(x, out_fp4)
     if out_scale is not None:
-        _check_byte_scales(out_scale, m, k, "out_scale")
+        scale_stride = _check_byte_scales(out_scale, m, k, "out_scale")
+        if out_scale.get_device() != index:
+            _cuda(x, out_scale)
+        scale_ptr = out_scale.data_ptr()
     if packed_sf is not None:
-        _check_packed_mxfp4(packed_sf, m, k, dev, "packed_sf")
-    with _on(dev):
-        _lib.check(getattr(_lib.load(), fn)(x.data_ptr(), m, k, _row_stride(x), out_fp4.data_ptr(), _row_stride(out_fp4),
-                                            out_scale.data_ptr() if out_scale is not None else None,
-                                            _row_stride(out_scale) if out_scale is not None else 0,
-                                            packed_sf.data_ptr() if packed_sf is not None else None, _stream(x)))
+        packed_ptr = _check_packed_mxfp4(packed_sf, m, k, "packed_sf")
+        if packed_sf.get_device() != index:
+            _cuda(x, packed_sf)
+    elif out_scale is None:
+        raise ValueError("give out_scale (row-major scales), packed_sf (the GEMM's layout) or both")
+    _call(index, fn, x.data_ptr(), m, k, ld, out_fp4.data_ptr(), ld_q, scale_ptr, scale_stride, packed_ptr)
 
 
 def quant_mxfp4(x: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor | None = None, packed_sf: torch.Tensor | None = None) -> None:
     """x bf16 [M,K] -> MXFP4: out_fp4 uint8 [M,K/2] and the E8M0 scales of its blocks of 32, row-major in out_scale uint8
     [M,K/32] and / or in the packed form of mxfp4_gemm_nt in packed_sf (uint8, packed_mxfp4_bytes(M, K) bytes).  The scale is
     the smallest power of two that clips nothing; a block with an infinity or a NaN becomes NaN."""
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
-        raise ValueError(f"x must be bf16 [M,K], contiguous along K, got {x.dtype} {tuple(x.shape)}")
-    _quant_mxfp4_call("kbn_quant_mxfp4", x, x.shape[1], out_fp4, out_scale, packed_sf)
+    m, k, ld = _bf16_rows(x, "x")
+    _quant_mxfp4_call(_lib.load().kbn_quant_mxfp4, x, m, k, ld, out_fp4, out_scale, packed_sf)
 
 
 def silu_mul_quant_mxfp4(inp: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor | None = None, packed_sf: torch.Tensor | None = None) -> None:
     """inp bf16 [M, 2*N2] (gate | up) -> bf16(bf16(silu(gate)) * up) in MXFP4, [M, N2]; outputs as in quant_mxfp4."""
-    if inp.dim() != 2 or inp.dtype != torch.bfloat16 or inp.stride(1) != 1 or inp.shape[1] % 2:
-        raise ValueError(f"inp must be bf16 [M, 2*N2], contiguous along the last dim, got {inp.dtype} {tuple(inp.shape)}")
-    _quant_mxfp4_call("kbn_silu_mul_quant_mxfp4", inp, inp.shape[1] // 2, out_fp4, out_scale, packed_sf)
+    m, n, ld = _bf16_rows(inp, "inp")
+    if n % 2:
+        raise ValueError(f"inp must hold gate and up halves, got {n} columns")
+    _quant_mxfp4_call(_lib.load().kbn_silu_mul_quant_mxfp4, inp, m, n // 2, ld, out_fp4, out_scale, packed_sf)
 
 
 def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
     """MXFP4 codes [M,K/2] with row-major scales [M,K/32] -> out bf16 [M,K] (exact within bf16's range)."""
-    dev = _cuda(q, scale, out)
-    if out.dim() != 2 or out.dtype != torch.bfloat16 or out.stride(1) != 1 or out.shape[1] % MX_BLOCK:
-        raise ValueError(f"out must be bf16 [M,K], contiguous along K, K a multiple of {MX_BLOCK}, got {out.dtype} {tuple(out.shape)}")
-    m, k = out.shape
-    _check_codes(q, m, k, "q")
-    _check_byte_scales(scale, m, k, "scale")
-    with _on(dev):
-        _lib.check(_lib.load().kbn_dequant_mxfp4(q.data_ptr(), _row_stride(q), scale.data_ptr(), _row_stride(scale), m, k, out.data_ptr(),
-                                                 _row_stride(out), _stream(out)))
+    m, k, ld = _bf16_rows(out, "out")
+    if k % MX_BLOCK:
+        raise ValueError(f"out must have a multiple of {MX_BLOCK} columns, got {k}")
+    ld_q, ld_s, index = _check_codes(q, m, k, "q"), _check_byte_scales(scale, m, k, "scale"), out.get_device()
+    if index < 0 or q.get_device() != index or scale.get_device() != index:
+        _cuda(out, q, scale)
+    _call(index, _lib.load().kbn_dequant_mxfp4, q.data_ptr(), ld_q, scale.data_ptr(), ld_s, m, k, out.data_ptr(), ld)
 
 
 def pack_mxfp4_scales(scale: torch.Tensor, k: int) -> torch.Tensor:
     """Row-major E8M0 scales uint8 [rows, K/32] -> packed uint8 buffer for mxfp4_gemm_nt (done once per weight)."""
     if scale.dim() != 2 or k % MX_BLOCK:
         raise ValueError(f"scale must be 2-D and K={k} a multiple of {MX_BLOCK}")
-    dev = _cuda(scale)
-    rows = scale.shape[0]
-    _check_byte_scales(scale, rows, k, "scale")
-    out = torch.empty(packed_mxfp4_bytes(rows, k), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.check(_lib.load().kbn_pack_mxfp4_scales(scale.data_ptr(), rows, k, _row_stride(scale), out.data_ptr(), _stream(scale)))
+    index, rows = _gpu(scale), scale.size(0)
+    ld = _check_byte_scales(scale, rows, k, "scale")
+    out = torch.empty(packed_mxfp4_bytes(rows, k), dtype=torch.uint8, device=scale.device)
+    _call(index, _lib.load().kbn_pack_mxfp4_scales, scale.data_ptr(), rows, k, ld, out.data_ptr())
     return out
 
 
-def _check_mxfp4_weight(b_q: torch.Tensor, b_sf: torch.Tensor, k: int, dev) -> int:
-    n = b_q.shape[0]
-    _check_codes(b_q, n, k, "b_q")
-    if not b_q.is_contiguous():
-        raise ValueError("b_q must be contiguous")
-    _check_packed_mxfp4(b_sf, n, k, dev, "b_sf")
-    return n
+def _check_mxfp4_operand(q: torch.Tensor, sf: torch.Tensor, rows: int, k: int, what: str) -> int:
+    """Address of the operand's packed scales."""
+    if _check_codes(q, rows, k, what + "_q") != k // 2:
+        raise ValueError(f"{what}_q must be contiguous")
+    return _check_packed_mxfp4(sf, rows, k, what + "_sf")
 
 
-def _check_out(out: torch.Tensor, m: int, n: int) -> None:
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (m, n) or (out.stride(1) != 1 and n > 1):
-        raise ValueError(f"out must be bf16 [{m}, {n}], contiguous along N")
+def _check_out(out: torch.Tensor, m: int, n: int) -> int:
+    rows, cols, ld = _bf16_rows(out, "out")
+    if rows != m or cols != n:
+        raise ValueError(f"out must be bf16 [{m}, {n}], got {tuple(out.shape)}")
+    return ld
 
 
 def mxfp4_gemm_nt(a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
                   bias: torch.Tensor | None = None) -> None:
     """out bf16 [M,N] = MXFP4 a_q [M,K/2] times MXFP4 b_q [N,K/2], transposed (+ bias, in fp32, before the rounding).  a_sf and
     b_sf are the packed scales (quant_mxfp4's packed_sf, pack_mxfp4_scales)."""
-    dev = _cuda(a_q, a_sf, b_q, b_sf, out)
-    if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[1] or a_q.shape[1] % 16:
+    if a_q.dim() != 2 or b_q.dim() != 2 or a_q.size(1) != b_q.size(1) or a_q.size(1) % 16:
         raise ValueError(f"a_q and b_q must be [M, K/2] and [N, K/2] with K a multiple of {MX_BLOCK}, got {tuple(a_q.shape)} and {tuple(b_q.shape)}")
-    m, k = a_q.shape[0], a_q.shape[1] * 2
-    _check_codes(a_q, m, k, "a_q")
-    if not a_q.is_contiguous():
-        raise ValueError("a_q must be contiguous")
-    _check_packed_mxfp4(a_sf, m, k, dev, "a_sf")
-    n = _check_mxfp4_weight(b_q, b_sf, k, dev)
-    _check_out(out, m, n)
-    with _on(dev):
-        _lib.check(_lib.load().kbn_mxfp4_gemm_nt(a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(), _bias_ptr(bias, n, dev), out.data_ptr(),
-                                                 _row_stride(out), m, n, k, _stream(out)))
+    m, n, k = a_q.size(0), b_q.size(0), a_q.size(1) * 2
+    a_sf_ptr, b_sf_ptr, ld = _check_mxfp4_operand(a_q, a_sf, m, k, "a"), _check_mxfp4_operand(b_q, b_sf, n, k, "b"), _check_out(out, m, n)
+    index = _gpu(a_q, a_sf, b_q, b_sf, out)
+    _call(index, _lib.load().kbn_mxfp4_gemm_nt, a_q.data_ptr(), a_sf_ptr, b_q.data_ptr(), b_sf_ptr,
+          None if bias is None else _bias_ptr(bias, n, out.device), out.data_ptr(), ld, m, n, k)
 
 
 def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
@@ -766,16 +801,11 @@ def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: to
     """The MXFP4 linear layer: x bf16 [M,K], quantised as quant_mxfp4 does, times b_q [N,K/2] / b_sf (packed) into out bf16
     [M,N].  a_q uint8 [M,K/2] and a_sf (packed_mxfp4_bytes(M, K) bytes) are scratch for the quantised rows; up to eight rows
     are quantised inside the one kernel that multiplies them and leave the scratch untouched."""
-    dev = _cuda(x, a_q, a_sf, b_q, b_sf, out)
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1 or x.shape[1] % MX_BLOCK:
-        raise ValueError(f"x must be bf16 [M,K], contiguous along K, K a multiple of {MX_BLOCK}, got {x.dtype} {tuple(x.shape)}")
-    m, k = x.shape
-    _check_codes(a_q, m, k, "a_q")
-    if not a_q.is_contiguous():
-        raise ValueError("a_q must be contiguous")
-    _check_packed_mxfp4(a_sf, m, k, dev, "a_sf")
-    n = _check_mxfp4_weight(b_q, b_sf, k, dev)
-    _check_out(out, m, n)
-    with _on(dev):
-        _lib.check(_lib.load().kbn_mxfp4_linear(x.data_ptr(), _row_stride(x), m, k, a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(),
-                                                _bias_ptr(bias, n, dev), out.data_ptr(), _row_stride(out), n, _stream(x)))
+    m, k, ld_x = _bf16_rows(x, "x")
+    if k % MX_BLOCK or k == 0:
+        raise ValueError(f"x must have a multiple of {MX_BLOCK} columns, got {k}")
+    n = b_q.size(0)
+    a_sf_ptr, b_sf_ptr, ld = _check_mxfp4_operand(a_q, a_sf, m, k, "a"), _check_mxfp4_operand(b_q, b_sf, n, k, "b"), _check_out(out, m, n)
+    index = _gpu(x, a_q, a_sf, b_q, b_sf, out)
+    _call(index, _lib.load().kbn_mxfp4_linear, x.data_ptr(), ld_x, m, k, a_q.data_ptr(), a_sf_ptr, b_q.data_ptr(), b_sf_ptr,
+          None if bias is None else _bias_ptr(bias, n, out.device), out.data_ptr(), ld, n)
