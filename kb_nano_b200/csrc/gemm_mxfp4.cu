@@ -30,6 +30,7 @@ constexpr int kEpiWarps = 8;
 constexpr int kGemmThreads = 32 * (2 + kEpiWarps);
 constexpr int kStagingBytes = kEpiWarps * 32 * 128;            // 32 rows x 64 bf16 columns per epilogue warp
 constexpr int kTmemColumns = 512, kColScales = 256;            // accumulators in columns 0-255, scales behind them
+constexpr int kSplitGain = 14;                                 // K-steps a split over the cluster has to save
 constexpr int kGroupM = 8;                                     // tile rows that run side by side, for reuse of B in L2
 
 // BN: tile columns, 256 or 128.
@@ -580,11 +581,14 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const vo
     if (M == 1) p.ldc = (N + 7) / 8 * 8;      // the stride of a single row is free
     p.tiled_out = aligned16(C) && p.ldc % 8 == 0;
     const int64_t wide = p.m_tiles * ((N + 255) / 256), narrow = p.m_tiles * ((N + 127) / 128);
-    // Few tiles: K split over the cluster, the most slices that are resident at once and leave each a step.
+    // Few tiles: K split over the cluster, the most slices that are resident at once and leave each a step.  The exchange of
+    // partial sums takes as long as a dozen steps, so a split has to save more: measured with the quantiser, 64 x 4096 x 7168
+    // (28 steps, S = 4) 15.5 us split and 16.5 not, 512 x 4096 x 7168 (S = 2) 18.5 and 18.6, 77 x 2056 x 1440 (6 steps) 11.4
+    // and 8.6.
     p.n_tiles = (int32_t)((N + 255) / 256);
     for (int S = 4; S >= 2; S /= 2) {
         const int per = (p.steps + S - 1) / S;
-        if (2 * S * wide > sm_count() || (S - 1) * per >= p.steps || wide > max_clusters<256, true>(2 * S)) continue;
+        if (2 * S * wide > sm_count() || (S - 1) * per >= p.steps || p.steps - per < kSplitGain || wide > max_clusters<256, true>(2 * S)) continue;
         p.S = S;
         return launch<256, true>(A, sfa_packed, B, sfb_packed, K, p, (unsigned)wide, st);
     }

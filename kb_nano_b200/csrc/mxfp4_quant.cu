@@ -3,9 +3,9 @@
 // quantisers (kb-nano has FP8 only: tasks/baseline/L1/fp8_linear.py:181-215, tasks/baseline/L1/silu_mul_quant_fp8.py:23-76).
 //
 // All four are HBM-bound: 2 B in and 17/32 B out per element (4 B in with the activation), the inverse the other way round.
-// A half-warp takes 128 consecutive values of a row (16 bytes a lane), so a block of 32 is four lanes: two shuffles give
-// its largest magnitude, and the four scale bytes of the 128 values meet in one word, which is stored whole, both in the
-// row-major scales and in the packed layout.
+// A lane takes 16 consecutive values (one 32-byte access), eight lanes 128 of a row: a block of 32 is two lanes, one shuffle
+// gives its largest magnitude, and the four scale bytes of the 128 values meet in one word, which is stored whole, both in
+// the row-major scales and in the packed layout.  Measured (share of 6.57 TB/s): QUANT_FIGURES
 #include "mxfp4.cuh"
 #include "silu_exact.cuh"
 
@@ -21,140 +21,221 @@ struct QuantOut {
     uint32_t* packed;
     int64_t kblocks;
     bool word_scales;      // the row-major scales allow 4-byte stores
+    bool pair_codes;       // the codes allow 8-byte stores
 };
 
-// The 16 lanes of a half-warp hold 8 values each of columns [128 g, 128 g + 128) of `row` (lanes past K hold zeros and
-// live == false).  Quantises and stores them.
-__device__ __forceinline__ void quant_group(const uint32_t (&w)[4], bool live, int64_t row, uint32_t g, uint32_t j, uint32_t K, const QuantOut& o) {
-    uint32_t m = max_u16x2(max_u16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), max_u16x2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+struct Vec16 {             // 16 bf16 values
+    uint32_t w[8];
+};
+__device__ __forceinline__ Vec16 load16(const void* p) {       // 32-byte aligned, read once
+    Vec16 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void store16(void* p, const Vec16& v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]),
+                 "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+                 : "memory");
+}
+// ALIGN: what the rows' start allows, 32, 16 or 2 bytes.
+template <int ALIGN>
+__device__ __forceinline__ Vec16 load_values(const uint16_t* p) {
+    Vec16 v;
+    if (ALIGN == 32) {
+        v = load16(p);
+    } else if (ALIGN == 16) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p)), b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+        v.w[0] = a.x; v.w[1] = a.y; v.w[2] = a.z; v.w[3] = a.w;
+        v.w[4] = b.x; v.w[5] = b.y; v.w[6] = b.z; v.w[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    }
+    return v;
+}
+
+// The eight lanes of a team hold 16 values each of columns [128 g, 128 g + 128) of `row` (lanes past K hold zeros and
+// live == false).  Quantises and stores them; returns the word of the group's four scale bytes, in every lane of the team.
+// A value times the block's power of two is exact in bf16 wherever it does not round to code 0 anyway, so the products are
+// packed ones.
+__device__ __forceinline__ uint32_t quant_group(const Vec16& v, bool live, int64_t row, uint32_t g, uint32_t j, uint32_t K, const QuantOut& o) {
+    uint32_t m = v.w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max_u16x2(m, v.w[i] & 0x7fff7fffu);
     m = max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const uint32_t b = scale_byte(max(m & 0xffffu, m >> 16));
-    // the four blocks' bytes in one word, in every lane; blocks past K count as 2^0, so that nothing read there is a NaN
-    uint32_t word = (g * 128u + j * 8u < K ? b : 127u) << (8u * (j >> 2));
+    // blocks past K count as 2^0, so that nothing read there is a NaN
+    uint32_t word = (g * 128u + j * 16u < K ? b : 127u) << (8u * (j >> 1));
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
     word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
     if (live) {
-        *reinterpret_cast<uint32_t*>(o.q + row * o.ld_q + g * 64u + j * 4u) = quant8(w, inv_scale(b), b == 255u);
-        if (o.scale != nullptr) {
-            uint8_t* s = o.scale + row * o.s_row + g * 4u;
-            if (o.word_scales && g * 128u + 128u <= K) {
-                if (j == 0) *reinterpret_cast<uint32_t*>(s) = word;
-            } else if ((j & 3u) == 0) {
-                s[j >> 2] = (uint8_t)b;
+        uint32_t q[2] = {0, 0};
+        if (b != 255u) {
+            const uint32_t inv = (uint32_t)(254u - b) * 0x00800080u;      // 2^(127 - b) in both halves
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t s = mul_bf16x2(v.w[i], inv);
+                q[i >> 2] |= pack_e2m1x2(bf16_lo(s), bf16_hi(s)) << (8 * (i & 3));
             }
         }
-        if (o.packed != nullptr && j == 0) o.packed[packed_word(row, g, o.kblocks)] = word;
+        uint32_t* qp = reinterpret_cast<uint32_t*>(o.q + row * o.ld_q + g * 64u + j * 8u);
+        if (o.pair_codes) *reinterpret_cast<uint2*>(qp) = make_uint2(q[0], q[1]);
+        else qp[0] = q[0], qp[1] = q[1];
+    }
+    return word;
+}
+
+// The scale words of U consecutive groups g0 .. of one row, stored by lanes 0 .. U - 1 of the team.
+template <int U>
+__device__ __forceinline__ void store_scales(const uint32_t (&word)[U], bool valid, int64_t row, uint32_t g0, uint32_t j, uint32_t G, uint32_t K, const QuantOut& o) {
+    uint32_t w = word[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u)
+        if (j == (uint32_t)u) w = word[u];
+    const uint32_t g = g0 + j;
+    if (!valid || j >= U || g >= G) return;
+    if (o.packed != nullptr) o.packed[packed_word(row, g, o.kblocks)] = w;
+    if (o.scale != nullptr) {
+        uint8_t* s = o.scale + row * o.s_row + g * 4u;
+        if (o.word_scales && g * 128u + 128u <= K) {
+            *reinterpret_cast<uint32_t*>(s) = w;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                if (g * 128u + i * 32u < K) s[i] = (uint8_t)(w >> (8 * i));
+        }
     }
 }
 
-// VEC: rows of x start on 16-byte boundaries.  U groups of 128 per half-warp, all loads issued before the first use.
-template <bool VEC, int U>
+// U groups of 128 per team, all loads issued before the first use.
+template <int ALIGN, int U>
 __global__ void __launch_bounds__(256)
 quant_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, uint32_t K, int64_t ld_x, QuantOut o, uint32_t G, uint32_t chunks_per_row, uint32_t n_chunks) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // a GEMM behind this kernel waits before it reads
-    const uint32_t j = threadIdx.x & 15u;
-    const uint32_t chunk = blockIdx.x * 16u + (threadIdx.x >> 4);
+    const uint32_t j = threadIdx.x & 7u;
+    const uint32_t chunk = blockIdx.x * 32u + (threadIdx.x >> 3);
     const bool valid = chunk < n_chunks;
     const uint32_t row = valid ? chunk / chunks_per_row : 0u;
     const uint32_t g0 = (chunk - row * chunks_per_row) * U;
     const uint16_t* xr = reinterpret_cast<const uint16_t*>(x) + (int64_t)row * ld_x;
-    uint32_t w[U][4];
+    Vec16 v[U];
     bool live[U];
+    uint32_t word[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t col = (g0 + u) * 128u + j * 8u;
+        const uint32_t col = (g0 + u) * 128u + j * 16u;
         live[u] = valid && g0 + u < G && col < K;
-        if (VEC) {
-            const uint4 v = live[u] ? __ldcs(reinterpret_cast<const uint4*>(xr + col)) : make_uint4(0, 0, 0, 0);
-            w[u][0] = v.x; w[u][1] = v.y; w[u][2] = v.z; w[u][3] = v.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[u][i] = live[u] ? (uint32_t)xr[col + 2 * i] | ((uint32_t)xr[col + 2 * i + 1] << 16) : 0u;
-        }
+        if (live[u]) v[u] = load_values<ALIGN>(xr + col);
+        else v[u] = Vec16{};
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) quant_group(w[u], live[u], row, g0 + u, j, K, o);
+    for (int u = 0; u < U; ++u) word[u] = quant_group(v[u], live[u], row, g0 + u, j, K, o);
+    store_scales<U>(word, valid, row, g0, j, G, K, o);
+}
+
+// Eight gates times eight ups -> four packed bf16x2 y = bf16(bf16(silu(g)) * up), silu exactly rounded.  For every bf16 gate
+// of at least -60 the five-instruction approximation lies on the right side of its rounding boundary (all 65,536 gates are
+// tested), so only gates below that, where the exponential overflows, come from the table of exactly rounded results.
+__device__ __forceinline__ void silu_mul_exact8(const uint32_t* g, const uint32_t* u, const uint16_t* __restrict__ table, uint32_t* y) {
+    const uint32_t gm = min_bf16x2(min_bf16x2(g[0], g[1]), min_bf16x2(g[2], g[3]));
+    uint32_t s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = pack_bf16x2(silu_approx(bf16_lo(g[i])), silu_approx(bf16_hi(g[i])));
+    if (fminf(bf16_lo(gm), bf16_hi(gm)) < -60.0f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = silu_table_pair(g[i], table);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = mul_bf16x2(s[i], u[i]);
 }
 
 // bf16(bf16(silu(gate)) * up) with the exactly rounded SiLU of the FP8 activation kernel (silu_exact.cuh), then as above.
 // The two roundings to bf16 are those of an unfused activation in the model's type, so that fused and unfused layers agree.
-template <bool VEC, int U>
+template <int ALIGN, int U>
 __global__ void __launch_bounds__(256)
 silu_mul_quant_mxfp4_kernel(const __nv_bfloat16* __restrict__ in, uint32_t N2, int64_t ld_in, QuantOut o, uint32_t G, uint32_t chunks_per_row,
                             uint32_t n_chunks, const uint16_t* __restrict__ table) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t j = threadIdx.x & 15u;
-    const uint32_t chunk = blockIdx.x * 16u + (threadIdx.x >> 4);
+    const uint32_t j = threadIdx.x & 7u;
+    const uint32_t chunk = blockIdx.x * 32u + (threadIdx.x >> 3);
     const bool valid = chunk < n_chunks;
     const uint32_t row = valid ? chunk / chunks_per_row : 0u;
     const uint32_t g0 = (chunk - row * chunks_per_row) * U;
     const uint16_t* gr = reinterpret_cast<const uint16_t*>(in) + (int64_t)row * ld_in;
-    uint4 gate[U], up[U];
+    Vec16 gate[U], up[U];
     bool live[U];
+    uint32_t word[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t col = (g0 + u) * 128u + j * 8u;
+        const uint32_t col = (g0 + u) * 128u + j * 16u;
         live[u] = valid && g0 + u < G && col < N2;
-        gate[u] = up[u] = make_uint4(0, 0, 0, 0);
+        gate[u] = up[u] = Vec16{};
         if (live[u]) {
-            if (VEC) {
-                gate[u] = __ldcs(reinterpret_cast<const uint4*>(gr + col));
-                up[u] = __ldcs(reinterpret_cast<const uint4*>(gr + N2 + col));
-            } else {
-                uint32_t a[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    a[i] = (uint32_t)gr[col + 2 * i] | ((uint32_t)gr[col + 2 * i + 1] << 16);
-                    b[i] = (uint32_t)gr[N2 + col + 2 * i] | ((uint32_t)gr[N2 + col + 2 * i + 1] << 16);
-                }
-                gate[u] = make_uint4(a[0], a[1], a[2], a[3]);
-                up[u] = make_uint4(b[0], b[1], b[2], b[3]);
-            }
+            gate[u] = load_values<ALIGN>(gr + col);
+            up[u] = load_values<ALIGN>(gr + N2 + col);
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t y[4];
-        silu_mul_8(gate[u], up[u], table, y);
-        quant_group(y, live[u], row, g0 + u, j, N2, o);
+        Vec16 y;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) silu_mul_exact8(gate[u].w + 4 * h, up[u].w + 4 * h, table, y.w + 4 * h);
+        word[u] = quant_group(y, live[u], row, g0 + u, j, N2, o);
     }
+    store_scales<U>(word, valid, row, g0, j, G, N2, o);
 }
 
-// 32 codes (16 bytes) per thread and step -> 32 bf16 values.  e2m1 times a power of two is exact in bf16 except where it
-// leaves bf16's range (6 * 2^126 and above becomes infinity).
-template <bool VEC>
+// 16 codes (8 bytes) per thread and vector -> 16 bf16 values.  e2m1 times a power of two is exact in bf16 except where it
+// leaves bf16's range (6 * 2^126 and above becomes infinity).  FLAT: everything is contiguous, rows do not matter.
+template <bool FLAT, bool VEC, int U>
 __global__ void __launch_bounds__(256)
-dequant_mxfp4_kernel(const uint8_t* __restrict__ q, int64_t ld_q, const uint8_t* __restrict__ scale, int64_t s_row, uint32_t vecs_per_row, int64_t n_vecs,
+dequant_mxfp4_kernel(const uint8_t* __restrict__ q, int64_t ld_q, const uint8_t* __restrict__ scale, int64_t s_row, uint32_t vecs_per_row, uint32_t n_vecs,
                      __nv_bfloat16* __restrict__ out, int64_t ld_out) {
-    // one vector = 8 values: 4 bytes of codes, a quarter of a block
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v >= n_vecs) return;
-    const int64_t row = v / vecs_per_row;
-    const uint32_t c = (uint32_t)(v - row * vecs_per_row);
-    uint32_t w;
-    const uint8_t* qp = q + row * ld_q + (int64_t)c * 4;
-    if (VEC) {
-        w = *reinterpret_cast<const uint32_t*>(qp);
-    } else {
-        w = (uint32_t)qp[0] | ((uint32_t)qp[1] << 8) | ((uint32_t)qp[2] << 16) | ((uint32_t)qp[3] << 24);
-    }
-    const float s = scale_value(scale[row * s_row + (c >> 2)]);
-    uint32_t h[4], r[4];
-    unpack_e2m1x8(w, h);
+    uint32_t w[U][2], sb[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 p = *reinterpret_cast<const __half2*>(&h[i]);
-        r[i] = pack_bf16x2(__low2float(p) * s, __high2float(p) * s);
-    }
-    uint16_t* op = reinterpret_cast<uint16_t*>(out) + row * ld_out + (int64_t)c * 8;
-    if (VEC) {
-        *reinterpret_cast<uint4*>(op) = make_uint4(r[0], r[1], r[2], r[3]);
-    } else {
+    for (int u = 0; u < U; ++u) {
+        const uint32_t v = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
+        w[u][0] = w[u][1] = sb[u] = 0;
+        if (v >= n_vecs) continue;
+        const uint32_t row = FLAT ? 0u : v / vecs_per_row, c = v - row * vecs_per_row;
+        const uint8_t* qp = q + (FLAT ? (int64_t)v * 8 : (int64_t)row * ld_q + (int64_t)c * 8);
+        if (VEC) {
+            const uint2 p = __ldcs(reinterpret_cast<const uint2*>(qp));
+            w[u][0] = p.x; w[u][1] = p.y;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            op[2 * i] = (uint16_t)(r[i] & 0xffffu);
-            op[2 * i + 1] = (uint16_t)(r[i] >> 16);
+            for (int i = 0; i < 8; ++i) w[u][i >> 2] |= (uint32_t)qp[i] << (8 * (i & 3));
+        }
+        sb[u] = FLAT ? scale[v >> 1] : scale[(int64_t)row * s_row + (c >> 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t v = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
+        if (v >= n_vecs) continue;
+        const uint32_t row = FLAT ? 0u : v / vecs_per_row, c = v - row * vecs_per_row;
+        const float s = scale_value(sb[u]);
+        Vec16 r;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t p[4];
+            unpack_e2m1x8(w[u][h], p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 f = *reinterpret_cast<const __half2*>(&p[i]);
+                r.w[4 * h + i] = pack_bf16x2(__low2float(f) * s, __high2float(f) * s);
+            }
+        }
+        uint16_t* op = reinterpret_cast<uint16_t*>(out) + (FLAT ? (int64_t)v * 16 : (int64_t)row * ld_out + (int64_t)c * 16);
+        if (VEC) {
+            store16(op, r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                op[2 * i] = (uint16_t)(r.w[i] & 0xffffu);
+                op[2 * i + 1] = (uint16_t)(r.w[i] >> 16);
+            }
         }
     }
 }
@@ -182,6 +263,12 @@ pack_mxfp4_scales_kernel(const uint8_t* __restrict__ scale, int64_t rows, uint32
     packed[i] = w;
 }
 
+// What the starts of a bf16 matrix's rows allow: accesses of 32, 16 or 2 bytes.
+static int row_alignment(const void* p, int64_t ld, int64_t rows) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (rows > 1 ? (uintptr_t)(ld * 2) : 0);
+    return (bits & 31u) == 0 ? 32 : ((bits & 15u) == 0 ? 16 : 2);
+}
+
 static int fill_out(QuantOut& o, const char* who, int64_t M, int64_t K, void* q, int64_t ld_q, void* scale, int64_t s_row, void* sf_packed) {
     KBN_REQUIRE(K % 32 == 0, KBN_ERR_ARG, "%s: K=%lld must be a multiple of 32", who, (long long)K);
     KBN_REQUIRE(q, KBN_ERR_ARG, "%s: null pointer", who);
@@ -197,6 +284,7 @@ static int fill_out(QuantOut& o, const char* who, int64_t M, int64_t K, void* q,
     o.s_row = s_row;
     o.packed = static_cast<uint32_t*>(sf_packed);
     o.kblocks = (K + 127) / 128;
+    o.pair_codes = ld_q % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
     o.word_scales = scale && s_row % 4 == 0 && (reinterpret_cast<uintptr_t>(scale) & 3u) == 0;
     return KBN_OK;
 }
@@ -222,14 +310,18 @@ extern "C" int kbn_quant_mxfp4(const void* x, int64_t M, int64_t K, int64_t ld_x
     if (rc != KBN_OK) return rc;
     const auto* xb = static_cast<const __nv_bfloat16*>(x);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    constexpr int U = 4;
-    const int64_t G = (K + 127) / 128, cpr = (G + U - 1) / U, n_chunks = M * cpr;
-    KBN_REQUIRE(n_chunks < (1ll << 31), KBN_ERR_ARG, "kbn_quant_mxfp4: more than 2^31 groups");
-    const unsigned blocks = (unsigned)((n_chunks + 15) / 16);
-    if (ld_x % 8 == 0 && aligned16(x))
-        quant_mxfp4_kernel<true, U><<<blocks, 256, 0, st>>>(xb, (uint32_t)K, ld_x, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks);
-    else
-        quant_mxfp4_kernel<false, U><<<blocks, 256, 0, st>>>(xb, (uint32_t)K, ld_x, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks);
+    const int64_t G = (K + 127) / 128;
+    KBN_REQUIRE(M * G < (1ll << 31), KBN_ERR_ARG, "kbn_quant_mxfp4: more than 2^31 groups");
+    // Four groups per team where that still gives every SM work; a few rows are spread over more teams.
+    auto go = [&](auto kernel, int U) {
+        const int64_t cpr = (G + U - 1) / U, n_chunks = M * cpr;
+        kernel<<<(unsigned)((n_chunks + 31) / 32), 256, 0, st>>>(xb, (uint32_t)K, ld_x, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks);
+    };
+    const int align = row_alignment(x, ld_x, M);
+    const bool many = M * G >= 32 * 4 * (int64_t)sm_count();
+    if (align == 32) many ? go(quant_mxfp4_kernel<32, 4>, 4) : go(quant_mxfp4_kernel<32, 1>, 1);
+    else if (align == 16) many ? go(quant_mxfp4_kernel<16, 4>, 4) : go(quant_mxfp4_kernel<16, 1>, 1);
+    else go(quant_mxfp4_kernel<2, 1>, 1);
     KBN_CHECK_LAUNCH();
     return KBN_OK;
 }
@@ -250,14 +342,18 @@ extern "C" int kbn_silu_mul_quant_mxfp4(const void* in, int64_t M, int64_t N2, i
     rc = silu_table_for_stream(st, &table);
     if (rc != KBN_OK) return rc;
     const auto* xb = static_cast<const __nv_bfloat16*>(in);
-    constexpr int U = 2;
-    const int64_t G = (N2 + 127) / 128, cpr = (G + U - 1) / U, n_chunks = M * cpr;
-    KBN_REQUIRE(n_chunks < (1ll << 31), KBN_ERR_ARG, "kbn_silu_mul_quant_mxfp4: more than 2^31 groups");
-    const unsigned blocks = (unsigned)((n_chunks + 15) / 16);
-    if (ld_in % 8 == 0 && aligned16(in))
-        silu_mul_quant_mxfp4_kernel<true, U><<<blocks, 256, 0, st>>>(xb, (uint32_t)N2, ld_in, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks, table);
-    else
-        silu_mul_quant_mxfp4_kernel<false, U><<<blocks, 256, 0, st>>>(xb, (uint32_t)N2, ld_in, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks, table);
+    const int64_t G = (N2 + 127) / 128;
+    KBN_REQUIRE(M * G < (1ll << 31), KBN_ERR_ARG, "kbn_silu_mul_quant_mxfp4: more than 2^31 groups");
+    auto go = [&](auto kernel, int U) {
+        const int64_t cpr = (G + U - 1) / U, n_chunks = M * cpr;
+        kernel<<<(unsigned)((n_chunks + 31) / 32), 256, 0, st>>>(xb, (uint32_t)N2, ld_in, o, (uint32_t)G, (uint32_t)cpr, (uint32_t)n_chunks, table);
+    };
+    // the up half starts N2 * 2 bytes, a multiple of 64, behind the gate half
+    const int align = row_alignment(in, ld_in, M);
+    const bool many = M * G >= 32 * 2 * (int64_t)sm_count();
+    if (align == 32) many ? go(silu_mul_quant_mxfp4_kernel<32, 2>, 2) : go(silu_mul_quant_mxfp4_kernel<32, 1>, 1);
+    else if (align == 16) many ? go(silu_mul_quant_mxfp4_kernel<16, 2>, 2) : go(silu_mul_quant_mxfp4_kernel<16, 1>, 1);
+    else go(silu_mul_quant_mxfp4_kernel<2, 1>, 1);
     KBN_CHECK_LAUNCH();
     return KBN_OK;
 }
@@ -271,17 +367,20 @@ extern "C" int kbn_dequant_mxfp4(const void* q, int64_t ld_q, const void* scale,
     KBN_REQUIRE(q && scale && out && (reinterpret_cast<uintptr_t>(out) & 1u) == 0, KBN_ERR_ARG, "kbn_dequant_mxfp4: null or odd pointer");
     KBN_REQUIRE(K % 32 == 0, KBN_ERR_ARG, "kbn_dequant_mxfp4: K=%lld must be a multiple of 32", (long long)K);
     KBN_REQUIRE(M == 1 || (ld_q >= K / 2 && s_row >= K / 32 && ld_out >= K), KBN_ERR_ARG, "kbn_dequant_mxfp4: a row stride is too small");
-    const int64_t n = M * (K / 8);
-    KBN_REQUIRE(K < (1ll << 31) && (n + 255) / 256 < (1ll << 31), KBN_ERR_ARG, "kbn_dequant_mxfp4: too many values");
-    const bool vec = ld_q % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 3u) == 0 && ld_out % 8 == 0 && aligned16(out);
+    const int64_t n = M * (K / 16);
+    KBN_REQUIRE(n < (1ll << 31), KBN_ERR_ARG, "kbn_dequant_mxfp4: more than 2^35 values");
+    const bool vec = (ld_q % 8 == 0 || M == 1) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && row_alignment(out, ld_out, M) == 32;
+    const bool flat = M == 1 || (ld_q == K / 2 && s_row == K / 32 && ld_out == K);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned blocks = (unsigned)((n + 255) / 256);
     auto* ob = static_cast<__nv_bfloat16*>(out);
     const auto *qb = static_cast<const uint8_t*>(q), *sb = static_cast<const uint8_t*>(scale);
-    if (vec)
-        dequant_mxfp4_kernel<true><<<blocks, 256, 0, st>>>(qb, ld_q, sb, s_row, (uint32_t)(K / 8), n, ob, ld_out);
-    else
-        dequant_mxfp4_kernel<false><<<blocks, 256, 0, st>>>(qb, ld_q, sb, s_row, (uint32_t)(K / 8), n, ob, ld_out);
+    auto go = [&](auto kernel, int U) {
+        kernel<<<(unsigned)((n + 256 * U - 1) / (256 * U)), 256, 0, st>>>(qb, ld_q, sb, s_row, (uint32_t)(K / 16), (uint32_t)n, ob, ld_out);
+    };
+    const bool many = n >= 256 * 4 * (int64_t)sm_count();
+    if (vec && flat) many ? go(dequant_mxfp4_kernel<true, true, 4>, 4) : go(dequant_mxfp4_kernel<true, true, 1>, 1);
+    else if (vec) many ? go(dequant_mxfp4_kernel<false, true, 4>, 4) : go(dequant_mxfp4_kernel<false, true, 1>, 1);
+    else go(dequant_mxfp4_kernel<false, false, 1>, 1);
     KBN_CHECK_LAUNCH();
     return KBN_OK;
 }

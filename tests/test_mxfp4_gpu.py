@@ -147,6 +147,18 @@ def test_silu_mul_quant_over_every_finite_gate(cuda_dev):
     check_quant(y, q, s, p)
 
 
+def test_silu_of_gates_far_below_zero_and_non_finite(cuda_dev):
+    """Gates below -60 beside ordinary ones; infinities and NaNs spoil their block."""
+    from kb_nano_b200 import ops
+    x = torch.randn(8, 128, device=cuda_dev).to(torch.bfloat16)
+    x[0, 3], x[1, 9], x[2, 33] = -60.5, -87.5, -88.0
+    x[3, 2], x[4, 5], x[5, 63], x[6, 100] = float("nan"), float("inf"), float("-inf"), float("nan")
+    q, s, p = outputs(8, 64, cuda_dev)
+    ops.silu_mul_quant_mxfp4(x, q, s, p)
+    g, u = x.double().chunk(2, dim=1)
+    check_quant(ref.bf16_round(ref.bf16_round(torch.where(torch.isinf(g) & (g < 0), torch.nan, g * torch.sigmoid(g))) * u), q, s, p)
+
+
 def test_silu_strides(cuda_dev):
     from kb_nano_b200 import ops
     wide = torch.randn(9, 140, device=cuda_dev).to(torch.bfloat16)
