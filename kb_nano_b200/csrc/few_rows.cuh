@@ -3,10 +3,10 @@
 //
 // With at most eight rows (tokens) per weight matrix a product is a weight stream, 2 to 16 flop per weight byte, and what
 // counts is that enough weight bytes are in flight on every SM all the time.  One CTA per SM walks a contiguous range of
-// units; a unit is 16 weight rows (two boxes of eight) over the whole K.  A producer warp keeps a ring of 16 KB stages
-// full with 3-D tiled TMA loads (eight rows of a box, up to 16 chunks of 128 K-values each, one instruction per box) and
+// units; a unit is 16 (FP8) or 32 (MXFP4) weight rows, in two boxes, over the whole K.  A producer warp keeps a ring of
+// 16 KB stages full with 3-D tiled TMA loads (the rows of a box, eight chunks of 128 K-values each, one instruction) and
 // the block scales beside them (tiled loads too where their rows allow it, else 4-byte asynchronous copies, which cost the
-// one producer warp about as many instructions as everything else); sixteen consumer warps split the chunks.
+// one producer warp about as many instructions as everything else); sixteen consumer warps split the chunks, eight per stage.
 //
 //   product    mma.sync.m16n8k16, f16 x f16 -> fp32: the 16 weight rows are its M, the tokens its N.  (tcgen05 would spend a
 //              128-row tile on them and needs its operands in fp8 or fp4; at this intensity the legacy instruction is far
@@ -41,29 +41,35 @@ constexpr int kMaxTokens = 16, kMaxTopk = 16, kMaxPairs = kMaxTokens * kMaxTopk;
 constexpr int kMaxStages = 12;
 constexpr int kMinStages = 5;                             // 80 KB in flight per SM: what 6.5 TB/s needs at about 1.5 us
 
+constexpr int kChunks = 8;                                // 128-K chunks per stage, one consumer warp each
+
 template <int FMT>
 struct Fmt;
 template <>
 struct Fmt<kFp8> {
-    static constexpr int kChunkBytes = 128, kChunks = 8, kScaleBytes = 512, kTokenPad = 16;
-    static constexpr int kArrivals = 8;                   // warps that read a stage
+    static constexpr int kTiles = 1;                      // 16-row tiles of the matrix instruction per unit
+    static constexpr int kChunkBytes = 128, kScaleBytes = 512, kTokenPad = 16;
 };
 template <>
 struct Fmt<kMxfp4> {
-    static constexpr int kChunkBytes = 64, kChunks = 16, kScaleBytes = 1024, kTokenPad = 64;
-    static constexpr int kArrivals = 16;
+    static constexpr int kTiles = 2;                      // half the bytes a row: two tiles share a warp's token loads and waits
+    static constexpr int kChunkBytes = 64, kScaleBytes = 1024, kTokenPad = 64;
 };
+template <int FMT>
+constexpr int kBoxRows = 8 * Fmt<FMT>::kTiles;            // rows of each of a unit's two boxes
+template <int FMT>
+constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * Fmt<FMT>::kTiles * 4;
 
 // Where a weight matrix's scales lie.  FP8: fp32 [rows / 128, KC].  MXFP4: one 32-bit word per row and chunk, row-major
 // (word (row, c) at row * KC + c) or, PACKED, in the packed layout of the tensor core.
-// MXFP4 row-major scales with 16-byte row strides (K % 512 == 0) also have a tensor map (boxes of eight rows x 64 bytes,
-// 64-byte swizzle).  In the ring a stage's word (row of 16, chunk) is always where that box puts it, see scale_word().
+// MXFP4 row-major scales with 16-byte row strides (K % 512 == 0) also have a tensor map (boxes of 16 rows x 32 bytes, 32-byte
+// swizzle).  In the ring a stage's word (row of 32, chunk) is always where that box puts it, see scale_word().
 struct ScaleSource {
     const void* base;
     const CUtensorMap* map;      // null: asynchronous copies
 };
 __device__ __forceinline__ uint32_t scale_word(int row, int chunk) {      // byte offset; no bank conflicts over eight rows
-    return (uint32_t)(row * 64 + ((((chunk >> 2) ^ (row >> 1)) & 3) << 4) + (chunk & 3) * 4);
+    return (uint32_t)(row * 32 + ((((chunk >> 2) ^ (row >> 2)) & 1) << 4) + (chunk & 3) * 4);
 }
 
 struct Smem {
@@ -71,7 +77,7 @@ struct Smem {
     uint8_t* scales;       // one area per stage
     uint8_t* tokens;       // f16 rows, stride token_stride
     float* token_scales;   // [rows, K / 128]: what a chunk's partial sum is multiplied by
-    float* red;            // one buffer of 16 warps x 128 partial sums per finisher
+    float* red;            // one buffer of 16 warps x 128 partial sums (times tiles) per finisher
     uint64_t* bars;        // full[stages], empty[stages], partials full[kFinishers], partials empty[kFinishers]
     int32_t stages;
 };
@@ -148,10 +154,10 @@ struct RingPos {
     }
 };
 
-__device__ __forceinline__ void init_ring(const Smem& s, int arrivals) {
+__device__ __forceinline__ void init_ring(const Smem& s) {
     for (int i = 0; i < s.stages; ++i) {
         ptx::mbar_init(ptx::smem_u32(s.bars + i), 1 + 32);                    // the producer's bytes, its 32 lanes' scale copies
-        ptx::mbar_init(ptx::smem_u32(s.bars + s.stages + i), (uint32_t)arrivals);
+        ptx::mbar_init(ptx::smem_u32(s.bars + s.stages + i), kChunks);
     }
     for (int i = 0; i < kFinishers; ++i) {
         ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + i), kConsumerWarps);
@@ -167,7 +173,7 @@ template <int FMT, bool PACKED = false>
 __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const void* tmap, const ScaleSource& sc, int32_t row_a, int32_t row_b,
                                              int32_t n_rows, int32_t KC, int lane, const WaitCtx& w) {
     using F = Fmt<FMT>;
-    for (int32_t c0 = 0; c0 < KC; c0 += F::kChunks) {
+    for (int32_t c0 = 0; c0 < KC; c0 += kChunks) {
         const uint32_t full = ptx::smem_u32(s.bars + pos.slot), empty = ptx::smem_u32(s.bars + s.stages + pos.slot);
         wait_ring(empty, pos.phase ^ 1u, w);
         const uint32_t dst = ptx::smem_u32(s.ring) + pos.slot * kStageBytes;
@@ -190,13 +196,12 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
                 cp_async4(sdst + lane * 4, static_cast<const float*>(sc.base) + (int64_t)(row >> 7) * KC + c);
             }
         } else if (!tiled) {
-            // eight words per lane, two chunks apart
-            const int32_t r = lane & 15, c = c0 + (lane >> 4);
-            const int32_t row = min((r < 8 ? row_a : row_b - 8) + r, n_rows - 1);
-            const uint32_t* src = static_cast<const uint32_t*>(sc.base) + (PACKED ? (int64_t)mxfp4::packed_word(row, c, KC) : (int64_t)row * KC + c);
+            // a row per lane, eight words each
+            const int32_t row = min((lane < 16 ? row_a : row_b - 16) + lane, n_rows - 1);
+            const uint32_t* src = static_cast<const uint32_t*>(sc.base) + (PACKED ? (int64_t)mxfp4::packed_word(row, c0, KC) : (int64_t)row * KC + c0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + 2 * i < KC) cp_async4(sdst + scale_word(r, (lane >> 4) + 2 * i), src + i * (PACKED ? 256 : 2));
+            for (int i = 0; i < kChunks; ++i)
+                if (c0 + i < KC) cp_async4(sdst + scale_word(lane, i), src + i * (PACKED ? 128 : 1));
         }
         cp_async_arrive(full);
         pos.advance((uint32_t)s.stages);
@@ -215,28 +220,27 @@ __device__ __forceinline__ TokenColumns token_columns(const Smem& s, uint32_t st
                         ptx::smem_u32(s.token_scales) + (uint32_t)(row_of(t1) * KC) * 4u};
 }
 
-// Consumer warp: its chunks of one unit, added to acc.  acc[0..1]: row g of box 0 with tokens 2t, 2t + 1; acc[2..3]: row g of
-// box 1.  FP8: a stage has work for eight warps; slots with an even number belong to warps 0-7, the others to warps 8-15.
-// A slot must always have the same readers: a warp may only test a barrier for a phase if it has seen the phase before it
-// complete, because the test tells two phases apart by their parity alone.
+// Consumer warp: its chunks of one unit, added to acc.  acc[i][0..1]: row 8 i + g of box 0 with tokens 2t, 2t + 1; acc[i][2..3]:
+// row 8 i + g of box 1.  A stage has work for eight warps: slots with an even number belong to warps 0-7, the others to warps
+// 8-15.  A slot must always have the same readers: a warp may only test a barrier for a phase if it has seen the phase
+// before it complete, because the test tells two phases apart by their parity alone.
 template <int FMT>
-__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, const TokenColumns& tc, float (&acc)[4],
-                                             const WaitCtx& w) {
+__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, const TokenColumns& tc,
+                                             float (&acc)[Fmt<FMT>::kTiles][4], const WaitCtx& w) {
     using F = Fmt<FMT>;
-    const int g = lane >> 2, t = lane & 3;
-    const int cw = FMT == kFp8 ? (warp & 7) : warp;
-    for (int32_t c0 = 0; c0 < KC; c0 += F::kChunks) {
+    const int g = lane >> 2, t = lane & 3, cw = warp & 7;
+    for (int32_t c0 = 0; c0 < KC; c0 += kChunks) {
         const RingPos here = pos;
         pos.advance((uint32_t)s.stages);
-        if (FMT == kFp8 && (here.slot & 1u) != (uint32_t)(warp >> 3)) continue;
+        if ((here.slot & 1u) != (uint32_t)(warp >> 3)) continue;
         wait_ring(ptx::smem_u32(s.bars + here.slot), here.phase, w);
         const int32_t c = c0 + cw;
         if (c < KC) {
-            const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * 8 + g) * F::kChunkBytes;
+            const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * kBoxRows<FMT> + g) * F::kChunkBytes;
             const uint32_t box1 = box0 + kStageBytes / 2;
             const uint32_t sdst = ptx::smem_u32(s.scales) + here.slot * F::kScaleBytes;
             const float x0s = __uint_as_float(lds32(tc.scale0 + (uint32_t)c * 4u)), x1s = __uint_as_float(lds32(tc.scale1 + (uint32_t)c * 4u));
-            if (FMT == kFp8) {
+            if constexpr (FMT == kFp8) {
                 float p[4], q[4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -257,38 +261,50 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
                     mma_f16_m16n8k16(q, a0, a1, a2, a3, x1.z, x1.w);
                 }
                 const float s0 = __uint_as_float(lds32(sdst + cw * 4)), s1 = __uint_as_float(lds32(sdst + 32 + cw * 4));
-                acc[0] = fmaf((p[0] + q[0]) * x0s, s0, acc[0]);
-                acc[1] = fmaf((p[1] + q[1]) * x1s, s0, acc[1]);
-                acc[2] = fmaf((p[2] + q[2]) * x0s, s1, acc[2]);
-                acc[3] = fmaf((p[3] + q[3]) * x1s, s1, acc[3]);
+                acc[0][0] = fmaf((p[0] + q[0]) * x0s, s0, acc[0][0]);
+                acc[0][1] = fmaf((p[1] + q[1]) * x1s, s0, acc[0][1]);
+                acc[0][2] = fmaf((p[2] + q[2]) * x0s, s1, acc[0][2]);
+                acc[0][3] = fmaf((p[3] + q[3]) * x1s, s1, acc[0][3]);
             } else {
-                const uint32_t sw0 = lds32(sdst + scale_word(g, cw)), sw1 = lds32(sdst + scale_word(g, cw) + 512);      // rows g and g + 8
-                const uint32_t swz = (uint32_t)(g >> 1) & 3u;
-                const uint32_t e0[2] = {mxfp4::scale_bf16x2(sw0), mxfp4::scale_bf16x2(sw0 >> 16)}, e1[2] = {mxfp4::scale_bf16x2(sw1), mxfp4::scale_bf16x2(sw1 >> 16)};
-                const uint32_t w0 = box0 + (swz << 4) + (uint32_t)t * 4u;      // 16-byte piece b of the row at w0 ^ 16 b
+                const uint32_t w0 = box0 + (uint32_t)(((g >> 1) & 3) << 4) + (uint32_t)t * 4u;      // 16-byte piece b of the row at w0 ^ 16 b
                 const uint32_t xa = tc.row + (uint32_t)(c * 128 + t * 8) * 2u;
-                float q[4];
+                uint32_t e[F::kTiles][2][2];      // tile, box, pair of blocks: two scales as packed bf16
+#pragma unroll
+                for (int i = 0; i < F::kTiles; ++i)
+#pragma unroll
+                    for (int box = 0; box < 2; ++box) {
+                        const uint32_t sw = lds32(sdst + scale_word(8 * i + g, cw) + box * 512);
+                        e[i][box][0] = mxfp4::scale_bf16x2(sw);
+                        e[i][box][1] = mxfp4::scale_bf16x2(sw >> 16);
+                    }
+                float q[F::kTiles][4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const uint32_t wb_at = w0 ^ (uint32_t)(16 * b);
-                    const uint32_t wa = lds32(wb_at), wb = lds32(wb_at + kStageBytes / 2);
+                    const uint32_t at = w0 ^ (uint32_t)(16 * b);
                     const uint4 x = lds128(xa + 64 * b);
-                    uint32_t ha[4], hb[4];
-                    mxfp4::unpack_e2m1x8(wa, ha);
-                    mxfp4::unpack_e2m1x8(wb, hb);
-                    float p[4];
-                    mma_f16_m16n8k16_first(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
-                    mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
-                    const float s0 = b & 1 ? bf16_hi(e0[b >> 1]) : bf16_lo(e0[b >> 1]), s1 = b & 1 ? bf16_hi(e1[b >> 1]) : bf16_lo(e1[b >> 1]);
-                    q[0] = b == 0 ? p[0] * s0 : fmaf(p[0], s0, q[0]);
-                    q[1] = b == 0 ? p[1] * s0 : fmaf(p[1], s0, q[1]);
-                    q[2] = b == 0 ? p[2] * s1 : fmaf(p[2], s1, q[2]);
-                    q[3] = b == 0 ? p[3] * s1 : fmaf(p[3], s1, q[3]);
+#pragma unroll
+                    for (int i = 0; i < F::kTiles; ++i) {
+                        uint32_t ha[4], hb[4];
+                        mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes), ha);
+                        mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes + kStageBytes / 2), hb);
+                        float p[4];
+                        mma_f16_m16n8k16_first(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+                        mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
+                        const float s0 = b & 1 ? bf16_hi(e[i][0][b >> 1]) : bf16_lo(e[i][0][b >> 1]);
+                        const float s1 = b & 1 ? bf16_hi(e[i][1][b >> 1]) : bf16_lo(e[i][1][b >> 1]);
+                        q[i][0] = b == 0 ? p[0] * s0 : fmaf(p[0], s0, q[i][0]);
+                        q[i][1] = b == 0 ? p[1] * s0 : fmaf(p[1], s0, q[i][1]);
+                        q[i][2] = b == 0 ? p[2] * s1 : fmaf(p[2], s1, q[i][2]);
+                        q[i][3] = b == 0 ? p[3] * s1 : fmaf(p[3], s1, q[i][3]);
+                    }
                 }
-                acc[0] = fmaf(q[0], x0s, acc[0]);
-                acc[1] = fmaf(q[1], x1s, acc[1]);
-                acc[2] = fmaf(q[2], x0s, acc[2]);
-                acc[3] = fmaf(q[3], x1s, acc[3]);
+#pragma unroll
+                for (int i = 0; i < F::kTiles; ++i) {
+                    acc[i][0] = fmaf(q[i][0], x0s, acc[i][0]);
+                    acc[i][1] = fmaf(q[i][1], x1s, acc[i][1]);
+                    acc[i][2] = fmaf(q[i][2], x0s, acc[i][2]);
+                    acc[i][3] = fmaf(q[i][3], x1s, acc[i][3]);
+                }
             }
         }
         __syncwarp();
@@ -296,30 +312,45 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
     }
 }
 
-// Consumer warp: its partial sums of the CTA's u-th unit to the finisher u % kFinishers; element (row of 16) * 8 + token.
-__device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, int lane, const float (&acc)[4], const WaitCtx& w) {
+// Consumer warp: its partial sums of the CTA's u-th unit to the finisher u % kFinishers; per tile element (row of 16) * 8 +
+// token, rows 0-7 box 0's, rows 8-15 box 1's.
+template <int TILES>
+__device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, int lane, const float (&acc)[TILES][4], const WaitCtx& w) {
     const int buf = (int)(u % kFinishers);
     wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf), (uint32_t)(u / kFinishers & 1) ^ 1u, w);
-    float* r = s.red + (buf * kConsumerWarps + warp) * 128;
+    float* r = s.red + (buf * kConsumerWarps + warp) * (128 * TILES);
     const int g = lane >> 2, t = lane & 3;
-    *reinterpret_cast<float2*>(r + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
-    *reinterpret_cast<float2*>(r + (g + 8) * 8 + 2 * t) = make_float2(acc[2], acc[3]);
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+        *reinterpret_cast<float2*>(r + i * 128 + g * 8 + 2 * t) = make_float2(acc[i][0], acc[i][1]);
+        *reinterpret_cast<float2*>(r + i * 128 + (g + 8) * 8 + 2 * t) = make_float2(acc[i][2], acc[i][3]);
+    }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + buf));
 }
-// Finisher warp u % kFinishers: the sums of the CTA's u-th unit.  Lane l receives row l / 2, tokens 4 (l % 2) .. + 3.
-__device__ __forceinline__ void take_over(const Smem& s, int64_t u, int lane, float (&v)[4], const WaitCtx& w) {
+// Finisher warp u % kFinishers: the sums of the CTA's u-th unit.  Lane l receives, of each tile, row l / 2, tokens 4 (l % 2) .. + 3.
+template <int TILES>
+__device__ __forceinline__ void take_over(const Smem& s, int64_t u, int lane, float (&v)[TILES][4], const WaitCtx& w) {
     const int buf = (int)(u % kFinishers);
     wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + buf), (uint32_t)(u / kFinishers & 1), w);
-    const float4* r = reinterpret_cast<const float4*>(s.red + buf * kConsumerWarps * 128) + lane;
-    v[0] = v[1] = v[2] = v[3] = 0.f;
+    const float4* r = reinterpret_cast<const float4*>(s.red + buf * kConsumerWarps * (128 * TILES)) + lane;
 #pragma unroll
-    for (int i = 0; i < kConsumerWarps; ++i) {
-        const float4 p = r[i * 32];
-        v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+    for (int i = 0; i < TILES; ++i) {
+        v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kConsumerWarps; ++j) {
+            const float4 p = r[(j * TILES + i) * 32];
+            v[i][0] += p.x; v[i][1] += p.y; v[i][2] += p.z; v[i][3] += p.w;
+        }
     }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf));
+}
+// Row of a unit, counted over its two boxes, that lane l's value of tile i belongs to.
+template <int FMT>
+__device__ __forceinline__ int row_of_lane(int tile, int lane) {
+    const int r = lane >> 1;
+    return 8 * tile + (r & 7) + (r >> 3) * kBoxRows<FMT>;
 }
 
 // x * 2^e for |e| up to 254, in two exact steps (one factor alone may leave fp32's range).
@@ -407,8 +438,8 @@ static int allow_smem(Kernel kernel, std::atomic<uint64_t>& done) {
     return KBN_OK;
 }
 
-// Weight matrix [rows, K] as (chunk, row, chunk number): one box is eight rows of kChunks chunks, each chunk's eight rows
-// side by side and swizzled, so that a warp reading one chunk of eight rows touches every bank once.
+// Weight matrix [rows, K] as (chunk, row, chunk number): one box is kBoxRows rows of kChunks chunks, each chunk's rows side by
+// side and swizzled, so that a warp reading one chunk of eight rows touches every bank once.
 template <int FMT>
 static int weight_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K) {
     using F = Fmt<FMT>;
@@ -419,7 +450,7 @@ static int weight_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K
     t.rank = 3;
     t.dims[0] = F::kChunkBytes; t.dims[1] = (uint64_t)rows; t.dims[2] = (uint64_t)(K / 128);
     t.strides[0] = row_bytes; t.strides[1] = F::kChunkBytes;
-    t.box[0] = F::kChunkBytes; t.box[1] = 8; t.box[2] = F::kChunks;
+    t.box[0] = F::kChunkBytes; t.box[1] = kBoxRows<FMT>; t.box[2] = kChunks;
     t.swizzle = FMT == kFp8 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
     return encode_tensor_map(tm, t);
@@ -433,8 +464,8 @@ static int scale_rows_map(CUtensorMap* tm, const void* base, int64_t rows, int64
     t.rank = 2;
     t.dims[0] = (uint64_t)(K / 32); t.dims[1] = (uint64_t)rows; t.dims[2] = 1;
     t.strides[0] = (uint64_t)(K / 32);
-    t.box[0] = 64; t.box[1] = 8; t.box[2] = 1;
-    t.swizzle = CU_TENSOR_MAP_SWIZZLE_64B;
+    t.box[0] = 4 * kChunks; t.box[1] = kBoxRows<kMxfp4>; t.box[2] = 1;
+    t.swizzle = CU_TENSOR_MAP_SWIZZLE_32B;
     t.promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
     return encode_tensor_map(tm, t);
 }

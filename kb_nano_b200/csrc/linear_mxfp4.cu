@@ -12,8 +12,8 @@
 namespace kbn {
 namespace few {
 
-constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
-constexpr int kLinearFixed = 1024 + kRedBytes + 256 + 128;      // alignment, partial sums, barriers, flag
+constexpr int kUnitRows = 2 * kBoxRows<kMxfp4>;
+constexpr int kLinearFixed = 1024 + kRedBytes<kMxfp4> + 256 + 128;      // alignment, partial sums, barriers, flag
 
 struct LinearArgs {
     const __nv_bfloat16* x;
@@ -89,7 +89,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     s.scales = p;
     p += (size_t)a.stages * Fmt<kMxfp4>::kScaleBytes;
     s.red = reinterpret_cast<float*>(p);
-    p += kRedBytes;
+    p += kRedBytes<kMxfp4>;
     s.bars = reinterpret_cast<uint64_t*>(p);
     p += 256;
     int* abort_flag = reinterpret_cast<int*>(p);
@@ -99,7 +99,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     s.stages = a.stages;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        init_ring(s, Fmt<kMxfp4>::kArrivals);
+        init_ring(s);
         *abort_flag = 0;
         ptx::prefetch_tensormap(&tm);
     }
@@ -107,12 +107,12 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
 
-    const int32_t units = (a.N + 15) / 16, KC = a.K / 128;
+    const int32_t units = (a.N + kUnitRows - 1) / kUnitRows, KC = a.K / 128;
     const int32_t u0 = (int32_t)((int64_t)units * blockIdx.x / gridDim.x), u1 = (int32_t)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
     if (warp == kProducerWarp) {
         const WaitCtx w{abort_flag, a.status, 17};
         RingPos pos;
-        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, 16 * u, 16 * u + 8, a.N, KC, lane, w);
+        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, kUnitRows * u, kUnitRows * u + kUnitRows / 2, a.N, KC, lane, w);
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
         RingPos pos;
@@ -120,22 +120,24 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
         consumer_sync();
         const TokenColumns columns = token_columns(s, (uint32_t)a.token_stride, KC, a.M, lane, [](int col) { return col; });
         for (int32_t u = u0; u < u1; ++u) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[Fmt<kMxfp4>::kTiles][4] = {};
             consume_unit<kMxfp4>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
         }
     } else {
         const WaitCtx w{abort_flag, a.status, 21};
         for (int32_t u = u0 + warp - kFirstFinisher; u < u1; u += kFinishers) {
-            float v[4];
+            float v[Fmt<kMxfp4>::kTiles][4];
             take_over(s, u - u0, lane, v, w);
-            const int n = 16 * u + (lane >> 1), tok0 = 4 * (lane & 1);
-            if (n < a.N) {
+            const int tok0 = 4 * (lane & 1);
+#pragma unroll
+            for (int tile = 0; tile < Fmt<kMxfp4>::kTiles; ++tile) {
+                const int n = kUnitRows * u + row_of_lane<kMxfp4>(tile, lane);
+                if (n >= a.N) continue;
                 const float bias = a.bias != nullptr ? __bfloat162float(a.bias[n]) : 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (tok0 + i < a.M)
-                        a.C[(int64_t)(tok0 + i) * a.ldc + n] = __float2bfloat16_rn(v[i] + bias);
+                    if (tok0 + i < a.M) a.C[(int64_t)(tok0 + i) * a.ldc + n] = __float2bfloat16_rn(v[tile][i] + bias);
             }
         }
     }
@@ -163,7 +165,7 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     static std::atomic<uint64_t> allowed{0};
     rc = allow_smem(mxfp4_linear_few_kernel, allowed);
     if (rc != KBN_OK) return rc;
-    const int64_t units = (N + 15) / 16;
+    const int64_t units = (N + kUnitRows - 1) / kUnitRows;
     const unsigned grid = (unsigned)std::min<int64_t>(units, sm_count());
     const size_t smem = (size_t)(kLinearFixed + M * (a.token_stride + K / 32) + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));
     const int vec = (ld_x % 8 == 0 || M == 1) && aligned16(x);

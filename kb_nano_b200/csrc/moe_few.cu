@@ -40,7 +40,7 @@ struct MoeArgs {
     float* y;                      // [pairs, I]
     float* rows;                   // [pairs, H]
     Jobs* jobs;
-    int32_t* counters;             // [H / 16], zeroed by the first kernel
+    int32_t* counters;             // one per column block of the second kernel, zeroed by the first
     __nv_bfloat16* out;
     int64_t ld_out;
     float* out_w;                  // may be null
@@ -58,7 +58,6 @@ struct Scratch {                   // small shared-memory state beside the ring
 };
 
 __host__ __device__ constexpr int scratch_bytes() { return (int)((sizeof(Scratch) + 127) / 128 * 128); }
-constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * 4;
 constexpr int kBarBytes = (2 * kMaxStages + 2 * kFinishers) * 8;
 
 template <int FMT>
@@ -70,7 +69,7 @@ __device__ __forceinline__ Smem carve(uint8_t* raw, int stages, int rows, int to
     s.scales = p;
     p += (size_t)stages * Fmt<FMT>::kScaleBytes;
     s.red = reinterpret_cast<float*>(p);
-    p += kRedBytes;
+    p += kRedBytes<FMT>;
     *scratch = reinterpret_cast<Scratch*>(p);
     p += scratch_bytes();
     s.bars = reinterpret_cast<uint64_t*>(p);
@@ -132,7 +131,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     Scratch& sc = *scp;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        init_ring(s, Fmt<FMT>::kArrivals);
+        init_ring(s);
         sc.abort_flag = 0;
         ptx::prefetch_tensormap(&tm);
     }
@@ -176,11 +175,12 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
             uint32_t* dst = reinterpret_cast<uint32_t*>(a.jobs);
             const int i0 = tid - (warp > kProducerWarp ? 32 : 0);      // the producer is not here
             for (int i = i0; i < (int)(sizeof(Jobs) / 4); i += kThreads - 32) dst[i] = src[i];
-            for (int i = i0; i < a.H / 16; i += kThreads - 32) a.counters[i] = 0;
+            for (int i = i0; i < a.H / (2 * kBoxRows<FMT>); i += kThreads - 32) a.counters[i] = 0;
         }
     }
 
-    const int32_t blocks = a.I / 8, KC = a.H / 128;
+    constexpr int kRows = kBoxRows<FMT>;      // gate rows, and as many up rows, of a unit
+    const int32_t blocks = a.I / kRows, KC = a.H / 128;
     const int64_t units = (int64_t)sc.jobs.n_jobs * blocks;
     const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
     int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
@@ -188,7 +188,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         const WaitCtx w{&sc.abort_flag, a.status, 8};
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
-            const int32_t row = sc.jobs.expert[job] * 2 * a.I + 8 * rb;
+            const int32_t row = sc.jobs.expert[job] * 2 * a.I + kRows * rb;
             produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s13, a.tiled13 ? &tm_scales : nullptr}, row, row + a.I, 2 * a.I * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
@@ -209,7 +209,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
                 loaded = job;
                 columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [&](int col) { return resident ? sc.jobs.pair[job][col] / a.topk : col; });
             }
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[Fmt<FMT>::kTiles][4] = {};
             consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
             if (++rb == blocks) rb = 0, ++job;
@@ -218,16 +218,17 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         const WaitCtx w{&sc.abort_flag, a.status, 19};
         for (int64_t u = u0; u < u1; ++u) {
             if ((u - u0) % kFinishers == warp - kFirstFinisher) {
-                float v[4];
+                float v[Fmt<FMT>::kTiles][4];
                 take_over(s, u - u0, lane, v, w);
                 const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float other = __shfl_down_sync(0xffffffffu, v[i], 16);      // rows 8-15 are the up projection's
-                    if (lane < 16 && tok0 + i < count) {
-                        a.y[(int64_t)sc.jobs.pair[job][tok0 + i] * a.I + 8 * rb + (lane >> 1)] = __fdiv_rn(v[i], 1.0f + expf(-v[i])) * other;
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int tile = 0; tile < Fmt<FMT>::kTiles; ++tile) {
+                        const float gate = v[tile][i], up = __shfl_down_sync(0xffffffffu, gate, 16);      // box 1 is the up projection's
+                        if (lane < 16 && tok0 + i < count)
+                            a.y[(int64_t)sc.jobs.pair[job][tok0 + i] * a.I + kRows * rb + row_of_lane<FMT>(tile, lane)] = __fdiv_rn(gate, 1.0f + expf(-gate)) * up;
                     }
-                }
             }
             if (++rb == blocks) rb = 0, ++job;
         }
@@ -235,10 +236,11 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     drain_after_abort(&sc.abort_flag);
 }
 
-// out[:, 16 rb .. + 15]: each token's rows with their router weights, in slot order, by one warp.
+// COLS output columns of every token: its rows with their router weights, in slot order, by one warp.
+template <int COLS>
 __device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, int rb, int lane) {
-    const int col = 16 * rb + (lane & 15);
-    for (int t = lane >> 4; t < a.T; t += 2) {
+    const int col = COLS * rb + lane % COLS;
+    for (int t = lane / COLS; t < a.T; t += 32 / COLS) {
         float v = 0.f;
         const float* rp = a.rows + (int64_t)t * a.topk * a.H + col;
 #pragma unroll 8
@@ -259,7 +261,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
     Scratch& sc = *scp;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        init_ring(s, Fmt<FMT>::kArrivals);
+        init_ring(s);
         sc.abort_flag = 0;
         ptx::prefetch_tensormap(&tm);
     }
@@ -273,7 +275,8 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
     }
     __syncthreads();
 
-    const int32_t blocks = a.H / 16, KC = a.I / 128, n_jobs = sc.jobs.n_jobs;
+    constexpr int kRows = 2 * kBoxRows<FMT>;      // output columns of a unit
+    const int32_t blocks = a.H / kRows, KC = a.I / 128, n_jobs = sc.jobs.n_jobs;
     if (n_jobs == 0) {                    // no token has an expert: every logit row held a NaN
         for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)a.T * a.H; i += (int64_t)gridDim.x * kThreads)
             a.out[i / a.H * a.ld_out + i % a.H] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
@@ -286,8 +289,8 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         const WaitCtx w{&sc.abort_flag, a.status, 10};
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
-            const int32_t row = sc.jobs.expert[job] * a.H + 16 * rb;
-            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + 8, a.H * a.E, KC, lane, w);
+            const int32_t row = sc.jobs.expert[job] * a.H + kRows * rb;
+            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + kRows / 2, a.H * a.E, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
     } else if (warp < kConsumerWarps) {
@@ -304,7 +307,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 loaded = job;
                 columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [](int col) { return col; });
             }
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[Fmt<FMT>::kTiles][4] = {};
             consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
             hand_over(s, u - u0, warp, lane, acc, w);
             if (++rb == blocks) rb = 0, ++job;
@@ -314,13 +317,14 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         int pending = 0, mine = 0;            // column blocks stored but not yet counted; lane i holds the i-th
         for (int64_t u = u0; u < u1; ++u) {
             if ((u - u0) % kFinishers == warp - kFirstFinisher) {
-                float v[4];
+                float v[Fmt<FMT>::kTiles][4];
                 take_over(s, u - u0, lane, v, w);
                 const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (tok0 + i < count)
-                        a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + 16 * rb + (lane >> 1)] = v[i];
+#pragma unroll
+                    for (int tile = 0; tile < Fmt<FMT>::kTiles; ++tile)
+                        if (tok0 + i < count) a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + kRows * rb + row_of_lane<FMT>(tile, lane)] = v[tile][i];
                 if (lane == pending) mine = rb;
                 ++pending;
             }
@@ -330,7 +334,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 __syncwarp();
                 unsigned last = __ballot_sync(0xffffffffu, lane < pending && atomicAdd(a.counters + mine, 1) == n_jobs - 1);
                 if (last) fence_gpu();
-                for (; last; last &= last - 1) add_up(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
+                for (; last; last &= last - 1) add_up<kRows>(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
                 pending = 0;
             }
             if (++rb == blocks) rb = 0, ++job;
@@ -350,7 +354,7 @@ struct Plan {
 template <int FMT>
 static bool plan(int64_t K, int want, Plan* p) {
     const int64_t stride = K * 2 + Fmt<FMT>::kTokenPad, row = stride + K / 32, per_stage = kStageBytes + Fmt<FMT>::kScaleBytes;
-    const int64_t fixed = 1024 + kRedBytes + scratch_bytes() + kBarBytes;
+    const int64_t fixed = 1024 + kRedBytes<FMT> + scratch_bytes() + kBarBytes;
     for (int g = want; g >= 1; --g) {
         const int64_t left = kSmemMax - fixed - g * row;
         if (left < kMinStages * per_stage) continue;
