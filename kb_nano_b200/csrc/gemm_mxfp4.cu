@@ -27,7 +27,8 @@ namespace mxfp4 {
 constexpr int kTileM = 256;
 constexpr int kABytes = 128 * 128;                             // this CTA's rows of A, one K-step of 256 values
 constexpr int kEpiWarps = 8;
-constexpr int kGemmThreads = 32 * (2 + kEpiWarps);
+constexpr int kScaleWarp = 2 + kEpiWarps;                      // warps: loads, products, epilogue, scales
+constexpr int kGemmThreads = 32 * (kScaleWarp + 1);
 constexpr int kStagingBytes = kEpiWarps * 32 * 128;            // 32 rows x 64 bf16 columns per epilogue warp
 constexpr int kTmemColumns = 512, kColScales = 256;            // accumulators in columns 0-255, scales behind them
 constexpr int kSplitGain = 14;                                 // K-steps a split over the cluster has to save
@@ -43,6 +44,8 @@ struct Cfg {
     static constexpr int kStages = BN == 256 ? 5 : 7;
     static constexpr uint32_t kTxPair = 2u * (kOperandBytes + kSfBytes);
     static constexpr int kAccs = 256 / BN;                     // accumulators: a 128-column tile is drained under the next one
+    static constexpr int kScaleCols = 4 * kSfBlocks;           // scale columns of 128 of K; every ring slot has its own
+    static_assert(kColScales + kStages * 2 * kScaleCols <= kTmemColumns, "tensor memory");
     static constexpr int kSmem = kStages * (kOperandBytes + kSfBytes) + kStagingBytes + 1024 + 256;
     static constexpr int kExchange = 2 * 3 * 128 * (BN / 4) * 4;      // split K: partial sums sent and received, S = 4
     static_assert(kExchange <= kStages * (kOperandBytes + kSfBytes) + kStagingBytes && kSmem <= 232448, "shared memory");
@@ -186,11 +189,12 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     uint8_t* sf = smem + (size_t)kStages * kOperandBytes;
     uint8_t* staging = sf + (size_t)kStages * kSfBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStagingBytes);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 5);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t bar_full = ptx::smem_u32(bars), bar_empty = ptx::smem_u32(bars + kStages);
-    const uint32_t bar_tfull = ptx::smem_u32(bars + 2 * kStages), bar_tempty = bar_tfull + 16, bar_xchg = bar_tfull + 32;      // two accumulators each
+    const uint32_t bar_scales = ptx::smem_u32(bars + 2 * kStages);             // a slot's scales are in tensor memory
+    const uint32_t bar_tfull = ptx::smem_u32(bars + 3 * kStages), bar_tempty = bar_tfull + 16, bar_xchg = bar_tfull + 32;      // two accumulators each
     const uint32_t tiles_smem = ptx::smem_u32(smem), sf_smem = ptx::smem_u32(sf);
 
     const uint32_t rank = ptx::cluster_ctarank();
@@ -201,6 +205,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         for (int s = 0; s < kStages; ++s) {
             ptx::mbar_init(bar_full + 8 * s, 1);         // armed by the even CTA for both CTAs' copies
             ptx::mbar_init(bar_empty + 8 * s, 1);        // one commit, delivered to both
+            ptx::mbar_init(bar_scales + 8 * s, 1);       // one commit, in the even CTA
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(bar_tfull + 8 * i, 1);
@@ -281,16 +286,14 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 }
                 const uint32_t d = tmem + acc * BN;
                 for (int32_t k = k0; k < k1; ++k) {
-                    ok = __all_sync(0xffffffffu, wait_bar(bar_full + 8 * slot, phase, w));
+                    ok = __all_sync(0xffffffffu, wait_bar(bar_scales + 8 * slot, phase, w));      // operands and scales are there
                     if (!ok) break;
                     ptx::tc_fence_after();
-                    const uint32_t a = tiles_smem + slot * kOperandBytes, s = sf_smem + slot * kSfBytes;
+                    const uint32_t a = tiles_smem + slot * kOperandBytes, scales = tmem + kColScales + slot * 2 * F::kScaleCols;
                     const uint64_t a_desc = ptx::umma_desc_k_sw128(a), b_desc = ptx::umma_desc_k_sw128(a + kABytes);
                     const int halves = min(2, p.kblocks - 2 * k);      // the last step may hold one 128-K block only
                     for (int h = 0; h < halves; ++h) {
-                        const uint32_t sfa = tmem + kColScales + 16 * h, sfb = sfa + 4;
-#pragma unroll
-                        for (int b = 0; b < F::kSfBlocks; ++b) copy_scales_pair(sfa + 4 * b, ptx::umma_desc_sf(s + 1024 * b + 512 * h));
+                        const uint32_t sfa = scales + F::kScaleCols * h, sfb = sfa + 4;
                         mma_mxf4_pair(d, a_desc + 4 * h, b_desc + 4 * h, idesc_mxf4(kTileM, BN, 0), sfa, sfb, (k > k0 || h > 0) ? 1u : 0u);
                         mma_mxf4_pair(d, a_desc + 4 * h + 2, b_desc + 4 * h + 2, idesc_mxf4(kTileM, BN, 2), sfa, sfb, 1u);
                     }
@@ -299,6 +302,28 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 }
                 if (ok) commit_pair(bar_tfull + 8 * acc, pair_mask);
                 if (++acc == F::kAccs) acc = 0, acc_phase ^= 1u;
+            }
+        }
+    } else if (warp == kScaleWarp) {
+        // Scales, shared memory -> tensor memory, by a warp of its own: beside the products' warp, whose four instructions a
+        // step then take less time to issue than the tensor cores need for them.
+        if (pr == 0) {
+            const WaitCtx w{abort_flag, p.status, 22};
+            uint32_t slot = 0, phase = 0;
+            bool ok = true;
+            for (int32_t t = cluster; ok && t < tiles; t += stride) {
+                for (int32_t k = k0; k < k1; ++k) {
+                    ok = __all_sync(0xffffffffu, wait_bar(bar_full + 8 * slot, phase, w));
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const uint32_t s = sf_smem + slot * kSfBytes, scales = tmem + kColScales + slot * 2 * F::kScaleCols;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)        // of a last step's missing block: never used
+#pragma unroll
+                        for (int b = 0; b < F::kSfBlocks; ++b) copy_scales_pair(scales + F::kScaleCols * h + 4 * b, ptx::umma_desc_sf(s + 1024 * b + 512 * h));
+                    commit_pair(bar_scales + 8 * slot, (uint16_t)(1u << leader));
+                    if (++slot == kStages) slot = 0, phase ^= 1u;
+                }
             }
         }
     } else if (!SPLIT) {
@@ -368,7 +393,8 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         const uint32_t swz = (uint32_t)r_in_tile & (units - 1u);
         // partial sums of the columns other slices own: rows of W floats, 16-byte units XOR-swizzled by the row so that a
         // lane per row stores without bank conflicts; one bulk copy per owner
-        if (warp >= 2) {
+        const bool epilogue = warp >= 2 && warp < kScaleWarp;
+        if (epilogue) {
 #pragma unroll 1
             for (int cc = half; cc < BN / 32; cc += 2) {
                 const uint32_t o = (uint32_t)(32 * cc / W);
@@ -394,7 +420,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                                           ptx::mapa(bar_xchg, owner));
             }
         }
-        if (warp >= 2) {
+        if (epilogue) {
             const WaitCtx w{abort_flag, p.status, 16};
             wait_bar(bar_xchg, 0u, w);
             __syncwarp();

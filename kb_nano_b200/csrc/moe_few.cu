@@ -250,7 +250,11 @@ __device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, in
 }
 
 constexpr int kCountBatch = 4;
-__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+__device__ __forceinline__ int add_acq_rel_gpu(int32_t* p) {
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+    return old;
+}
 
 template <int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -328,12 +332,14 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 if (lane == pending) mine = rb;
                 ++pending;
             }
-            // One fence and one round of counting for several units.  Who completes a column block (every job once) adds it up.
+            // One round of counting for several units; the release half of the atomic publishes the warp's rows, its acquire
+            // half makes the others' visible.  Who completes a column block (every job once) adds it up.
             if (pending == kCountBatch || (pending > 0 && u + kFinishers >= u1)) {
-                fence_gpu();
                 __syncwarp();
-                unsigned last = __ballot_sync(0xffffffffu, lane < pending && atomicAdd(a.counters + mine, 1) == n_jobs - 1);
-                if (last) fence_gpu();
+                int before = -1;
+                if (lane < pending) before = add_acq_rel_gpu(a.counters + mine);
+                unsigned last = __ballot_sync(0xffffffffu, before == n_jobs - 1);
+                __syncwarp();
                 for (; last; last &= last - 1) add_up<kRows>(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
                 pending = 0;
             }
