@@ -73,6 +73,7 @@ class _MoeBlock(nn.Module):
         getattr(self, scale_names[1]).weight_loader = self._w2_scale_loader
         self.ep_max_tokens, self.ep_max_m = ep_max_tokens, ep_max_m
         self._ep_layer: _ep.EpMoe | None = None
+        self.few_tokens = 0                      # batches up to this size take the few-token kernels; see use_few_tokens
         self._use_custom_op = False
         self._layer_name = ""
 
@@ -117,6 +118,16 @@ class _MoeBlock(nn.Module):
             self._ep_layer.close()
             self._ep_layer = None
 
+    def use_few_tokens(self, max_tokens: int = _moe.FEW_TOKENS_MAX) -> None:
+        """Lets batches of at most `max_tokens` tokens on one rank run as moe.few_tokens_moe, routing included, in two kernels
+        (0 switches it off, the default).  Those kernels leave the activations unquantised, so a small batch then differs
+        from the same tokens inside a larger one by the FP8 rounding of the larger one's activations."""
+        if not 0 <= max_tokens <= _moe.FEW_TOKENS_MAX:
+            raise ValueError(f"the few-token kernels take at most {_moe.FEW_TOKENS_MAX} tokens, got {max_tokens}")
+        if max_tokens and self.ep_size != 1:
+            raise ValueError("the few-token kernels run on one rank; this layer spans several")
+        self.few_tokens = max_tokens
+
     def _ep(self, x: torch.Tensor) -> "_ep.EpMoe":
         t = x.shape[0]
         if t > self.ep_max_tokens:
@@ -132,6 +143,9 @@ class _MoeBlock(nn.Module):
         """Router logits -> experts.  One rank: the routing kernel, then the single-GPU pipeline.  Several ranks: the
         expert-parallel layer routes inside its dispatch kernel."""
         if self.ep_size == 1:
+            if 0 < x.shape[0] <= self.few_tokens:
+                w13_s, w2_s = getattr(self, self._scale_names[0]), getattr(self, self._scale_names[1])
+                return _moe.few_tokens_moe(x, router_logits, self.w13, w13_s, self.w2, w2_s, self.top_k, **route)
             tw, ti = _ops.moe_route_topk(router_logits, self.top_k, **route)
             return self._run_experts(x, tw, ti)
         w13_s, w2_s = getattr(self, self._scale_names[0]), getattr(self, self._scale_names[1])
@@ -200,11 +214,17 @@ class MixtralMoE(_MoeBlock):
         self._init_experts(config.num_local_experts, config.hidden_size, config.intermediate_size, config.num_experts_per_tok,
                            ("w13_scale", "w2_scale"), group)
 
+    def use_few_tokens(self, max_tokens: int = _moe.FEW_TOKENS_MAX) -> None:
+        if max_tokens:
+            raise NotImplementedError("MixtralMoE rounds its router weights to bf16, which the few-token kernels do not")
+        super().use_few_tokens(0)
+
     def forward_impl(self, hidden_states: torch.Tensor) -> torch.Tensor:
         orig_shape = hidden_states.shape
         x = hidden_states.reshape(-1, self.hidden_size)
         x = x if x.is_contiguous() else x.contiguous()
         router_logits = self.gate(x)
+        # always routed apart: the few-token kernels do not round the weights
         tw, ti = _ops.moe_route_topk(router_logits, self.top_k, "softmax", renormalize=True, renorm_floor=1e-20)
         tw = tw.to(x.dtype).float()              # the baseline's topk_weights.to(hidden_states.dtype)
         out = self._run_experts(x, tw, ti)

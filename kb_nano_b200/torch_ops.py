@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import moe, ops
 
 
 @torch.library.custom_op("kbn_b200::per_token_group_quant_fp8", mutates_args=("output_fp8", "output_scale"))
@@ -40,3 +40,29 @@ def m_grouped_gemm_nt_contiguous(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_f
 def m_grouped_gemm_nt_masked(a_fp8: torch.Tensor, a_scale: torch.Tensor, b_fp8: torch.Tensor,
                              b_scale: torch.Tensor, c_bf16: torch.Tensor, masked_m: torch.Tensor) -> None:
     ops.m_grouped_fp8_gemm_nt_masked(a_fp8, a_scale, b_fp8, b_scale, c_bf16, masked_m)
+
+
+# The 4-bit counterparts and the MoE layer for a few tokens (no counterpart in kb-nano).
+
+@torch.library.custom_op("kbn_b200::quant_mxfp4", mutates_args=("output_fp4", "output_scale"))
+def quant_mxfp4(input: torch.Tensor, output_fp4: torch.Tensor, output_scale: torch.Tensor) -> None:
+    ops.quant_mxfp4(input, output_fp4, output_scale)
+
+
+@torch.library.custom_op("kbn_b200::silu_mul_quant_mxfp4", mutates_args=("output_fp4", "output_scale"))
+def silu_mul_quant_mxfp4(input: torch.Tensor, output_fp4: torch.Tensor, output_scale: torch.Tensor) -> None:
+    ops.silu_mul_quant_mxfp4(input, output_fp4, output_scale)
+
+
+@torch.library.custom_op("kbn_b200::mxfp4_linear", mutates_args=("a_fp4", "a_packed", "output"))
+def mxfp4_linear(input: torch.Tensor, a_fp4: torch.Tensor, a_packed: torch.Tensor, b_fp4: torch.Tensor, b_packed: torch.Tensor,
+                 output: torch.Tensor, bias: torch.Tensor | None = None) -> None:
+    ops.mxfp4_linear(input, a_fp4, a_packed, b_fp4, b_packed, output, bias)
+
+
+@torch.library.custom_op("kbn_b200::few_tokens_moe", mutates_args=("output",))
+def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
+                   w2_scale: torch.Tensor, output: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None,
+                   n_group: int = 1, topk_group: int = 1, renormalize: bool = True, renorm_floor: float = 0.0, scale: float = 1.0) -> None:
+    moe.few_tokens_moe(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, scoring, bias, n_group, topk_group, renormalize,
+                       renorm_floor, scale, out=output)

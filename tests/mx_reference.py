@@ -79,14 +79,22 @@ def route(logits: torch.Tensor, top_k: int, scoring="softmax", bias=None, n_grou
     return w * scale, ids
 
 
-def moe(x, w13, w2, w, ids):
+def moe(x, w13, w2, w, ids, fp8_activations=False):
     """fp64 layer and, per output, a bound on the kernel's error.  w13(e), w2(e): the experts' fp64 weights.
 
     u = 2^-24.  A sum of K fp32 products in any order is off by at most K u sum|a b|.  Beside that the kernel rounds: the
     tokens not at all (bf16 in f16 with a power of two per row), silu's exponential, add and divide and the product with
     the up projection (16 u is generous for the four), the activated rows to 11 bits (2^-11) and the result to bf16 (2^-8).
-    |silu'| <= 1.1."""
+    |silu'| <= 1.1.
+    fp8_activations: the bound of a pipeline that holds gate, up, silu and their product in bf16 (2^-8 each) and rounds tokens and
+    activated rows to e4m3 with a power-of-two scale per 128 values: 2^-4 of a value, or half of the smallest step, 2^-10 of a
+    scale of at most 2^-7.8 of the largest value (2 / 448), whichever is more."""
     u = 2.0**-24
+
+    def fp8(v):
+        return v.abs() * 2.0**-4 + v.abs().amax(dim=1, keepdim=True) * 2.0**-17.8 if fp8_activations else 0.0 * v
+
+    store = 2.0**-8 if fp8_activations else 0.0
     t, h = x.shape
     out = torch.zeros(t, h, dtype=torch.float64, device=x.device)
     err = torch.zeros_like(out)
@@ -97,13 +105,15 @@ def moe(x, w13, w2, w, ids):
         xe = x[tok].double()
         both, mag = xe @ a.t(), xe.abs() @ a.abs().t()
         g, up = both[:, :i], both[:, i:]
-        dg, du = mag[:, :i] * (h + 16) * u, mag[:, i:] * (h + 16) * u
+        d = mag * (h + 16) * u + fp8(xe) @ a.abs().t() + both.abs() * store
+        dg, du = d[:, :i], d[:, i:]
         s = g * torch.sigmoid(g)
         y = s * up
-        dy = 1.1 * dg * up.abs() + s.abs() * du + 1.1 * dg * du + y.abs() * (16 * u + 2.0**-11)
+        dy = 1.1 * dg * up.abs() + s.abs() * du + 1.1 * dg * du + y.abs() * (16 * u + 2.0**-11 + 2 * store)
+        dy = dy + fp8(y.abs() + dy)
         row = y @ b.t()
         drow = dy @ b.abs().t() + (y.abs() @ b.abs().t()) * (i + 16) * u
         ws = w[tok, slot].double().unsqueeze(1)
         out.index_add_(0, tok, ws * row)
-        err.index_add_(0, tok, ws.abs() * (drow + row.abs() * 64 * u))      # the weight itself, the weighted sum
+        err.index_add_(0, tok, ws.abs() * (drow + row.abs() * (64 * u + store)))      # the weight itself, the weighted sum
     return out, err + out.abs() * 2.0**-8 + 1e-30

@@ -204,3 +204,80 @@ def test_refusals(cuda_dev):
         off = torch.zeros(2, 264, dtype=torch.bfloat16, device=cuda_dev)[:, 1:257]
         moe.few_tokens_moe(off, lg, w13, s13, w2, s2, 2)
 
+
+def test_layers_take_it_when_told_to(cuda_dev):
+    """Qwen3MoE and DeepSeekMoE with use_few_tokens: both forms within their own error of the layer in 64 bits (the pipeline's is
+    the FP8 rounding of its activations), larger batches and the default untouched, MixtralMoE refuses (its router weights
+    are rounded to bf16)."""
+    from types import SimpleNamespace
+
+    from kb_nano_b200 import layers, moe, ops
+    quant = {"weight_block_size": [128, 128]}
+    e, h, i, top = 16, 512, 256, 4
+    w13, s13, w2, s2, f13, f2 = experts("fp8", e, h, i, cuda_dev, 30)
+    qwen = layers.Qwen3MoE(SimpleNamespace(num_experts=e, num_experts_per_tok=top, hidden_size=h, moe_intermediate_size=i, norm_topk_prob=True), quant)
+    deep = layers.DeepSeekMoE(SimpleNamespace(n_routed_experts=e, num_experts_per_tok=top, hidden_size=h, moe_intermediate_size=i, n_group=4, topk_group=2,
+                                              scoring_func="sigmoid", norm_topk_prob=True, topk_method="noaux_tc", n_shared_experts=None,
+                                              routed_scaling_factor=1.5), quant)
+    for layer, names in ((qwen, ("w13_scale", "w2_scale")), (deep, ("w13_weight_scale_inv", "w2_weight_scale_inv"))):
+        layer.to(cuda_dev)
+        layer.w13.data, layer.w2.data = w13, w2
+        getattr(layer, names[0]).data, getattr(layer, names[1]).data = s13, s2
+        gate = layer.gate.weight if layer is qwen else layer.gate_weight
+        gate.data = (torch.randn(e, h, device=cuda_dev) * 0.1).to(torch.bfloat16)
+        layer.requires_grad_(False)
+        x = torch.randn(3, 4, h, device=cuda_dev).to(torch.bfloat16)
+        before = layer(x)
+        layer.use_few_tokens()
+        got = layer(x)
+        assert got.shape == x.shape and not torch.equal(got, before)
+        flat, logits = x.view(12, h), torch.nn.functional.linear(x.view(12, h), gate)
+        if layer is qwen:
+            w, ids = ref.route(logits, top)
+            factor = 1.0
+        else:                                                     # bf16 scores and weights: taken from the routing kernel
+            w, ids = ops.moe_route_topk(logits, top, "sigmoid", layer.e_score_correction_bias, 4, 2, True, round_bf16=True)
+            factor = 1.5                                           # applied to the rounded bf16 result: one more rounding
+        for out, fp8 in ((got, False), (before, True)):
+            want, err = ref.moe(flat, f13, f2, w.double(), ids.long(), fp8)
+            check(out.view(12, h), want * factor, err * factor + (want.abs() * factor * 2.0**-8 if factor != 1.0 else 0.0))
+        big = torch.randn(20, h, device=cuda_dev).to(torch.bfloat16)
+        many = layer(big)
+        layer.use_few_tokens(0)
+        assert torch.equal(layer(x), before) and torch.equal(layer(big), many)
+        with pytest.raises(ValueError, match="at most"):
+            layer.use_few_tokens(17)
+    mixtral = layers.MixtralMoE(SimpleNamespace(num_local_experts=e, num_experts_per_tok=2, hidden_size=h, intermediate_size=i), quant)
+    with pytest.raises(NotImplementedError):
+        mixtral.use_few_tokens()
+    assert ops.gemm_status(cuda_dev) == 0 and moe.FEW_TOKENS_MAX == 16
+
+
+def test_registered_ops(cuda_dev):
+    from kb_nano_b200 import moe, ops, torch_ops  # noqa: F401
+    w13, s13, w2, s2, _, _ = experts("mxfp4", 4, 256, 128, cuda_dev, 31)
+    x, lg = torch.randn(3, 256, device=cuda_dev).to(torch.bfloat16), torch.randn(3, 4, device=cuda_dev)
+    out = torch.empty_like(x)
+    torch.ops.kbn_b200.few_tokens_moe(x, lg, w13, s13, w2, s2, out, 2)
+    assert torch.equal(out, moe.few_tokens_moe(x, lg, w13, s13, w2, s2, 2))
+    q, s = torch.empty(3, 128, dtype=torch.uint8, device=cuda_dev), torch.empty(3, 8, dtype=torch.uint8, device=cuda_dev)
+    torch.ops.kbn_b200.quant_mxfp4(x, q, s)
+    assert torch.equal(q, ref.quant(x)[0]) and torch.equal(s, ref.quant(x)[1])
+    wp, sf = ops.pack_mxfp4_scales(s2[0].contiguous(), 128), torch.empty(ops.packed_mxfp4_bytes(3, 128), dtype=torch.uint8, device=cuda_dev)
+    y, y2 = torch.empty(3, 256, dtype=torch.bfloat16, device=cuda_dev), torch.empty(3, 256, dtype=torch.bfloat16, device=cuda_dev)
+    half = x[:, :128].contiguous()
+    torch.ops.kbn_b200.mxfp4_linear(half, q[:, :64].contiguous(), sf, w2[0], wp, y)
+    ops.mxfp4_linear(half, q[:, :64].contiguous(), sf, w2[0], wp, y2)
+    assert torch.equal(y, y2)
+
+
+def test_two_gpus_worth_of_checks_on_one(cuda_dev):
+    """Tensors that live on another device than the others are refused before anything is launched."""
+    from kb_nano_b200 import moe
+    w13, s13, w2, s2, _, _ = experts("fp8", 4, 256, 128, cuda_dev, 32)
+    x, lg = torch.zeros(1, 256, dtype=torch.bfloat16, device=cuda_dev), torch.zeros(1, 4, device=cuda_dev)
+    for bad in range(6):
+        args = [x, lg, w13, s13, w2, s2]
+        args[bad] = args[bad].cpu()
+        with pytest.raises(ValueError, match="CUDA tensors|same device"):
+            moe.few_tokens_moe(*args, 2)
