@@ -424,36 +424,48 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             const WaitCtx w{abort_flag, p.status, 16};
             wait_bar(bar_xchg, 0u, w);
             __syncwarp();
-            if (quarter * 32 < live) {
+            if (quarter * 32 < live && *abort_flag == 0) {
+                // this warp's half of the owned band; two slices leave the staging rows free and hand whole boxes to the TMA
+                const bool boxes = p.S == 2 && p.tiled_out;
+                const uint32_t mine = ptx::smem_u32(staging) + (uint32_t)(warp - 2) * (32 * 128);
+                const int32_t c0 = (int32_t)ks * W + half * (W / 2);
 #pragma unroll 1
-                for (int cc = half; cc < BN / 32; cc += 2) {
-                    if ((uint32_t)(32 * cc / W) != ks) continue;
+                for (int c = 0; c < W / 64; ++c) {
+                    const int32_t col = c0 + 32 * c, n0 = nt * BN + col;
                     uint32_t r[32];
-                    ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + 32 * cc, r);
+                    ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + col, r);
                     ptx::tmem_ld_wait(r);
-                    if (r_in_tile < live && *abort_flag == 0) {
-                        float f[32];
+                    float f[32];
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) f[q] = 0.f;
-                        const uint32_t u0 = (uint32_t)(32 * cc % W) / 4u;
-                        for (uint32_t sl = 0; sl < (uint32_t)p.S; ++sl) {
-                            if (sl == ks) {
+                    for (int q = 0; q < 32; ++q) f[q] = 0.f;
+                    const uint32_t u0 = (uint32_t)(col % W) / 4u;
+                    for (uint32_t sl = 0; sl < (uint32_t)p.S; ++sl) {
+                        if (sl == ks) {
 #pragma unroll
-                                for (int q = 0; q < 32; ++q) f[q] += __uint_as_float(r[q]);
-                                continue;
-                            }
-                            const uint32_t recv = sl < ks ? sl : sl - 1u;
-                            const uint32_t base = tiles_smem + ((uint32_t)(p.S - 1) + recv) * slot_bytes + (uint32_t)r_in_tile * (uint32_t)W * 4u;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float4 v = ptx::ld_shared_v4(base + (((u0 + (uint32_t)i) ^ swz) << 4));
-                                f[4 * i + 0] += v.x; f[4 * i + 1] += v.y; f[4 * i + 2] += v.z; f[4 * i + 3] += v.w;
-                            }
+                            for (int q = 0; q < 32; ++q) f[q] += __uint_as_float(r[q]);
+                            continue;
                         }
-                        add_bias(f, p, nt * BN + 32 * cc);
-                        store_row(f, p, row0 + r_in_tile, nt * BN + 32 * cc);
+                        const uint32_t recv = sl < ks ? sl : sl - 1u;
+                        const uint32_t base = tiles_smem + ((uint32_t)(p.S - 1) + recv) * slot_bytes + (uint32_t)r_in_tile * (uint32_t)W * 4u;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 v = ptx::ld_shared_v4(base + (((u0 + (uint32_t)i) ^ swz) << 4));
+                            f[4 * i + 0] += v.x; f[4 * i + 1] += v.y; f[4 * i + 2] += v.z; f[4 * i + 3] += v.w;
+                        }
+                    }
+                    add_bias(f, p, n0);
+                    if (boxes) {
+                        stage_row(f, mine, lane, c & 1);
+                        if ((c & 1) == 1 && n0 - 32 < p.N) {
+                            ptx::fence_proxy_async();
+                            __syncwarp();
+                            store_box(&tmC, (n0 - 32) * 2, row0 + quarter * 32, mine);
+                        }
+                    } else if (r_in_tile < live) {
+                        store_row(f, p, row0 + r_in_tile, n0);
                     }
                 }
+                stores_have_read();
             }
         }
     }

@@ -236,16 +236,23 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     drain_after_abort(&sc.abort_flag);
 }
 
-// COLS output columns of every token: its rows with their router weights, in slot order, by one warp.
+// COLS output columns of every token: its rows with their router weights, in slot order, by one warp.  Two columns a lane,
+// so that several tokens' rows are under way at once: this is the last thing a block does, and round trips to L2 count.
 template <int COLS>
 __device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, int rb, int lane) {
-    const int col = COLS * rb + lane % COLS;
-    for (int t = lane / COLS; t < a.T; t += 32 / COLS) {
-        float v = 0.f;
-        const float* rp = a.rows + (int64_t)t * a.topk * a.H + col;
+    const int col = COLS * rb + 2 * (lane % (COLS / 2));
+    for (int t = lane / (COLS / 2); t < a.T; t += 64 / COLS) {
+        float2 v = make_float2(0.f, 0.f);
+        const float2* rp = reinterpret_cast<const float2*>(a.rows + (int64_t)t * a.topk * a.H + col);
 #pragma unroll 8
-        for (int k = 0; k < a.topk; ++k) v = fmaf(weight[t * a.topk + k], __ldcg(rp + (int64_t)k * a.H), v);
-        a.out[(int64_t)t * a.ld_out + col] = __float2bfloat16_rn(v);
+        for (int k = 0; k < a.topk; ++k) {
+            const float2 r = __ldcg(rp + (int64_t)k * (a.H / 2));
+            v.x = fmaf(weight[t * a.topk + k], r.x, v.x);
+            v.y = fmaf(weight[t * a.topk + k], r.y, v.y);
+        }
+        __nv_bfloat16* o = a.out + (int64_t)t * a.ld_out + col;
+        o[0] = __float2bfloat16_rn(v.x);
+        o[1] = __float2bfloat16_rn(v.y);
     }
 }
 
