@@ -704,7 +704,7 @@ def _check_byte_scales(s: torch.Tensor, m: int, k: int, what: str) -> int:
 def _check_packed_mxfp4(buf: torch.Tensor, rows: int, k: int, what: str) -> int:
     """Address of a packed scale buffer of [rows, k] values."""
     ptr = buf.data_ptr()
-    if ptr & 15 or buf.dtype != torch.uint8 or buf.numel() < packed_mxfp4_bytes(rows, k) or not buf.is_contiguous():
+    if ptr & 15 or buf.dtype != torch.uint8 or buf.numel() < ((rows + 127) >> 7) * ((k + 127) >> 7) << 9 or not buf.is_contiguous():
         raise ValueError(f"{what} must be a contiguous, 16-byte aligned uint8 buffer with at least {packed_mxfp4_bytes(rows, k)} bytes")
     return ptr
 
@@ -777,10 +777,12 @@ def _check_mxfp4_operand(q: torch.Tensor, sf: torch.Tensor, rows: int, k: int, w
 
 
 def _check_out(out: torch.Tensor, m: int, n: int) -> int:
-    rows, cols, ld = _bf16_rows(out, "out")
-    if rows != m or cols != n:
-        raise ValueError(f"out must be bf16 [{m}, {n}], got {tuple(out.shape)}")
-    return ld
+    if out.dtype != torch.bfloat16 or out.shape != (m, n):
+        raise ValueError(f"out must be bf16 [{m}, {n}], got {out.dtype} {tuple(out.shape)}")
+    ld, step = out.stride()
+    if step != 1 and n > 1:
+        raise ValueError(f"out must be contiguous along the last dim, got strides {out.stride()}")
+    return ld if m > 1 else n
 
 
 def mxfp4_gemm_nt(a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
@@ -805,7 +807,11 @@ def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: to
     if k % MX_BLOCK or k == 0:
         raise ValueError(f"x must have a multiple of {MX_BLOCK} columns, got {k}")
     n = b_q.size(0)
-    a_sf_ptr, b_sf_ptr, ld = _check_mxfp4_operand(a_q, a_sf, m, k, "a"), _check_mxfp4_operand(b_q, b_sf, n, k, "b"), _check_out(out, m, n)
-    index = _gpu(x, a_q, a_sf, b_q, b_sf, out)
-    _call(index, _lib.load().kbn_mxfp4_linear, x.data_ptr(), ld_x, m, k, a_q.data_ptr(), a_sf_ptr, b_q.data_ptr(), b_sf_ptr,
-          None if bias is None else _bias_ptr(bias, n, out.device), out.data_ptr(), ld, n)
+    if _check_codes(a_q, m, k, "a_q") != k // 2 or _check_codes(b_q, n, k, "b_q") != k // 2:
+        raise ValueError("a_q and b_q must be contiguous")
+    a_sf_ptr, b_sf_ptr, ld = _check_packed_mxfp4(a_sf, m, k, "a_sf"), _check_packed_mxfp4(b_sf, n, k, "b_sf"), _check_out(out, m, n)
+    index = x.get_device()
+    if index < 0 or not index == a_q.get_device() == a_sf.get_device() == b_q.get_device() == b_sf.get_device() == out.get_device():
+        _cuda(x, a_q, a_sf, b_q, b_sf, out)
+    bias_ptr = None if bias is None else _bias_ptr(bias, n, out.device)
+    _call(index, _lib.load().kbn_mxfp4_linear, x.data_ptr(), ld_x, m, k, a_q.data_ptr(), a_sf_ptr, b_q.data_ptr(), b_sf_ptr, bias_ptr, out.data_ptr(), ld, n)
