@@ -318,8 +318,9 @@ int kbn_pack_mxfp4_scales(const void* scale, int64_t rows, int64_t K, int64_t s_
  * packed form, fp32 accumulation (tcgen05 kind::mxf4), bf16 out with row stride ldc.  bias: bf16 [N] or null.  K % 32 == 0;
  * operand pointers 16-byte aligned.  The 4-bit counterpart of kbn_fp8_gemm_nt_ue8m0.
  * kbn_mxfp4_linear: the same on bf16 rows x [M,K] (row stride ld_x), quantised on the way as kbn_quant_mxfp4 does.  a_q
- * (M*K/2 bytes) and a_sf (kbn_packed_mxfp4_bytes(M, K) bytes) are scratch, 16-byte aligned; up to eight rows with
- * K % 128 == 0 take one launch that leaves them untouched, if the rows fit the shared memory of an SM. */
+ * (M*K/2 bytes) and a_sf (kbn_packed_mxfp4_bytes(M, K) bytes) are scratch, 16-byte aligned, one each for calls that may
+ * overlap in time; up to eight rows with K % 128 == 0 take one launch that leaves them untouched, if the rows fit the shared
+ * memory of an SM.  C must not share memory with x (rows side by side in one matrix are fine): refused. */
 int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const void* B, const void* sfb_packed, const void* bias,
                       void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, kbn_stream_t stream);
 int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t K, void* a_q, void* a_sf, const void* B,
@@ -336,8 +337,9 @@ int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t K, void* a_
  *     All contiguous.
  *   out [T,H] bf16, row stride ld_out; out_w fp32 [T,topk] and out_ids int32 [T,topk] (both or neither): the routing.
  * The activations are not quantised (a few tokens cost no bytes): out = bf16(sum_s w_s * W2 (silu(W1 x) * (W3 x))), summed
- * in fp32 in slot order, tokens and activated rows rounded to 11 bits beside a power of two per row.  A token whose logits
- * hold a NaN gets NaNs (and ids -1).  workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents
+ * in fp32 in slot order, tokens and activated rows rounded to 11 bits beside a power of two per 128 values.  A NaN logit
+ * makes all of a softmax router's scores NaN, and only its own expert's score of a sigmoid router; a NaN score is never
+ * chosen.  A token without a single choice gets ids -1 and a row of NaNs.  out may be x.  workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents
  * irrelevant; calls that may overlap need one each.  KBN_ERR_UNSUPPORTED when a row of max(H, I) values does not fit the
  * shared memory of an SM (about 55,000).  Waits inside are bounded and report through kbn_gemm_status.
  */

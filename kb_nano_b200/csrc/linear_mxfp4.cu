@@ -174,6 +174,17 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     return KBN_OK;
 }
 
+// Whether M rows of na and of nb bf16 values share memory.  Rows that lie side by side in
+// one wider matrix (equal strides) do not; with unequal strides the whole extents count.
+static bool rows_overlap(const void* a, int64_t ld_a, int64_t na, const void* b, int64_t ld_b, int64_t nb, int64_t M) {
+    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a), pb = (int64_t)reinterpret_cast<uintptr_t>(b);
+    if (M == 1) ld_a = ld_b = 0;
+    if (pa + 2 * (ld_a * (M - 1) + na) <= pb || pb + 2 * (ld_b * (M - 1) + nb) <= pa) return false;
+    if (ld_a != ld_b || M == 1) return true;
+    const int64_t ld = 2 * ld_a, d = ((pb - pa) % ld + ld) % ld;      // where b's rows start in a's
+    return d < 2 * na || d + 2 * nb > ld;
+}
+
 }  // namespace few
 }  // namespace kbn
 
@@ -188,6 +199,8 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
     KBN_REQUIRE(aligned16(B) && aligned16(sfb_packed) && aligned16(a_q) && aligned16(a_sf), KBN_ERR_ARG, "kbn_mxfp4_linear: pointers must be 16-byte aligned");
     KBN_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1u) == 0 && (reinterpret_cast<uintptr_t>(C) & 1u) == 0 && ((ld_x >= K && ldc >= N) || M == 1), KBN_ERR_ARG,
                 "kbn_mxfp4_linear: odd pointer or a row stride too small");
+    // the one-launch form still reads x where it already writes C
+    KBN_REQUIRE(!rows_overlap(x, ld_x, K, C, ldc, N, M), KBN_ERR_ARG, "kbn_mxfp4_linear: x and the output overlap");
     // The weight stream serves up to eight rows, as long as their f16 values leave room for the ring.
     if (M <= kMaxGroup && K % 128 == 0 && K < (1ll << 17) && N < (1ll << 27)) {
         const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad + K / 32);

@@ -126,6 +126,10 @@ class _MoeBlock(nn.Module):
             raise ValueError(f"the few-token kernels take at most {_moe.FEW_TOKENS_MAX} tokens, got {max_tokens}")
         if max_tokens and self.ep_size != 1:
             raise ValueError("the few-token kernels run on one rank; this layer spans several")
+        e, h, i = self.w13.shape[0], self.w2.shape[1], self.w2.shape[2]
+        if max_tokens and (self.top_k > 16 or e > 1024 or h % 128 or i % 128):
+            raise ValueError(f"the few-token kernels take at most 16 of 1024 experts and sizes that are multiples of 128 (top_k={self.top_k}, experts={e}, "
+                             f"hidden={h}, intermediate={i})")
         self.few_tokens = max_tokens
 
     def _ep(self, x: torch.Tensor) -> "_ep.EpMoe":

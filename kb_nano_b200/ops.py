@@ -801,8 +801,9 @@ def mxfp4_gemm_nt(a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf
 def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf: torch.Tensor, out: torch.Tensor,
                  bias: torch.Tensor | None = None) -> None:
     """The MXFP4 linear layer: x bf16 [M,K], quantised as quant_mxfp4 does, times b_q [N,K/2] / b_sf (packed) into out bf16
-    [M,N].  a_q uint8 [M,K/2] and a_sf (packed_mxfp4_bytes(M, K) bytes) are scratch for the quantised rows; up to eight rows
-    are quantised inside the one kernel that multiplies them and leave the scratch untouched."""
+    [M,N], which must not share memory with x.  a_q uint8 [M,K/2] and a_sf (packed_mxfp4_bytes(M, K) bytes) are scratch for the
+    quantised rows (calls that may overlap in time need their own); up to eight rows, K a multiple of 128, are quantised inside
+    the one kernel that multiplies them and leave the scratch untouched."""
     m, k, ld_x = _bf16_rows(x, "x")
     if k % MX_BLOCK or k == 0:
         raise ValueError(f"x must have a multiple of {MX_BLOCK} columns, got {k}")

@@ -281,3 +281,31 @@ def test_two_gpus_worth_of_checks_on_one(cuda_dev):
         args[bad] = args[bad].cpu()
         with pytest.raises(ValueError, match="CUDA tensors|same device"):
             moe.few_tokens_moe(*args, 2)
+
+
+def test_a_nan_logit_of_a_sigmoid_router_takes_one_expert_away(cuda_dev):
+    """Seven of eight experts left for top-4, then three left: the fourth slot repeats the lowest choice, as ops.moe_route_topk does."""
+    from kb_nano_b200 import moe, ops
+    w13, s13, w2, s2, f13, f2 = experts("fp8", 8, 256, 128, cuda_dev, 33)
+    x = torch.randn(3, 256, device=cuda_dev).to(torch.bfloat16)
+    lg = torch.randn(3, 8, device=cuda_dev)
+    lg[0, 2] = float("nan")
+    lg[1, :5] = float("nan")
+    ow, oi = torch.empty(3, 4, device=cuda_dev), torch.empty(3, 4, dtype=torch.int32, device=cuda_dev)
+    got = moe.few_tokens_moe(x, lg, w13, s13, w2, s2, 4, "sigmoid", out_w=ow, out_ids=oi)
+    w, ids = ops.moe_route_topk(lg, 4, "sigmoid")
+    assert torch.equal(ow, w) and torch.equal(oi, ids.to(torch.int32))
+    assert 2 not in oi[0].tolist() and min(oi[1].tolist()) >= 5
+    want, err = ref.moe(x, f13, f2, w.double(), ids.long(), False)
+    check(got, want, err)
+
+
+def test_layers_refuse_what_the_kernels_do_not_take(cuda_dev):
+    from types import SimpleNamespace
+
+    from kb_nano_b200 import layers
+    wide = layers.Qwen3MoE(SimpleNamespace(num_experts=32, num_experts_per_tok=17, hidden_size=256, moe_intermediate_size=128, norm_topk_prob=True),
+                           {"weight_block_size": [128, 128]})
+    with pytest.raises(ValueError, match="at most 16"):
+        wide.use_few_tokens()
+    wide.use_few_tokens(0)

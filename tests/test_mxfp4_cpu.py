@@ -43,6 +43,12 @@ def test_gemm_arguments(kbn_lib):
     assert lin(A, 64, 4, 64, A, A, A, A, None, A, 16, 0, None) == 0
 
 
+def test_linear_refuses_an_output_on_top_of_its_input(kbn_lib):
+    lin = kbn_lib.kbn_mxfp4_linear
+    for ld_x, m, c, ldc in [(64, 4, A, 64), (64, 4, A + 32, 64), (64, 1, A + 126, 16), (64, 1, A - 30, 16), (256, 4, A + 3 * 512 + 96, 16), (256, 4, A + 512 - 16, 256)]:
+        refused(kbn_lib, lin(A, ld_x, m, 64, 2 * A, 2 * A, 2 * A, 2 * A, None, c, ldc, 16, None), "overlap")
+
+
 def moe_args(**kw):
     d = dict(x=A, ld_x=256, T=2, logits=A, bf16=0, ld=8, E=8, softmax=1, bias=None, n_group=1, topk_group=1, topk=2, renorm=1, floor=0.0, scale=1.0, round=0,
              fmt=0, w13=A, s13=A, w2=A, s2=A, H=256, I=128, out=A, ld_out=256, ow=None, oi=None, ws=A, wb=1 << 30)

@@ -222,3 +222,113 @@ def test_refusals(cuda_dev):
         ops.mxfp4_gemm_nt(aq[:, :24].contiguous(), asf, bq[:, :24].contiguous(), bsf, out)
     with pytest.raises(ValueError, match="CUDA tensors"):
         ops.mxfp4_gemm_nt(aq.cpu(), asf, bq, bsf, out)
+
+
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_input_and_output_side_by_side_in_one_matrix(cuda_dev, m):
+    """Rows of x and of the result as columns of one buffer: allowed, since they share no memory."""
+    from kb_nano_b200 import ops
+    n, k = 64, 256
+    gen = torch.Generator(device=cuda_dev).manual_seed(60 + m)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bsf = ops.pack_mxfp4_scales(bsc, k)
+    both = torch.randn(m, n + k + 8, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    before = both.clone()
+    want = linear(both[:, n:n + k].contiguous(), bq, bsf, n)
+    linear(both[:, n:n + k], bq, bsf, n, out=both[:, :n])
+    assert torch.equal(both[:, :n], want) and torch.equal(both[:, n:], before[:, n:])
+
+
+def test_rows_further_apart_than_32_bit_offsets(cuda_dev):
+    """Three rows 1.1 G values apart, in and out of every 4-bit entry point: the same bits as from close rows."""
+    from kb_nano_b200 import ops
+    ld, k, n = 1_100_000_000, 512, 264
+    big = torch.empty(2 * ld + 1024, dtype=torch.bfloat16, device=cuda_dev)
+    gen = torch.Generator(device=cuda_dev).manual_seed(70)
+
+    def far(cols, dtype=torch.bfloat16, stride=ld):
+        return big.view(dtype).as_strided((3, cols), (stride, 1))
+
+    x = torch.randn(3, k, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    q, s = torch.empty(3, k // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(3, k // 32, dtype=torch.uint8, device=cuda_dev)
+    sf = torch.empty(ops.packed_mxfp4_bytes(3, k), dtype=torch.uint8, device=cuda_dev)
+    ops.quant_mxfp4(x, q, s, sf)
+    far(k).copy_(x)
+    q2, s2 = torch.empty_like(q), torch.empty_like(s)
+    ops.quant_mxfp4(far(k), q2, s2)
+    assert torch.equal(q2, q) and torch.equal(s2, s)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bsf = ops.pack_mxfp4_scales(bsc, k)
+    want = linear(x, bq, bsf, n)
+    assert torch.equal(linear(far(k), bq, bsf, n), want)                                     # far rows in
+    linear(x, bq, bsf, n, out=far(n))                                                        # and out, one launch
+    assert torch.equal(far(n), want)
+    gemm = torch.empty(3, n, dtype=torch.bfloat16, device=cuda_dev)
+    ops.mxfp4_gemm_nt(q, sf, bq, bsf, gemm)
+    for offset in (0, 3):                                                                    # stored as boxes, and value by value
+        view = big.as_strided((3, n), (ld, 1), offset)
+        ops.mxfp4_gemm_nt(q, sf, bq, bsf, view)
+        assert torch.equal(view, gemm)
+    fq, fs = far(k // 2, torch.uint8, 2 * ld - 8), torch.empty_like(s)
+    ops.quant_mxfp4(x, fq, fs)
+    assert torch.equal(fq, q) and torch.equal(fs, s)
+    near = torch.empty_like(x)
+    ops.dequant_mxfp4(q, s, near)
+    ops.dequant_mxfp4(q, s, far(k))
+    assert torch.equal(far(k), near)
+    a, b = torch.empty(3, k // 4, dtype=torch.uint8, device=cuda_dev), torch.empty(3, k // 64, dtype=torch.uint8, device=cuda_dev)
+    far(k).copy_(x)
+    ops.silu_mul_quant_mxfp4(far(k), a, b)
+    a2, b2 = torch.empty_like(a), torch.empty_like(b)
+    ops.silu_mul_quant_mxfp4(x, a2, b2)
+    assert torch.equal(a, a2) and torch.equal(b, b2)
+    assert ops.gemm_status(cuda_dev) == 0
+
+
+FIRST_CALLS = """
+import torch
+from kb_nano_b200 import moe, ops
+d = torch.device("cuda")
+torch.manual_seed(0)
+k, n = 512, 256
+xs = [torch.randn(m, k, device=d).to(torch.bfloat16) for m in (2, 300)]
+w = torch.randint(0, 256, (n, k // 2), device=d, dtype=torch.uint8)
+wsf = torch.full((ops.packed_mxfp4_bytes(n, k),), 120, dtype=torch.uint8, device=d)
+gate = torch.randn(3, 2 * k, device=d).to(torch.bfloat16)
+gate[0, :4] = -70.0
+lg = torch.randn(2, 4, device=d)
+e13, e2 = torch.randint(0, 256, (4, 256, k // 2), device=d, dtype=torch.uint8), torch.randint(0, 256, (4, k, 64), device=d, dtype=torch.uint8)
+c13, c2 = torch.full((4, 256, k // 32), 120, dtype=torch.uint8, device=d), torch.full((4, k, 4), 120, dtype=torch.uint8, device=d)
+def calls():
+    outs = []
+    for x in xs:
+        m = x.shape[0]
+        q, sf = torch.empty(m, k // 2, dtype=torch.uint8, device=d), torch.empty(ops.packed_mxfp4_bytes(m, k), dtype=torch.uint8, device=d)
+        outs.append(torch.empty(m, n, dtype=torch.bfloat16, device=d))
+        ops.mxfp4_linear(x, q, sf, w, wsf, outs[-1])
+    q, s = torch.empty(3, k // 2, dtype=torch.uint8, device=d), torch.empty(3, k // 32, dtype=torch.uint8, device=d)
+    ops.silu_mul_quant_mxfp4(gate, q, s)
+    outs += [q, s, torch.empty(3, k, dtype=torch.bfloat16, device=d)]
+    ops.dequant_mxfp4(q, s, outs[-1])
+    outs.append(moe.few_tokens_moe(xs[0], lg, e13, c13, e2, c2, 2))
+    return outs
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+for o in got:
+    o.zero_()
+g.replay()
+want = calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.isfinite(want[0]).all() and ops.gemm_status(d) == 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(cuda_dev):
+    import pathlib
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=240, cwd=pathlib.Path(__file__).parents[1])
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
