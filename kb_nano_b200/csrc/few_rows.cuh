@@ -21,7 +21,8 @@
 //              eight (MXFP4), and reads the same K-values of its token.
 //   sums       fp32; the warps' partial results meet in shared memory, where two finisher warps (one per buffer, every other
 //              unit) add them in warp order (bit-reproducible) and do what the unit's results need, so that no consumer
-//              waits for a store, a fence or another consumer.
+//              waits for a store, a fence or another consumer.  HALVES (a unit is a single stage, K <= 1024, and so belongs to
+//              eight warps): each half of the consumers has a finisher and two buffers of eight partial sums to itself.
 #pragma once
 #include "gemm_common.cuh"
 #include "mxfp4.cuh"
@@ -32,7 +33,7 @@ namespace few {
 
 enum WeightFormat : int { kFp8 = 0, kMxfp4 = 1 };
 
-constexpr int kConsumerWarps = 16, kFinishers = 2;
+constexpr int kConsumerWarps = 16, kFinishers = 2, kBuffers = 4;      // HALVES uses all four buffers, else the first two
 constexpr int kProducerWarp = kConsumerWarps, kFirstFinisher = kConsumerWarps + 1;
 constexpr int kThreads = 32 * (kConsumerWarps + 1 + kFinishers);
 constexpr int kStageBytes = 16384;                        // two boxes of 8 KB
@@ -77,8 +78,8 @@ struct Smem {
     uint8_t* scales;       // one area per stage
     uint8_t* tokens;       // f16 rows, stride token_stride
     float* token_scales;   // [rows, K / 128]: what a chunk's partial sum is multiplied by
-    float* red;            // one buffer of 16 warps x 128 partial sums (times tiles) per finisher
-    uint64_t* bars;        // full[stages], empty[stages], partials full[kFinishers], partials empty[kFinishers]
+    float* red;            // 32 x 128 partial sums (times tiles): two buffers of 16 warps or four of 8
+    uint64_t* bars;        // full[stages], empty[stages], partials full[kBuffers], partials empty[kBuffers]
     int32_t stages;
 };
 
@@ -154,14 +155,15 @@ struct RingPos {
     }
 };
 
+template <bool HALVES = false>
 __device__ __forceinline__ void init_ring(const Smem& s) {
     for (int i = 0; i < s.stages; ++i) {
         ptx::mbar_init(ptx::smem_u32(s.bars + i), 1 + 32);                    // the producer's bytes, its 32 lanes' scale copies
         ptx::mbar_init(ptx::smem_u32(s.bars + s.stages + i), kChunks);
     }
-    for (int i = 0; i < kFinishers; ++i) {
-        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + i), kConsumerWarps);
-        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + i), 1);
+    for (int i = 0; i < kBuffers; ++i) {
+        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + i), HALVES ? 8 : kConsumerWarps);
+        ptx::mbar_init(ptx::smem_u32(s.bars + 2 * s.stages + kBuffers + i), 1);
     }
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
@@ -312,13 +314,13 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
     }
 }
 
-// Consumer warp: its partial sums of the CTA's u-th unit to the finisher u % kFinishers; per tile element (row of 16) * 8 +
-// token, rows 0-7 box 0's, rows 8-15 box 1's.
-template <int TILES>
-__device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, int lane, const float (&acc)[TILES][4], const WaitCtx& w) {
-    const int buf = (int)(u % kFinishers);
-    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf), (uint32_t)(u / kFinishers & 1) ^ 1u, w);
-    float* r = s.red + (buf * kConsumerWarps + warp) * (128 * TILES);
+// Consumer warp: its partial sums of its n-th unit to a finisher; per tile element (row of 16) * 8 + token, rows 0-7 box 0's,
+// rows 8-15 box 1's.  Each buffer always has the same writers, for the reason given above.
+template <bool HALVES = false, int TILES>
+__device__ __forceinline__ void hand_over(const Smem& s, uint32_t n, int warp, int lane, const float (&acc)[TILES][4], const WaitCtx& w) {
+    const int buf = (int)(n & 1u) + (HALVES ? 2 * (warp >> 3) : 0);
+    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + kBuffers + buf), (n >> 1 & 1u) ^ 1u, w);
+    float* r = s.red + (HALVES ? buf * 8 + (warp & 7) : buf * kConsumerWarps + warp) * (128 * TILES);
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
@@ -328,23 +330,26 @@ __device__ __forceinline__ void hand_over(const Smem& s, int64_t u, int warp, in
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + buf));
 }
-// Finisher warp u % kFinishers: the sums of the CTA's u-th unit.  Lane l receives, of each tile, row l / 2, tokens 4 (l % 2) .. + 3.
-template <int TILES>
-__device__ __forceinline__ void take_over(const Smem& s, int64_t u, int lane, float (&v)[TILES][4], const WaitCtx& w) {
-    const int buf = (int)(u % kFinishers);
-    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + buf), (uint32_t)(u / kFinishers & 1), w);
-    const float4* r = reinterpret_cast<const float4*>(s.red + buf * kConsumerWarps * (128 * TILES)) + lane;
+// HALVES: whose unit is the one at this ring slot (0: warps 0-7, 1: warps 8-15).  The finishers follow the ring with a RingPos.
+__device__ __forceinline__ int half_of(const RingPos& pos) { return (int)(pos.slot & 1u); }
+// Finisher: the sums of its n-th unit.  Lane l receives, of each tile, row l / 2, tokens 4 (l % 2) .. + 3.
+template <bool HALVES = false, int TILES>
+__device__ __forceinline__ void take_over(const Smem& s, int finisher, uint32_t n, int lane, float (&v)[TILES][4], const WaitCtx& w) {
+    constexpr int kPartials = HALVES ? 8 : kConsumerWarps;
+    const int buf = HALVES ? 2 * finisher + (int)(n & 1u) : finisher;
+    wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + buf), (HALVES ? n >> 1 : n) & 1u, w);
+    const float4* r = reinterpret_cast<const float4*>(s.red + buf * kPartials * (128 * TILES)) + lane;
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
         v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < kConsumerWarps; ++j) {
+        for (int j = 0; j < kPartials; ++j) {
             const float4 p = r[(j * TILES + i) * 32];
             v[i][0] += p.x; v[i][1] += p.y; v[i][2] += p.z; v[i][3] += p.w;
         }
     }
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + kFinishers + buf));
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + kBuffers + buf));
 }
 // Row of a unit, counted over its two boxes, that lane l's value of tile i belongs to.
 template <int FMT>

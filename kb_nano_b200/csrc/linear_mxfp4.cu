@@ -122,13 +122,13 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
         for (int32_t u = u0; u < u1; ++u) {
             float acc[Fmt<kMxfp4>::kTiles][4] = {};
             consume_unit<kMxfp4>(s, pos, KC, warp, lane, columns, acc, w);
-            hand_over(s, u - u0, warp, lane, acc, w);
+            hand_over(s, (uint32_t)(u - u0), warp, lane, acc, w);
         }
     } else {
         const WaitCtx w{abort_flag, a.status, 21};
         for (int32_t u = u0 + warp - kFirstFinisher; u < u1; u += kFinishers) {
             float v[Fmt<kMxfp4>::kTiles][4];
-            take_over(s, u - u0, lane, v, w);
+            take_over(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
             const int tok0 = 4 * (lane & 1);
 #pragma unroll
             for (int tile = 0; tile < Fmt<kMxfp4>::kTiles; ++tile) {
