@@ -112,7 +112,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
     if (warp == kProducerWarp) {
         const WaitCtx w{abort_flag, a.status, 17};
         RingPos pos;
-        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, kUnitRows * u, kUnitRows * u + kUnitRows / 2, a.N, KC, lane, w);
+        for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, kUnitRows * u, kUnitRows * u + kUnitRows / 2, a.N, KC, 0, KC, lane, w);
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
         RingPos pos;

@@ -38,7 +38,7 @@ struct MoeArgs {
     const void *s13, *s2;          // weight scales
     int32_t tiled13, tiled2;       // their loads are tiled (MXFP4, K % 512 == 0)
     float* y;                      // [pairs, I]
-    float* rows;                   // [pairs, H]
+    float* rows;                   // [pairs, 2^log_parts, H]
     Jobs* jobs;
     int32_t* counters;             // one per column block of the second kernel, zeroed by the first
     __nv_bfloat16* out;
@@ -47,6 +47,7 @@ struct MoeArgs {
     int32_t* out_ids;
     int32_t* status;
     int32_t stages, token_stride, token_rows;
+    int32_t log_parts;             // second kernel: parts of K per job
 };
 
 constexpr int kMaxExperts = 32 * kRouteMaxPerLane;
@@ -189,7 +190,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * 2 * a.I + kRows * rb;
-            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s13, a.tiled13 ? &tm_scales : nullptr}, row, row + a.I, 2 * a.I * a.E, KC, lane, w);
+            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s13, a.tiled13 ? &tm_scales : nullptr}, row, row + a.I, 2 * a.I * a.E, KC, 0, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
         }
     } else if (warp < kConsumerWarps) {
@@ -239,16 +240,18 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 // COLS output columns of every token: its rows with their router weights, in slot order, by one warp.  Two columns a lane,
 // so that several tokens' rows are under way at once: this is the last thing a block does, and round trips to L2 count.
 template <int COLS>
-__device__ __forceinline__ void add_up(const MoeArgs& a, const float* weight, int rb, int lane) {
+__device__ __forceinline__ void add_up(const MoeArgs& a, int log_parts, const float* weight, int rb, int lane) {
     const int col = COLS * rb + 2 * (lane % (COLS / 2));
+    const int n = a.topk << log_parts;
     for (int t = lane / (COLS / 2); t < a.T; t += 64 / COLS) {
         float2 v = make_float2(0.f, 0.f);
-        const float2* rp = reinterpret_cast<const float2*>(a.rows + (int64_t)t * a.topk * a.H + col);
+        const float2* rp = reinterpret_cast<const float2*>(a.rows + (int64_t)t * n * a.H + col);
 #pragma unroll 8
-        for (int k = 0; k < a.topk; ++k) {
+        for (int k = 0; k < n; ++k) {
             const float2 r = __ldcg(rp + (int64_t)k * (a.H / 2));
-            v.x = fmaf(weight[t * a.topk + k], r.x, v.x);
-            v.y = fmaf(weight[t * a.topk + k], r.y, v.y);
+            const float wk = weight[t * a.topk + (k >> log_parts)];
+            v.x = fmaf(wk, r.x, v.x);
+            v.y = fmaf(wk, r.y, v.y);
         }
         __nv_bfloat16* o = a.out + (int64_t)t * a.ld_out + col;
         o[0] = __float2bfloat16_rn(v.x);
@@ -263,11 +266,13 @@ __device__ __forceinline__ int add_acq_rel_gpu(int32_t* p) {
     return old;
 }
 
-// HALVES: see few_rows.cuh.
-template <int FMT, bool HALVES>
+// kWhole: a unit is the whole K.  kHalves: a unit is a single stage, see few_rows.cuh.  kParts: K in parts.
+enum DownMode : int { kWhole, kHalves, kParts };
+template <int FMT, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_scales, const MoeArgs a) {
     extern __shared__ uint8_t raw[];
+    constexpr bool HALVES = MODE == kHalves;
     Scratch* scp;
     const Smem s = carve<FMT>(raw, a.stages, a.token_rows, a.token_stride, &scp);
     Scratch& sc = *scp;
@@ -294,37 +299,43 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
             a.out[i / a.H * a.ld_out + i % a.H] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
         return;
     }
-    const int64_t units = (int64_t)n_jobs * blocks;
+    // A job's K is worked on in parts of whole stages; vj = (job << log_parts) + part.
+    const int32_t lp = MODE == kParts ? a.log_parts : 0, n_parts = n_jobs << lp, k_stages = (KC + kChunks - 1) / kChunks;
+    auto first_chunk = [&](int32_t part) { return min(KC, (k_stages * part >> lp) * kChunks); };
+    const int64_t units = (int64_t)n_parts * blocks;
     const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+    int32_t vj = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)vj * blocks);
     if (warp == kProducerWarp) {
         const WaitCtx w{&sc.abort_flag, a.status, 10};
         RingPos pos;
         for (int64_t u = u0; u < u1; ++u) {
-            const int32_t row = sc.jobs.expert[job] * a.H + kRows * rb;
-            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + kRows / 2, a.H * a.E, KC, lane, w);
-            if (++rb == blocks) rb = 0, ++job;
+            const int32_t row = sc.jobs.expert[vj >> lp] * a.H + kRows * rb, part = vj & ((1 << lp) - 1);
+            produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + kRows / 2, a.H * a.E, KC, first_chunk(part), first_chunk(part + 1), lane, w);
+            if (++rb == blocks) rb = 0, ++vj;
         }
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{&sc.abort_flag, a.status, 11};
         RingPos pos;
-        int32_t loaded = -1;
+        int32_t loaded = -1, kc = 0;
         uint32_t handed = 0;
         TokenColumns columns{};
         for (int64_t u = u0; u < u1; ++u) {
-            const int count = sc.jobs.count[job];
-            if (job != loaded) {
+            if (vj != loaded) {
+                const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job];
+                const int32_t c0 = first_chunk(part);
+                kc = first_chunk(part + 1) - c0;
                 consumer_sync();
-                load_tokens<float, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, a.I, [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I; }, tid);
+                load_tokens<float, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, 128 * kc,
+                                                        [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I + 128 * c0; }, tid);
                 consumer_sync();
-                loaded = job;
-                columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [](int col) { return col; });
+                loaded = vj;
+                columns = token_columns(s, (uint32_t)a.token_stride, kc, count, lane, [](int col) { return col; });
             }
             float acc[Fmt<FMT>::kTiles][4] = {};
             const bool part = !HALVES || half_of(pos) == warp >> 3;
-            consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
+            consume_unit<FMT>(s, pos, kc, warp, lane, columns, acc, w);
             if (part) hand_over<HALVES>(s, handed++, warp, lane, acc, w);
-            if (++rb == blocks) rb = 0, ++job;
+            if (++rb == blocks) rb = 0, ++vj;
         }
     } else {
         const WaitCtx w{&sc.abort_flag, a.status, 20};
@@ -336,12 +347,12 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
             if ((HALVES ? half_of(pos) : (int)((u - u0) % kFinishers)) == finisher) {
                 float v[Fmt<FMT>::kTiles][4];
                 take_over<HALVES>(s, finisher, taken++, lane, v, w);
-                const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
+                const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int tile = 0; tile < Fmt<FMT>::kTiles; ++tile)
-                        if (tok0 + i < count) a.rows[(int64_t)sc.jobs.pair[job][tok0 + i] * a.H + kRows * rb + row_of_lane<FMT>(tile, lane)] = v[tile][i];
+                        if (tok0 + i < count) a.rows[(((int64_t)sc.jobs.pair[job][tok0 + i] << lp) + part) * a.H + kRows * rb + row_of_lane<FMT>(tile, lane)] = v[tile][i];
                 if (lane == pending) mine = rb;
                 ++pending;
             }
@@ -351,13 +362,13 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 __syncwarp();
                 int before = -1;
                 if (lane < pending) before = add_acq_rel_gpu(a.counters + mine);
-                unsigned last = __ballot_sync(0xffffffffu, before == n_jobs - 1);
+                unsigned last = __ballot_sync(0xffffffffu, before == n_parts - 1);
                 __syncwarp();
-                for (; last; last &= last - 1) add_up<kRows>(a, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
+                for (; last; last &= last - 1) add_up<kRows>(a, lp, sc.jobs.weight, __shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1), lane);
                 pending = 0;
             }
             if (HALVES) pos.advance((uint32_t)s.stages);      // a stage per unit
-            if (++rb == blocks) rb = 0, ++job;
+            if (++rb == blocks) rb = 0, ++vj;
         }
     }
     drain_after_abort(&sc.abort_flag);
@@ -370,16 +381,24 @@ struct Plan {
     size_t smem;
 };
 
+template <int FMT>
+static int64_t row_bytes(int64_t K) {      // of a token row with its chunk scales
+    return K * 2 + Fmt<FMT>::kTokenPad + K / 32;
+}
+template <int FMT>
+static int64_t fixed_bytes() {
+    return 1024 + kRedBytes<FMT> + scratch_bytes() + kBarBytes;
+}
+
 // As many token rows of K values (with their chunk scales), up to `want`, as leave room for a ring of at least kMinStages.
 template <int FMT>
 static bool plan(int64_t K, int want, Plan* p) {
-    const int64_t stride = K * 2 + Fmt<FMT>::kTokenPad, row = stride + K / 32, per_stage = kStageBytes + Fmt<FMT>::kScaleBytes;
-    const int64_t fixed = 1024 + kRedBytes<FMT> + scratch_bytes() + kBarBytes;
+    const int64_t row = row_bytes<FMT>(K), per_stage = kStageBytes + Fmt<FMT>::kScaleBytes, fixed = fixed_bytes<FMT>();
     for (int g = want; g >= 1; --g) {
         const int64_t left = kSmemMax - fixed - g * row;
         if (left < kMinStages * per_stage) continue;
         p->rows = g;
-        p->token_stride = (int)stride;
+        p->token_stride = (int)(row - K / 32);
         p->stages = (int)std::min<int64_t>(left / per_stage, kMaxStages);
         p->smem = (size_t)(fixed + g * row + p->stages * per_stage);
         return true;
@@ -387,17 +406,35 @@ static bool plan(int64_t K, int want, Plan* p) {
     return false;
 }
 
+// Parts of K per job of the second kernel, as a power of two, and the longest part's length.  The rows of a job's tokens
+// share the shared memory with the ring: with long rows whole, a job holds fewer tokens, and an expert with more is streamed
+// again.  So: one part if that leaves a ring beside a full job, else the fewest parts, of three stages or more, that leave a
+// ring of seven.  I 14336, 8 experts, whole / two / four parts: MXFP4, 16 tokens 319 / 260 / 223 us, 5 tokens 161.5 / 161.5 /
+// 157.5; FP8, 5 tokens 209 / 211 / 215, where the rule takes two.  Where a full job fits parts only cost: MXFP4, I 7168, 5
+// tokens 90.3 / 95.3.
+template <int FMT>
+static int log_parts(int64_t T, int64_t I, int64_t* longest) {
+    const int64_t S = (I / 128 + kChunks - 1) / kChunks;
+    for (int lp = 0;; ++lp) {
+        *longest = std::min(I, ((S + ((int64_t)1 << lp) - 1) >> lp) * kChunks * 128);
+        const int64_t ring = kSmemMax - fixed_bytes<FMT>() - std::min<int64_t>(T, kMaxGroup) * row_bytes<FMT>(*longest);
+        if (ring >= (lp == 0 ? kMinStages : 7) * (kStageBytes + Fmt<FMT>::kScaleBytes) || (S >> (lp + 1)) < 3) return lp;
+    }
+}
+
 struct WorkspaceLayout {
     int64_t jobs, counters, y, rows, total;
 };
 static WorkspaceLayout workspace_layout(int64_t T, int64_t topk, int64_t H, int64_t I) {
     WorkspaceLayout w;
+    int64_t longest;
+    const int parts = std::max(log_parts<kFp8>(T, I, &longest), log_parts<kMxfp4>(T, I, &longest));      // whichever the weights are
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     w.jobs = 0;
     w.counters = up((int64_t)sizeof(Jobs));
     w.y = w.counters + up(H / 16 * 4);
     w.rows = w.y + up(T * topk * I * 4);
-    w.total = w.rows + up(T * topk * H * 4);
+    w.total = w.rows + up((T * topk * H * 4) << parts);
     return w;
 }
 
@@ -406,11 +443,13 @@ static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& 
     // One grouping of the pairs for both kernels: as many rows as either can hold.  The first keeps all tokens if it can.
     Plan p1, p2;
     const int most = std::min(a.T, kMaxGroup);
-    KBN_REQUIRE(plan<FMT>(a.H, most, &p1) && plan<FMT>(a.I, most, &p2), KBN_ERR_UNSUPPORTED,
+    int64_t longest;
+    a.log_parts = log_parts<FMT>(a.T, a.I, &longest);
+    KBN_REQUIRE(plan<FMT>(a.H, most, &p1) && plan<FMT>(longest, most, &p2), KBN_ERR_UNSUPPORTED,
                 "kbn_moe_few_tokens: a row of %d values does not fit the shared memory", std::max(a.H, a.I));
     a.group = std::min(p1.rows, p2.rows);
     Plan all;
-    KBN_REQUIRE(plan<FMT>(a.H, a.T, &all) && plan<FMT>(a.I, a.group, &p2), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
+    KBN_REQUIRE(plan<FMT>(a.H, a.T, &all) && plan<FMT>(longest, a.group, &p2), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
     if (all.rows < a.T) plan<FMT>(a.H, a.group, &all);
     p1 = all;
     CUtensorMap t13, t2;
@@ -427,13 +466,13 @@ static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& 
     rc = gemm_status_ptr(&a.status);
     if (rc != KBN_OK) return rc;
     auto up_kernel = a.E <= 256 ? few_gate_up_kernel<FMT, 8> : few_gate_up_kernel<FMT, 32>;
-    static std::atomic<uint64_t> up_small{0}, up_large{0}, down{0}, down_halves{0};
+    static std::atomic<uint64_t> up_small{0}, up_large{0}, down{0}, down_halves{0}, down_parts{0};
     rc = allow_smem(up_kernel, a.E <= 256 ? up_small : up_large);
     if (rc != KBN_OK) return rc;
     // one token, 8 of 128 experts, H 2048, I 768: 24.6 us without halves, 23.5 with them; four tokens, I 1024: 81.3 and 80.3
     const bool halves = a.I <= 128 * kChunks;
-    auto down_kernel = halves ? few_down_kernel<FMT, true> : few_down_kernel<FMT, false>;
-    rc = allow_smem(down_kernel, halves ? down_halves : down);
+    auto down_kernel = halves ? few_down_kernel<FMT, kHalves> : (a.log_parts > 0 ? few_down_kernel<FMT, kParts> : few_down_kernel<FMT, kWhole>);
+    rc = allow_smem(down_kernel, halves ? down_halves : (a.log_parts > 0 ? down_parts : down));
     if (rc != KBN_OK) return rc;
     const unsigned grid = (unsigned)sm_count();
     a.stages = p1.stages;

@@ -309,3 +309,10 @@ def test_layers_refuse_what_the_kernels_do_not_take(cuda_dev):
     with pytest.raises(ValueError, match="at most 16"):
         wide.use_few_tokens()
     wide.use_few_tokens(0)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("t,h,i,e,top", [(16, 256, 14336, 2, 1), (5, 128, 14336, 2, 2), (16, 128, 13696, 3, 2), (9, 256, 7296, 2, 2), (16, 128, 24576, 2, 1)])
+def test_long_intermediate_rows_worked_on_in_parts(cuda_dev, fmt, t, h, i, e, top):
+    """Rows too long for a full job's tokens beside the weights' ring: the second kernel takes K in two or four parts."""
+    run_case(cuda_dev, fmt, t, h, i, e, top, seed=t + i)
