@@ -155,6 +155,25 @@ struct RingPos {
     }
 };
 
+// A consumer warp's place in the ring: its next slot (one of its half's), and how many stages ahead of the current unit's
+// first that is.
+struct OwnPos {
+    uint32_t slot, phase;
+    int32_t ahead;
+    __device__ __forceinline__ explicit OwnPos(int warp) : slot((uint32_t)warp >> 3), phase(0), ahead(warp >> 3) {}
+    __device__ __forceinline__ void advance(uint32_t stages) {      // two on, or to the first of the half's slots in the next lap
+        const uint32_t half = slot & 1u, next = slot + 2u;
+        if (next < stages) {
+            slot = next;
+            ahead += 2;
+        } else {
+            ahead += (int32_t)(stages - slot + half);
+            slot = half;
+            phase ^= 1u;
+        }
+    }
+};
+
 template <bool HALVES = false>
 __device__ __forceinline__ void init_ring(const Smem& s) {
     for (int i = 0; i < s.stages; ++i) {
@@ -227,16 +246,14 @@ __device__ __forceinline__ TokenColumns token_columns(const Smem& s, uint32_t st
 // 8-15.  A slot must always have the same readers: a warp may only test a barrier for a phase if it has seen the phase
 // before it complete, because the test tells two phases apart by their parity alone.
 template <int FMT>
-__device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_t KC, int warp, int lane, const TokenColumns& tc,
+__device__ __forceinline__ void consume_unit(const Smem& s, OwnPos& here, int32_t KC, int warp, int lane, const TokenColumns& tc,
                                              float (&acc)[Fmt<FMT>::kTiles][4], const WaitCtx& w) {
     using F = Fmt<FMT>;
     const int g = lane >> 2, t = lane & 3, cw = warp & 7;
-    for (int32_t c0 = 0; c0 < KC; c0 += kChunks) {
-        const RingPos here = pos;
-        pos.advance((uint32_t)s.stages);
-        if ((here.slot & 1u) != (uint32_t)(warp >> 3)) continue;
+    const int32_t n = (KC + kChunks - 1) / kChunks;
+    for (; here.ahead < n; here.advance((uint32_t)s.stages)) {
         wait_ring(ptx::smem_u32(s.bars + here.slot), here.phase, w);
-        const int32_t c = c0 + cw;
+        const int32_t c = here.ahead * kChunks + cw;
         if (c < KC) {
             const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * kBoxRows<FMT> + g) * F::kChunkBytes;
             const uint32_t box1 = box0 + kStageBytes / 2;
@@ -312,6 +329,7 @@ __device__ __forceinline__ void consume_unit(const Smem& s, RingPos& pos, int32_
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + s.stages + here.slot));
     }
+    here.ahead -= n;
 }
 
 // Consumer warp: its partial sums of its n-th unit to a finisher; per tile element (row of 16) * 8 + token, rows 0-7 box 0's,

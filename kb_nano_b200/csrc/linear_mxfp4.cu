@@ -115,7 +115,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
         for (int32_t u = u0; u < u1; ++u) produce_unit<kMxfp4, true>(s, pos, &tm, ScaleSource{a.sfb, nullptr}, kUnitRows * u, kUnitRows * u + kUnitRows / 2, a.N, KC, 0, KC, lane, w);
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{abort_flag, a.status, 18};
-        RingPos pos;
+        OwnPos pos(warp);
         quantise_tokens(s, a, vec != 0, tid);
         consumer_sync();
         const TokenColumns columns = token_columns(s, (uint32_t)a.token_stride, KC, a.M, lane, [](int col) { return col; });

@@ -195,7 +195,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         }
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{&sc.abort_flag, a.status, 9};
-        RingPos pos;
+        OwnPos pos(warp);
         int32_t loaded = -1;
         TokenColumns columns{};
         for (int64_t u = u0; u < u1; ++u) {
@@ -315,7 +315,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         }
     } else if (warp < kConsumerWarps) {
         const WaitCtx w{&sc.abort_flag, a.status, 11};
-        RingPos pos;
+        OwnPos pos(warp);
         int32_t loaded = -1, kc = 0;
         uint32_t handed = 0;
         TokenColumns columns{};
@@ -332,7 +332,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 columns = token_columns(s, (uint32_t)a.token_stride, kc, count, lane, [](int col) { return col; });
             }
             float acc[Fmt<FMT>::kTiles][4] = {};
-            const bool part = !HALVES || half_of(pos) == warp >> 3;
+            const bool part = !HALVES || pos.ahead == 0;      // a unit is one stage
             consume_unit<FMT>(s, pos, kc, warp, lane, columns, acc, w);
             if (part) hand_over<HALVES>(s, handed++, warp, lane, acc, w);
             if (++rb == blocks) rb = 0, ++vj;
