@@ -287,34 +287,41 @@ __device__ __forceinline__ void consume_unit(const Smem& s, OwnPos& here, int32_
             } else {
                 const uint32_t w0 = box0 + (uint32_t)(((g >> 1) & 3) << 4) + (uint32_t)t * 4u;      // 16-byte piece b of the row at w0 ^ 16 b
                 const uint32_t xa = tc.row + (uint32_t)(c * 128 + t * 8) * 2u;
-                uint32_t e[F::kTiles][2][2];      // tile, box, pair of blocks: two scales as packed bf16
+                uint32_t sw[F::kTiles][2];        // tile, box: four scale bytes
 #pragma unroll
                 for (int i = 0; i < F::kTiles; ++i)
 #pragma unroll
-                    for (int box = 0; box < 2; ++box) {
-                        const uint32_t sw = lds32(sdst + scale_word(8 * i + g, cw) + box * 512);
-                        e[i][box][0] = mxfp4::scale_bf16x2(sw);
-                        e[i][box][1] = mxfp4::scale_bf16x2(sw >> 16);
-                    }
-                float q[F::kTiles][4];
+                    for (int box = 0; box < 2; ++box) sw[i][box] = lds32(sdst + scale_word(8 * i + g, cw) + box * 512);
+                float q[F::kTiles][4] = {};
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const uint32_t at = w0 ^ (uint32_t)(16 * b);
-                    const uint4 x = lds128(xa + 64 * b);
+                for (int pair = 0; pair < 2; ++pair) {
+                    uint32_t e[F::kTiles][2];
 #pragma unroll
-                    for (int i = 0; i < F::kTiles; ++i) {
-                        uint32_t ha[4], hb[4];
-                        mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes), ha);
-                        mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes + kStageBytes / 2), hb);
-                        float p[4];
-                        mma_f16_m16n8k16_first(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
-                        mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
-                        const float s0 = b & 1 ? bf16_hi(e[i][0][b >> 1]) : bf16_lo(e[i][0][b >> 1]);
-                        const float s1 = b & 1 ? bf16_hi(e[i][1][b >> 1]) : bf16_lo(e[i][1][b >> 1]);
-                        q[i][0] = b == 0 ? p[0] * s0 : fmaf(p[0], s0, q[i][0]);
-                        q[i][1] = b == 0 ? p[1] * s0 : fmaf(p[1], s0, q[i][1]);
-                        q[i][2] = b == 0 ? p[2] * s1 : fmaf(p[2], s1, q[i][2]);
-                        q[i][3] = b == 0 ? p[3] * s1 : fmaf(p[3], s1, q[i][3]);
+                    for (int i = 0; i < F::kTiles; ++i)
+#pragma unroll
+                        for (int box = 0; box < 2; ++box) {
+                            e[i][box] = mxfp4::scale_bf16x2(sw[i][box]);
+                            sw[i][box] >>= 16;
+                        }
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t at = w0 ^ (uint32_t)(32 * pair + 16 * b);
+                        const uint4 x = lds128(xa + 64 * b + 128 * pair);
+#pragma unroll
+                        for (int i = 0; i < F::kTiles; ++i) {
+                            uint32_t ha[4], hb[4];
+                            mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes), ha);
+                            mxfp4::unpack_e2m1x8(lds32(at + i * 8 * F::kChunkBytes + kStageBytes / 2), hb);
+                            float p[4];
+                            mma_f16_m16n8k16_first(p, ha[0], hb[0], ha[1], hb[1], x.x, x.y);
+                            mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
+                            const float s0 = b & 1 ? bf16_hi(e[i][0]) : bf16_lo(e[i][0]);
+                            const float s1 = b & 1 ? bf16_hi(e[i][1]) : bf16_lo(e[i][1]);
+                            q[i][0] = fmaf(p[0], s0, q[i][0]);
+                            q[i][1] = fmaf(p[1], s0, q[i][1]);
+                            q[i][2] = fmaf(p[2], s1, q[i][2]);
+                            q[i][3] = fmaf(p[3], s1, q[i][3]);
+                        }
                     }
                 }
 #pragma unroll
