@@ -6,15 +6,28 @@
 //
 // At 4 bits the tensor cores eat 93 B/clk and SM of operands from a 128 x 256 tile on one SM, more than L2 delivers (about 64);
 // so two SMs share a 256 x 256 tile (cta_group::2): each loads its own 128 rows of A and half of the tile's 256 rows of B, 62
-// B/clk.  One K-step is 256 values (128 bytes a row): 32 KB of codes and 3 KB of scales per SM, six steps in the ring.  All
-// copies are plain tiled TMA loads into the issuing CTA's own shared memory, counted on the even CTA's barrier.
+// B/clk.  One K-step is 256 values (128 bytes a row): 32 KB of codes and 3 KB of scales per SM, five steps in the ring (seven of
+// 24 + 2 KB with 128-column tiles).  All copies are plain tiled TMA loads into the issuing CTA's own shared memory, counted on
+// the even CTA's barrier.
 //
+//   warps       loads; products; epilogue (eight); scales.  A step is four products of K = 64; its scales are copied from shared
+//               to tensor memory by a warp of their own, into columns of the step's ring slot, because the products' warp, with
+//               the copies' instructions between its own, took longer to issue a step than the tensor cores to run it
+//               (8192 x 7168 x 7168: 197 -> 153 us with the rest of this list).
 //   many tiles  persistent CTA pairs over the tiles.  The epilogue warps drain the accumulator into registers (128 columns a
 //               thread), release it, and convert and store while the next tile's products run.  (Two 256-column accumulators
-//               and the scales do not fit the 512 columns of tensor memory.)
-//   few tiles   (a few hundred rows or fewer) one tile per cluster of 2 S CTAs, whose S pairs split K.  Each pair owns 256 / S
-//               columns and receives the other pairs' partial sums of them as one bulk copy each through the cluster's shared
-//               memory; partials are added in slice order, so results are reproducible.
+//               and the scales do not fit the 512 columns of tensor memory.)  The results go through shared memory to tiled
+//               stores where the output's rows allow it, else straight to global memory.
+//   few tiles   256 x 128 tiles while every pair then has one tile at most.
+//   few tiles, long K   one 256 x 256 tile per cluster of 2 S CTAs, whose S pairs split K.  Each pair owns 256 / S columns and
+//               receives the other pairs' partial sums of them as one bulk copy each through the cluster's shared memory;
+//               partials are added in slice order, so results are reproducible.
+//
+// Measured: 8192 x 7168 x 7168 153 us, 5.5 PFLOP/s, 82 % of four times the measured bf16 rate of cuBLAS.  What is missing is
+// the drain of the accumulator between two tiles (1 to 2 us of 11.8) and the last round (896 tiles on 74 pairs: 8 in the
+// thirteenth round; a second launch with those 8 as 16 narrow tiles cost 3.5 us more than it saved).  In a loop of seconds the
+// power cap sets the clock.  512 x 4096 x 7168: 17.6 us with the quantiser (3.5) in front, against 4.5 for the products
+// alone: one tile per pair has nothing to hide its first loads, its drain and the exchange behind.
 #include <algorithm>
 
 #include "gemm_common.cuh"
@@ -73,7 +86,8 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t m, uint32_t n, uint32
 }
 // The issuing warps run their loops whole, every lane with the same values, and elect one lane inside each instruction.  With
 // one lane branched off instead, the operands cannot stay in uniform registers and each tcgen05 or TMA instruction cost its
-// issuer about 70 cycles: more, over a step, than the tensor cores need for it (8192 x 7168 x 7168: 259 -> 197 us).
+// issuer about 70 cycles: more, over a step, than the tensor cores need for it (8192 x 7168 x 7168, with the quantiser:
+// 259 -> 197 us).
 #define KBN_ELECT "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
 __device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     asm volatile(KBN_ELECT

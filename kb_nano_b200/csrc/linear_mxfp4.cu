@@ -1,10 +1,13 @@
 // The MXFP4 linear layer: bf16 rows in, quantised to MXFP4 on the way, times MXFP4 weights.
 //
 // At most eight rows (a decode step): one launch.  Every CTA quantises the rows itself -- a few thousand values, under a
-// microsecond -- into f16 rows in shared memory and streams its share of the weight rows (few_rows.cuh).  The values are
+// microsecond a row -- into f16 rows in shared memory and streams its share of the weight rows (few_rows.cuh).  The values are
 // the ones the quantiser would have stored: a code times 2^(b - b_max), b_max the largest of the scale bytes of 128 values, is
 // exact in f16 down to 2^-36 of the largest block, and the power is taken out of the 128 values' partial sum.
 // More rows, or K no multiple of 128: the quantiser and the tensor-core GEMM.
+// Measured, one row, 4096 x 7168 (15.6 MB, 2.4 us at a copy's rate): 6.3 us, against
+// 14.9 for quantiser and GEMM; 7168 x 2048, one to eight rows, 5.2 to 6.5 and 8.7 to 9.4.  Every row adds what its quantisation
+// takes in every CTA: 4096 x 7168, four rows, 9.1 us.
 #include <algorithm>
 
 #include "few_rows.cuh"
@@ -12,6 +15,10 @@
 namespace kbn {
 namespace few {
 
+// Rows that leave a shorter ring go through the GEMM.  Weight stream against quantiser and GEMM, with four stages: 8 rows,
+// 4096 x 7168 12.2 and 14.8 us, 7 rows, 16384 x 8192 24.4 and 23.3; with three: 8 rows, 4096 x 8192 14.1 and 15.5, 16384 x 8192
+// 27.5 and 22.7; with two: 8 rows, 7168 x 9216 24.0 and 17.8.
+constexpr int kLinearMinStages = 4;
 constexpr int kUnitRows = 2 * kBoxRows<kMxfp4>;
 constexpr int kLinearFixed = 1024 + kRedBytes<kMxfp4> + 256 + 128;      // alignment, partial sums, barriers, flag
 
@@ -205,7 +212,7 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
     if (M <= kMaxGroup && K % 128 == 0 && K < (1ll << 17) && N < (1ll << 27)) {
         const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad + K / 32);
         const int64_t stages = std::min<int64_t>(left / (kStageBytes + Fmt<kMxfp4>::kScaleBytes), kMaxStages);
-        if (stages >= kMinStages) return linear_few(x, ld_x, M, K, B, sfb_packed, bias, C, ldc, N, (int)stages, static_cast<cudaStream_t>(stream));
+        if (stages >= kLinearMinStages) return linear_few(x, ld_x, M, K, B, sfb_packed, bias, C, ldc, N, (int)stages, static_cast<cudaStream_t>(stream));
     }
     const int rc = kbn_quant_mxfp4(x, M, K, ld_x, a_q, K / 2, nullptr, 0, a_sf, stream);
     if (rc != KBN_OK) return rc;
