@@ -113,6 +113,22 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
     return lib
 
 
+_calls_module = None
+
+
+def calls():
+    """The native call path of the small operators (csrc/calls.cpp).  Raises if it has not been built."""
+    global _calls_module
+    if _calls_module is None:
+        load()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError(f"kb_nano_b200/_calls.so cannot be loaded ({e}): run `python -m kb_nano_b200.build`") from e
+        _calls_module = module
+    return _calls_module
+
+
 def check(code: int) -> None:
     if code != 0:
         raise KbnError(code, load().kbn_last_error().decode("utf-8", "replace"))

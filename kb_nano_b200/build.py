@@ -1,8 +1,9 @@
-"""Builds libkbn_fp8.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Builds libkbn_fp8.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _calls.so (the native call path of the
+small operators, csrc/calls.cpp, which reads torch tensors itself) with g++.
 
     python -m kb_nano_b200.build [--force] [--verbose]
 
-The library is rebuilt only when a source or header is newer than it.  nvcc cross-compiles
+Either is rebuilt only when a source or header is newer than it.  nvcc cross-compiles
 without a GPU, so this also serves as the "does it build" check on a CPU-only machine.
 """
 from __future__ import annotations
@@ -19,6 +20,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libkbn_fp8.so")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
+CALLS_SRC = os.path.join(CSRC, "calls.cpp")
+CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -59,7 +62,32 @@ def _compile_one(nvcc: str, src: str, verbose: bool) -> tuple[str, str]:
     return obj, r.stderr if verbose else ""
 
 
+def _build_calls() -> None:
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    include = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    lib = os.path.join(root, "lib")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), CALLS_SRC, "-o", CALLS_PATH,
+           f"-L{PKG_DIR}", "-l:" + os.path.basename(LIB_PATH), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {CALLS_SRC}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    _build_lib(force, verbose)
+    if force or not os.path.exists(CALLS_PATH) or any(os.path.getmtime(f) > os.path.getmtime(CALLS_PATH) for f in (CALLS_SRC, os.path.join(INCLUDE, "kbn_fp8.h"))):
+        _build_calls()
+    return LIB_PATH
+
+
+def _build_lib(force: bool, verbose: bool) -> str:
     if not force and not needs_build():
         return LIB_PATH
     nvcc = _nvcc()

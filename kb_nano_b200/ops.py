@@ -642,7 +642,11 @@ def requant_weights_ue8m0(w_fp8: torch.Tensor, scale: torch.Tensor, eps: float =
 
 # ---- MXFP4: blocks of 32 along K, e2m1 codes (two per byte, even element in the low nibble), E8M0 scale bytes --------
 
+# Each of the calls below goes through csrc/calls.cpp first, which accepts what is right in a fraction of the time the checks
+# here take.  What it does not accept comes back, and the checks here say why.
+
 MX_BLOCK = 32
+_calls = _lib.calls
 _CODE_DTYPES = (torch.uint8, torch.float4_e2m1fn_x2)
 _BYTE_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
 
@@ -735,12 +739,16 @@ def quant_mxfp4(x: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor 
     """x bf16 [M,K] -> MXFP4: out_fp4 uint8 [M,K/2] and the E8M0 scales of its blocks of 32, row-major in out_scale uint8
     [M,K/32] and / or in the packed form of mxfp4_gemm_nt in packed_sf (uint8, packed_mxfp4_bytes(M, K) bytes).  The scale is
     the smallest power of two that clips nothing; a block with an infinity or a NaN becomes NaN."""
+    if _calls().quant_mxfp4(x, out_fp4, out_scale, packed_sf):
+        return
     m, k, ld = _bf16_rows(x, "x")
     _quant_mxfp4_call(_lib.load().kbn_quant_mxfp4, x, m, k, ld, out_fp4, out_scale, packed_sf)
 
 
 def silu_mul_quant_mxfp4(inp: torch.Tensor, out_fp4: torch.Tensor, out_scale: torch.Tensor | None = None, packed_sf: torch.Tensor | None = None) -> None:
     """inp bf16 [M, 2*N2] (gate | up) -> bf16(bf16(silu(gate)) * up) in MXFP4, [M, N2]; outputs as in quant_mxfp4."""
+    if _calls().silu_mul_quant_mxfp4(inp, out_fp4, out_scale, packed_sf):
+        return
     m, n, ld = _bf16_rows(inp, "inp")
     if n % 2:
         raise ValueError(f"inp must hold gate and up halves, got {n} columns")
@@ -749,6 +757,8 @@ def silu_mul_quant_mxfp4(inp: torch.Tensor, out_fp4: torch.Tensor, out_scale: to
 
 def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
     """MXFP4 codes [M,K/2] with row-major scales [M,K/32] -> out bf16 [M,K] (exact within bf16's range)."""
+    if _calls().dequant_mxfp4(q, scale, out):
+        return
     m, k, ld = _bf16_rows(out, "out")
     if k % MX_BLOCK:
         raise ValueError(f"out must have a multiple of {MX_BLOCK} columns, got {k}")
@@ -789,6 +799,8 @@ def mxfp4_gemm_nt(a_q: torch.Tensor, a_sf: torch.Tensor, b_q: torch.Tensor, b_sf
                   bias: torch.Tensor | None = None) -> None:
     """out bf16 [M,N] = MXFP4 a_q [M,K/2] times MXFP4 b_q [N,K/2], transposed (+ bias, in fp32, before the rounding).  a_sf and
     b_sf are the packed scales (quant_mxfp4's packed_sf, pack_mxfp4_scales)."""
+    if _calls().mxfp4_gemm_nt(a_q, a_sf, b_q, b_sf, out, bias):
+        return
     if a_q.dim() != 2 or b_q.dim() != 2 or a_q.size(1) != b_q.size(1) or a_q.size(1) % 16:
         raise ValueError(f"a_q and b_q must be [M, K/2] and [N, K/2] with K a multiple of {MX_BLOCK}, got {tuple(a_q.shape)} and {tuple(b_q.shape)}")
     m, n, k = a_q.size(0), b_q.size(0), a_q.size(1) * 2
@@ -804,6 +816,8 @@ def mxfp4_linear(x: torch.Tensor, a_q: torch.Tensor, a_sf: torch.Tensor, b_q: to
     [M,N], which must not share memory with x.  a_q uint8 [M,K/2] and a_sf (packed_mxfp4_bytes(M, K) bytes) are scratch for the
     quantised rows (calls that may overlap in time need their own); up to eight rows, K a multiple of 128, are quantised inside
     the one kernel that multiplies them and leave the scratch untouched."""
+    if _calls().mxfp4_linear(x, a_q, a_sf, b_q, b_sf, out, bias):
+        return
     m, k, ld_x = _bf16_rows(x, "x")
     if k % MX_BLOCK or k == 0:
         raise ValueError(f"x must have a multiple of {MX_BLOCK} columns, got {k}")

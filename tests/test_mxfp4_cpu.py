@@ -110,3 +110,18 @@ def test_reference_routing_by_hand():
     assert ids.tolist() == [[2, 0, 1]] and abs(w.sum().item() - 1) < 1e-12
     w, ids = ref.route(torch.tensor([[5.0, -9.0, 1.0, 1.5]]), 1, "sigmoid", torch.zeros(4), n_group=2, topk_group=1)
     assert ids.tolist() == [[3]]                                      # 1 + 2 of group two beat 5 and -9: sums of the two best
+
+
+def test_native_calls_accept_nothing_that_is_not_a_cuda_tensor(kbn_lib):
+    """The native call path answers False, without an exception, for what it does not know; the Python checks then say why."""
+    from kb_nano_b200 import _lib
+    calls = _lib.calls()
+    x, q, s, p = torch.zeros(2, 128, dtype=torch.bfloat16), torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 4, dtype=torch.uint8), torch.zeros(1 << 12, dtype=torch.uint8)
+    out = torch.zeros(2, 2, dtype=torch.bfloat16)
+    for fn, args in ((calls.quant_mxfp4, (x, q, s, None)), (calls.silu_mul_quant_mxfp4, (torch.zeros(2, 256, dtype=torch.bfloat16), q, s, p)),
+                     (calls.dequant_mxfp4, (q, s, x)), (calls.mxfp4_gemm_nt, (q, p, q, p, out, None)), (calls.mxfp4_linear, (x, q, p, q, p, out, None))):
+        assert fn(*args) is False
+        for i in range(len(args)):
+            for bad in (None, 3, "x", object(), torch.Tensor, torch.zeros(2, 128, device="meta"), torch.zeros(()), torch.eye(2).to_sparse()):
+                assert fn(*args[:i], bad, *args[i + 1:]) is False
+        assert fn() is False and fn(*args, None) is False and fn(*args[:-1]) is False

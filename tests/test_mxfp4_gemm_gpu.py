@@ -332,3 +332,61 @@ def test_first_calls_of_a_process_inside_a_capture(cuda_dev):
     import sys
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=240, cwd=pathlib.Path(__file__).parents[1])
     assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_native_calls_accept_what_the_checks_accept(cuda_dev):
+    """The native call path takes every well-formed call (whole, strided, on another stream) and turns down one wrong argument at a
+    time, whatever it is; the public functions then raise."""
+    from kb_nano_b200 import _lib, ops
+    calls = _lib.calls()
+    m, n, k = 3, 40, 256
+    gen = torch.Generator(device=cuda_dev).manual_seed(80)
+    wide = torch.randn(m, 2 * k + 6, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    x, gu = wide[:, 2:2 + k], wide[:, 4:4 + 2 * k]
+    q, s = torch.empty(m, k // 2 + 8, dtype=torch.uint8, device=cuda_dev)[:, :k // 2], torch.empty(m, k // 32 + 3, dtype=torch.uint8, device=cuda_dev)[:, :k // 32]
+    p = torch.empty(ops.packed_mxfp4_bytes(m, k), dtype=torch.uint8, device=cuda_dev)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bp, bias = ops.pack_mxfp4_scales(bsc, k), torch.randn(n, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    dq, out, back = torch.empty(m, k // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(m, n + 8, dtype=torch.bfloat16, device=cuda_dev)[:, :n], torch.empty_like(x)
+    good = [(calls.quant_mxfp4, ops.quant_mxfp4, (x, q, s, p)), (calls.quant_mxfp4, ops.quant_mxfp4, (x, q, None, p)), (calls.quant_mxfp4, ops.quant_mxfp4, (x, dq, s, None)),
+            (calls.silu_mul_quant_mxfp4, ops.silu_mul_quant_mxfp4, (gu, q, s, p)), (calls.dequant_mxfp4, ops.dequant_mxfp4, (q, s, back)),
+            (calls.mxfp4_gemm_nt, ops.mxfp4_gemm_nt, (dq, p, bq, bp, out, bias)), (calls.mxfp4_linear, ops.mxfp4_linear, (x, dq, p, bq, bp, out, bias)),
+            (calls.mxfp4_linear, ops.mxfp4_linear, (x, dq, p, bq, bp, out, None))]
+    before = _lib.launch_count()
+    for native, public, args in good:
+        assert native(*args) is True
+        with torch.cuda.stream(torch.cuda.Stream()):
+            assert native(*args) is True
+        torch.cuda.synchronize()
+    assert _lib.launch_count() >= before + 2 * len(good)
+    for native, public, args in good:
+        for i, a in enumerate(args):
+            if a is None:
+                continue
+            bads = [a.cpu(), a.float(), a[:0], a.t() if a.dim() == 2 else a[: a.numel() - 1], a.double()]
+            for bad in bads:
+                wrong = (*args[:i], bad, *args[i + 1:])
+                if bad.numel() == 0 and i == 0:
+                    continue                                      # no rows: nothing to do, not an error
+                assert native(*wrong) is False, (native, i, bad.shape, bad.dtype)
+                with pytest.raises((ValueError, RuntimeError)):
+                    public(*wrong)
+    assert ops.gemm_status(cuda_dev) == 0
+
+
+def test_native_calls_run_on_the_current_stream(cuda_dev):
+    """A call inside a stream context is ordered with that stream's work: a long fill before it, a copy behind it."""
+    from kb_nano_b200 import ops
+    x, y = torch.zeros(4096, 8192, dtype=torch.bfloat16, device=cuda_dev), torch.full((4096, 8192), 3.0, dtype=torch.bfloat16, device=cuda_dev)
+    q, s = torch.zeros(4096, 4096, dtype=torch.uint8, device=cuda_dev), torch.zeros(4096, 256, dtype=torch.uint8, device=cuda_dev)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(50):
+            x.copy_(y)
+            x.mul_(2.0)
+        ops.quant_mxfp4(x, q, s)
+        got = q.clone(), s.clone()
+    stream.synchronize()
+    want = ref.quant(torch.full((1, 32), 6.0))
+    assert (got[0] == int(want[0][0, 0])).all() and (got[1] == int(want[1][0, 0])).all()
