@@ -214,7 +214,7 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
         const int64_t stages = std::min<int64_t>(left / (kStageBytes + Fmt<kMxfp4>::kScaleBytes), kMaxStages);
         if (stages >= kLinearMinStages) return linear_few(x, ld_x, M, K, B, sfb_packed, bias, C, ldc, N, (int)stages, static_cast<cudaStream_t>(stream));
     }
-    const int rc = kbn_quant_mxfp4(x, M, K, ld_x, a_q, K / 2, nullptr, 0, a_sf, stream);
+    const int rc = mxfp4::quantise(x, M, K, ld_x, a_q, K / 2, nullptr, 0, a_sf, true, static_cast<cudaStream_t>(stream));
     if (rc != KBN_OK) return rc;
     return kbn_mxfp4_gemm_nt(a_q, a_sf, B, sfb_packed, bias, C, ldc, M, N, K, stream);
 }

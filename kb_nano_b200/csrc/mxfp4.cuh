@@ -91,6 +91,9 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t w, uint32_t (&h)[4]) {
         : "r"(w));
 }
 
+// kbn_quant_mxfp4 (mxfp4_quant.cu).  behind_gemm: the calls come in a row with GEMMs.
+int quantise(const void* x, int64_t M, int64_t K, int64_t ld_x, void* q, int64_t ld_q, void* scale, int64_t s_row, void* sf_packed, bool behind_gemm, cudaStream_t st);
+
 // Position of a row's scale word for 128-K block kb in the packed layout the tensor core reads: per 128 rows and 128 of K
 // 128 words, word (l, i) <-> row 32 i + l; the word's four bytes are the scales of the block's four 32-value groups.
 __host__ __device__ __forceinline__ size_t packed_word(int64_t row, int64_t kb, int64_t kblocks) {
