@@ -19,6 +19,8 @@ namespace mxfp4 {
 // of them ends, and the kernel behind them in its turn.  It is let in only after the wait: a kernel that reads its weights
 // before its own wait then still finds what was written two kernels ahead of it.  Calls in a row, against plain launches: quantise
 // and back 8192 x 7168 52.2 -> 48.4 us, 1 x 7168 6.7 -> 5.7; SiLU*up, quantise and back 129 x 2048 8.2 -> 6.2.
+// What they read may be written while they are already resident: their pointers are not __restrict__ and no load takes the
+// read-only path, which the wait does not hold back.
 __device__ __forceinline__ void begin_kernel() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -41,9 +43,10 @@ struct Vec16 {             // 16 bf16 values
 };
 __device__ __forceinline__ Vec16 load16(const void* p) {       // 32-byte aligned, read once
     Vec16 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
-                 : "l"(p));
+                 : "l"(p)
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ void store16(void* p, const Vec16& v) {
@@ -124,7 +127,7 @@ __device__ __forceinline__ void store_scales(const uint32_t (&word)[U], bool val
 // U groups of 128 per team, all loads issued before the first use.
 template <int ALIGN, int U>
 __global__ void __launch_bounds__(256)
-quant_mxfp4_kernel(const __nv_bfloat16* __restrict__ x, uint32_t K, int64_t ld_x, QuantOut o, uint32_t G, uint32_t chunks_per_row, uint32_t n_chunks) {
+quant_mxfp4_kernel(const __nv_bfloat16* x, uint32_t K, int64_t ld_x, QuantOut o, uint32_t G, uint32_t chunks_per_row, uint32_t n_chunks) {
     begin_kernel();
     const uint32_t j = threadIdx.x & 7u;
     const uint32_t chunk = blockIdx.x * 32u + (threadIdx.x >> 3);
@@ -167,8 +170,8 @@ __device__ __forceinline__ void silu_mul_exact8(const uint32_t* g, const uint32_
 // The two roundings to bf16 are those of an unfused activation in the model's type, so that fused and unfused layers agree.
 template <int ALIGN, int U>
 __global__ void __launch_bounds__(256)
-silu_mul_quant_mxfp4_kernel(const __nv_bfloat16* __restrict__ in, uint32_t N2, int64_t ld_in, QuantOut o, uint32_t G, uint32_t chunks_per_row,
-                            uint32_t n_chunks, const uint16_t* __restrict__ table) {
+silu_mul_quant_mxfp4_kernel(const __nv_bfloat16* in, uint32_t N2, int64_t ld_in, QuantOut o, uint32_t G, uint32_t chunks_per_row,
+                            uint32_t n_chunks, const uint16_t* table) {
     begin_kernel();
     const uint32_t j = threadIdx.x & 7u;
     const uint32_t chunk = blockIdx.x * 32u + (threadIdx.x >> 3);
@@ -203,8 +206,8 @@ silu_mul_quant_mxfp4_kernel(const __nv_bfloat16* __restrict__ in, uint32_t N2, i
 // leaves bf16's range (6 * 2^126 and above becomes infinity).  FLAT: everything is contiguous, rows do not matter.
 template <bool FLAT, bool VEC, int U>
 __global__ void __launch_bounds__(256)
-dequant_mxfp4_kernel(const uint8_t* __restrict__ q, int64_t ld_q, const uint8_t* __restrict__ scale, int64_t s_row, uint32_t vecs_per_row, uint32_t n_vecs,
-                     __nv_bfloat16* __restrict__ out, int64_t ld_out) {
+dequant_mxfp4_kernel(const uint8_t* q, int64_t ld_q, const uint8_t* scale, int64_t s_row, uint32_t vecs_per_row, uint32_t n_vecs,
+                     __nv_bfloat16* out, int64_t ld_out) {
     begin_kernel();
     uint32_t w[U][2], sb[U];
 #pragma unroll

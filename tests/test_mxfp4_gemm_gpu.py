@@ -390,3 +390,36 @@ def test_native_calls_run_on_the_current_stream(cuda_dev):
     stream.synchronize()
     want = ref.quant(torch.full((1, 32), 6.0))
     assert (got[0] == int(want[0][0, 0])).all() and (got[1] == int(want[1][0, 0])).all()
+
+
+@pytest.mark.parametrize("m", [1, 8, 77, 600])
+def test_a_chain_of_launches_equals_the_same_calls_one_by_one(cuda_dev, m):
+    """Kernels are let in while the one before them ends.  Thirty rounds over the same buffers, each input the last call's output
+    (clamped, since gate * up squares it): the same bits as with a synchronisation after every call."""
+    from kb_nano_b200 import ops
+    k, n = 512, 1024
+    gen = torch.Generator(device=cuda_dev).manual_seed(90 + m)
+    bq, bsc = operand(n, k, gen, cuda_dev, 2)
+    bsf = ops.pack_mxfp4_scales((bsc - 4), k)
+    start = torch.randn(m, k, generator=gen, device=cuda_dev).to(torch.bfloat16)
+
+    def chain(wait):
+        x, q, s = start.clone(), torch.empty(m, k // 2, dtype=torch.uint8, device=cuda_dev), torch.empty(m, k // 32, dtype=torch.uint8, device=cuda_dev)
+        aq, asf = torch.empty_like(q), torch.empty(ops.packed_mxfp4_bytes(m, k), dtype=torch.uint8, device=cuda_dev)
+        y, seen = torch.empty(m, n, dtype=torch.bfloat16, device=cuda_dev), []
+        torch.cuda.synchronize()
+        for i in range(30):
+            for f in (lambda: ops.mxfp4_linear(x, aq, asf, bq, bsf, y), lambda: ops.silu_mul_quant_mxfp4(y, q, s), lambda: ops.dequant_mxfp4(q, s, x),
+                      lambda: x.clamp_(-1, 1).add_(start), lambda: ops.quant_mxfp4(x, q, s), lambda: ops.dequant_mxfp4(q, s, x)):
+                f()
+                if wait:
+                    torch.cuda.synchronize()
+            seen.append((x.clone(), q.clone(), s.clone()))
+        torch.cuda.synchronize()
+        return seen
+
+    want = chain(True)
+    assert all(torch.isfinite(a[0]).all() for a in want) and not torch.equal(want[0][0], want[-1][0])
+    for _ in range(5):
+        got = chain(False)
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
