@@ -157,6 +157,11 @@ def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13
     The activations are not quantised (with a few tokens that saves no bytes), so results differ from fused_experts_fp8 by
     that pipeline's FP8 rounding of its activations.  Scratch comes from the caching allocator with every call: calls on
     several streams, and captured graphs, do not share any."""
+    done = _lib.calls().few_tokens_moe(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, scoring, bias, n_group, topk_group, renormalize,
+                                       renorm_floor, scale, round_bf16, out, out_w, out_ids)
+    if done is not False:
+        return done
+    # not accepted there: the checks below say why (or accept a call with arguments of unusual types)
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"unsupported scoring function {scoring!r}")
     if hidden_states.dim() != 2 or hidden_states.dtype != torch.bfloat16 or hidden_states.stride(1) != 1:

@@ -316,3 +316,34 @@ def test_layers_refuse_what_the_kernels_do_not_take(cuda_dev):
 def test_long_intermediate_rows_worked_on_in_parts(cuda_dev, fmt, t, h, i, e, top):
     """Rows too long for a full job's tokens beside the weights' ring: the second kernel takes K in two or four parts."""
     run_case(cuda_dev, fmt, t, h, i, e, top, seed=t + i)
+
+
+def test_native_call_accepts_what_the_checks_accept(cuda_dev):
+    """The native call path takes a well-formed call of either format (every optional argument given or not) and answers False to one
+    wrong argument at a time, whatever it is; the public function then raises, or does what it did before for an odd type."""
+    from kb_nano_b200 import _lib, moe, ops
+    native = _lib.calls().few_tokens_moe
+    for fmt in ("fp8", "mxfp4"):
+        w13, s13, w2, s2, _, _ = experts(fmt, 8, 256, 128, cuda_dev, 34)
+        x, lg, bias = torch.randn(3, 256, device=cuda_dev).to(torch.bfloat16), torch.randn(3, 8, device=cuda_dev), torch.randn(8, device=cuda_dev) * 0.1
+        out, ow, oi = torch.empty_like(x), torch.empty(3, 2, device=cuda_dev), torch.empty(3, 2, dtype=torch.int32, device=cuda_dev)
+        full = (x, lg, w13, s13, w2, s2, 2, "sigmoid", bias, 2, 1, True, 0.0, 1.0, False, out, ow, oi)
+        plain = (x, lg.to(torch.bfloat16), w13, s13, w2, s2, 2, "softmax", None, 1, 1, False, 0.0, 2.5, True, None, None, None)
+        assert native(*full) is out
+        fresh = native(*plain)
+        assert fresh.shape == x.shape and fresh.dtype == x.dtype and fresh.is_contiguous()
+        assert torch.equal(fresh, moe.few_tokens_moe(*plain))
+        for i, a in enumerate(full):
+            if isinstance(a, torch.Tensor):
+                bads = [a.cpu(), a.double(), a[:0], a[..., :-1], 3, None if i in (0, 1, 2, 3, 4, 5) else "x"]
+            else:
+                bads = {6: [0, 9, 17, "2", None], 7: ["tanh", 1, None], 9: [3, 0, None], 10: [3, 0, None], 11: [None], 12: [None], 13: [None], 14: [None]}[i]
+            for bad in bads:
+                args = (*full[:i], bad, *full[i + 1:])
+                assert native(*args) is False, (fmt, i, bad)
+                if isinstance(bad, torch.Tensor) and bad.numel() or i in (6, 7, 9, 10) and isinstance(bad, int):
+                    with pytest.raises((ValueError, RuntimeError, TypeError)):
+                        moe.few_tokens_moe(*args)
+        assert torch.equal(moe.few_tokens_moe(*full[:13], 1, *full[14:]), native(*full))      # an int factor: through the checks
+        assert native() is False and native(*full[:-1]) is False
+    assert ops.gemm_status(cuda_dev) == 0
