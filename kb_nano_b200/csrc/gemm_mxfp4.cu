@@ -26,8 +26,8 @@
 // Measured: 8192 x 7168 x 7168 153 us, 5.5 PFLOP/s, 82 % of four times the measured bf16 rate of cuBLAS.  What is missing is
 // the drain of the accumulator between two tiles (1 to 2 us of 11.8) and the last round (896 tiles on 74 pairs: 8 in the
 // thirteenth round; a second launch with those 8 as 16 narrow tiles cost 3.5 us more than it saved).  In a loop of seconds the
-// power cap sets the clock.  512 x 4096 x 7168: 17.6 us with the quantiser (3.5) in front, against 4.5 for the products
-// alone: one tile per pair has nothing to hide its first loads, its drain and the exchange behind.
+// power cap sets the clock.  512 x 4096 x 7168: 17.1 us with the quantiser (3.2) in front, against 4.5 for the products
+// alone: one tile per pair has nothing to hide its first loads and its drain behind.
 #include <algorithm>
 
 #include "gemm_common.cuh"
@@ -44,7 +44,7 @@ constexpr int kScaleWarp = 2 + kEpiWarps;                      // warps: loads, 
 constexpr int kGemmThreads = 32 * (kScaleWarp + 1);
 constexpr int kStagingBytes = kEpiWarps * 32 * 128;            // 32 rows x 64 bf16 columns per epilogue warp
 constexpr int kTmemColumns = 512, kColScales = 256;            // accumulators in columns 0-255, scales behind them
-constexpr int kSplitGain = 14;                                 // K-steps a split over the cluster has to save
+constexpr int kSplitGain = 18;                                 // K-steps a split over the cluster has to save
 constexpr int kGroupM = 8;                                     // tile rows that run side by side, for reuse of B in L2
 
 // BN: tile columns, 256 or 128.
@@ -634,9 +634,9 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const vo
     p.tiled_out = aligned16(C) && p.ldc % 8 == 0;
     const int64_t wide = p.m_tiles * ((N + 255) / 256), narrow = p.m_tiles * ((N + 127) / 128);
     // Few tiles: K split over the cluster, the most slices that are resident at once and leave each a step.  The exchange of
-    // partial sums takes as long as a dozen steps, so a split has to save more: measured with the quantiser, 64 x 4096 x 7168
-    // (28 steps, S = 4) 15.5 us split and 16.5 not, 512 x 4096 x 7168 (S = 2) 18.5 and 18.6, 77 x 2056 x 1440 (6 steps) 11.4
-    // and 8.6.
+    // partial sums takes as long as 18 steps, so a split has to save as many: measured with the quantiser, split and not:
+    // 512 x 4096 x 7168 (S = 2 saves 14 of 28 steps) 17.6 and 17.1 us, x 9216 (18 of 36) 20.3 and 20.2, x 12288 (24 of 48) 23.3
+    // and 24.4; 64 x 4096 x 7168 (S = 4, 21 of 28) 13.4 and 13.6, 64 x 2048 x 16384 (48 of 64) 17.1 and 23.7.
     p.n_tiles = (int32_t)((N + 255) / 256);
     for (int S = 4; S >= 2; S /= 2) {
         const int per = (p.steps + S - 1) / S;

@@ -423,3 +423,23 @@ def test_a_chain_of_launches_equals_the_same_calls_one_by_one(cuda_dev, m):
     for _ in range(5):
         got = chain(False)
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 2600, 9216), (512, 4608, 9280), (257, 2561, 9984), (77, 2056, 12320), (1, 1000, 16384), (40, 8, 14336)])
+def test_gemm_with_k_split_over_a_cluster(cuda_dev, m, n, k):
+    """Few tiles and long K, two and four slices, whole boxes and ragged edges."""
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(m + n + k)
+    aq, asc = operand(m, k, gen, cuda_dev)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bias = torch.randn(n, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    asf, bsf = ops.pack_mxfp4_scales(asc, k), ops.pack_mxfp4_scales(bsc, k)
+    a, b = ref.values(aq, asc), ref.values(bq, bsc)
+    for bb in (None, bias):
+        out, again = torch.full((m, n + 8), 7.0, dtype=torch.bfloat16, device=cuda_dev), torch.empty(m, n, dtype=torch.bfloat16, device=cuda_dev)
+        ops.mxfp4_gemm_nt(aq, asf, bq, bsf, out[:, :n], bb)
+        check(out[:, :n], a, b, bb)
+        assert (out[:, n:] == 7).all()
+        ops.mxfp4_gemm_nt(aq, asf, bq, bsf, again, bb)
+        assert torch.equal(out[:, :n], again)
+    assert ops.gemm_status(cuda_dev) == 0
