@@ -70,7 +70,10 @@ public:
         stream_ = c10::cuda::getCurrentCUDAStream(index_).stream();
     }
     ~Launch() {
-        if (ok_ && before_ != index_) c10::cuda::set_device(before_);
+        try {
+            if (ok_ && before_ != index_) c10::cuda::set_device(before_);
+        } catch (...) {      // the call's own result stands
+        }
     }
     Launch(const Launch&) = delete;
     Launch& operator=(const Launch&) = delete;
