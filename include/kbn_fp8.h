@@ -340,7 +340,7 @@ int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t K, void* a_
  * in fp32 in slot order, tokens and activated rows rounded to 11 bits beside a power of two per 128 values.  A NaN logit
  * makes all of a softmax router's scores NaN, and only its own expert's score of a sigmoid router; a NaN score is never
  * chosen.  A token without a single choice gets ids -1 and a row of NaNs.  out may be x.  workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents
- * irrelevant; calls that may overlap need one each.  KBN_ERR_UNSUPPORTED when a row of max(H, I) values does not fit the
+ * irrelevant; calls that may overlap need one each.  KBN_ERR_UNSUPPORTED when a row of H values does not fit the
  * shared memory of an SM (about 55,000).  Waits inside are bounded and report through kbn_gemm_status.
  */
 int64_t kbn_moe_few_tokens_workspace_bytes(int64_t T, int64_t topk, int64_t H, int64_t I);

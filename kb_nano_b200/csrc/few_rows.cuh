@@ -194,8 +194,9 @@ __device__ __forceinline__ void init_ring(const Smem& s) {
     ptx::fence_proxy_async();
 }
 
-// Producer warp: all stages of one unit's chunks c_begin (a multiple of kChunks) .. c_end - 1 (up to a multiple, or KC).  row_a, row_b: first rows of the two boxes (in rows of the tensor map; a box past
-// the last row is filled with zeros by the TMA).  n_rows: rows the scale array covers.
+// Producer warp: all stages of one unit's chunks c_begin (a multiple of kChunks) .. c_end - 1 (up to a multiple, or KC).
+// row_a, row_b: first rows of the two boxes (in rows of the tensor map; a box past the last row is filled with zeros by the
+// TMA).  n_rows: rows the scale array covers.
 template <int FMT, bool PACKED = false>
 __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const void* tmap, const ScaleSource& sc, int32_t row_a, int32_t row_b,
                                              int32_t n_rows, int32_t KC, int32_t c_begin, int32_t c_end, int lane, const WaitCtx& w) {

@@ -347,3 +347,9 @@ def test_native_call_accepts_what_the_checks_accept(cuda_dev):
         assert torch.equal(moe.few_tokens_moe(*full[:13], 1, *full[14:]), native(*full))      # an int factor: through the checks
         assert native() is False and native(*full[:-1]) is False
     assert ops.gemm_status(cuda_dev) == 0
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("t,i", [(1, 65536), (3, 102400), (16, 32896)])
+def test_intermediate_rows_longer_than_shared_memory(cuda_dev, fmt, t, i):
+    run_case(cuda_dev, fmt, t, 128, i, 1, 1, seed=t + i)

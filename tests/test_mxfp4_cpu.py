@@ -125,3 +125,8 @@ def test_native_calls_accept_nothing_that_is_not_a_cuda_tensor(kbn_lib):
             for bad in (None, 3, "x", object(), torch.Tensor, torch.zeros(2, 128, device="meta"), torch.zeros(()), torch.eye(2).to_sparse()):
                 assert fn(*args[:i], bad, *args[i + 1:]) is False
         assert fn() is False and fn(*args, None) is False and fn(*args[:-1]) is False
+
+
+def test_moe_refuses_token_rows_longer_than_shared_memory(kbn_lib):
+    for fmt in (0, 1):
+        refused(kbn_lib, kbn_lib.kbn_moe_few_tokens(*moe_args(H=131072, ld_x=131072, ld_out=131072, fmt=fmt, wb=1 << 40)), "shared memory")
