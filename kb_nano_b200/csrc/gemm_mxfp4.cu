@@ -25,7 +25,7 @@
 //
 // Measured: 8192 x 7168 x 7168 153 us, 5.5 PFLOP/s, 82 % of four times the measured bf16 rate of cuBLAS.  What is missing is
 // the drain of the accumulator between two tiles (1 to 2 us of 11.8) and the last round (896 tiles on 74 pairs: 8 in the
-// thirteenth round; a second launch with those 8 as 16 narrow tiles cost 3.5 us more than it saved).  In a loop of seconds the
+// thirteenth round, which run as 16 halves).  In a loop of seconds the
 // power cap sets the clock.  512 x 4096 x 7168: 17.1 us with the quantiser (3.2) in front, against 4.5 for the products
 // alone: one tile per pair has nothing to hide its first loads and its drain behind.
 #include <algorithm>
@@ -71,6 +71,7 @@ struct GemmArgs {
     int32_t* status;
     int32_t M, N, kblocks, steps;      // kblocks: 128-K blocks (scales), steps: 256-K steps
     int32_t m_tiles, n_tiles, S;
+    int32_t whole;                     // tiles from this one on are worked on as two halves of 128 columns each
     int32_t tiled_out;                 // the output's rows allow tiled stores
 };
 
@@ -137,7 +138,13 @@ __device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) 
     return ok != 0;
 }
 
-__device__ __forceinline__ void tile_of(int32_t t, const GemmArgs& p, int32_t& m_tile, int32_t& n_tile) {
+// `half`: 0 or 1 of a halved tile, -1 of a whole one.
+__device__ __forceinline__ void tile_of(int32_t t, const GemmArgs& p, int32_t& m_tile, int32_t& n_tile, int32_t& half) {
+    half = -1;
+    if (t >= p.whole) {
+        half = (t - p.whole) & 1;
+        t = p.whole + ((t - p.whole) >> 1);
+    }
     const int32_t per_group = kGroupM * p.n_tiles;
     const int32_t grp = t / per_group, first = grp * kGroupM;
     const int32_t size = min(kGroupM, p.m_tiles - first);
@@ -195,7 +202,7 @@ __device__ __forceinline__ void stage_row(const float (&f)[32], uint32_t staging
 template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSfa,
-                  const __grid_constant__ CUtensorMap tmSfb, const __grid_constant__ CUtensorMap tmC, const GemmArgs p) {
+                  const __grid_constant__ CUtensorMap tmSfb, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmBh, const GemmArgs p) {
     using F = Cfg<BN>;
     constexpr int kStages = F::kStages, kOperandBytes = F::kOperandBytes, kSfBytes = F::kSfBytes;
     extern __shared__ uint8_t raw[];
@@ -249,7 +256,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     ptx::grid_dependency_wait();
     ptx::launch_dependents();
 
-    const int32_t tiles = p.m_tiles * p.n_tiles;
+    const int32_t tiles = 2 * p.m_tiles * p.n_tiles - p.whole;      // halves count for themselves
     const int32_t cluster = (int32_t)(blockIdx.x / (SPLIT ? 2u * (uint32_t)p.S : 2u));
     const int32_t stride = SPLIT ? tiles : (int32_t)(gridDim.x / 2);          // split: one tile per cluster
     const int32_t per_slice = SPLIT ? (p.steps + p.S - 1) / p.S : p.steps;
@@ -260,18 +267,19 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         uint32_t slot = 0, phase = 0;
         bool ok = true;
         for (int32_t t = cluster; ok && t < tiles; t += stride) {
-            int32_t mt, nt;
-            tile_of(t, p, mt, nt);
-            const int32_t row_a = mt * kTileM + (int32_t)pr * 128, row_b = nt * BN + (int32_t)pr * (BN / 2);
+            int32_t mt, nt, half;
+            tile_of(t, p, mt, nt, half);
+            const bool halved = half >= 0;
+            const int32_t row_a = mt * kTileM + (int32_t)pr * 128, row_b = nt * BN + (halved ? half * (BN / 2) + (int32_t)pr * (BN / 4) : (int32_t)pr * (BN / 2));
             const int32_t sfa_row = (row_a >> 7) * p.kblocks, sfb_row = nt * (BN / 128) * p.kblocks;
             for (int32_t k = k0; k < k1; ++k) {
                 ok = __all_sync(0xffffffffu, wait_bar(bar_empty + 8 * slot, phase ^ 1u, w));
                 if (!ok) break;
-                if (pr == 0) expect_bytes(bar_full + 8 * slot, F::kTxPair);
+                if (pr == 0) expect_bytes(bar_full + 8 * slot, halved ? F::kTxPair - F::kBBytes : F::kTxPair);
                 const uint32_t bar = ptx::mapa(bar_full + 8 * slot, leader);
                 const uint32_t dst = tiles_smem + slot * kOperandBytes, sdst = sf_smem + slot * kSfBytes;
                 load_pair(dst, &tmA, k * 128, row_a, bar);
-                load_pair(dst + kABytes, &tmB, k * 128, row_b, bar);
+                load_pair(dst + kABytes, halved ? &tmBh : &tmB, k * 128, row_b, bar);
                 // scales: the packed array as rows of 256 bytes, two per 512-byte block
                 load_pair(sdst, &tmSfa, 0, 2 * (sfa_row + 2 * k), bar);
 #pragma unroll
@@ -299,6 +307,10 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     ptx::tc_fence_after();
                 }
                 const uint32_t d = tmem + acc * BN;
+                int32_t mt, nt, half;
+                tile_of(t, p, mt, nt, half);
+                const uint32_t id0 = half >= 0 ? idesc_mxf4(kTileM, BN / 2, 0) : idesc_mxf4(kTileM, BN, 0), id2 = id0 | idesc_mxf4(0, 0, 2);
+                const uint32_t sfb_at = half > 0 ? 8u : 4u;      // the second half's scales are the tile's second block
                 for (int32_t k = k0; k < k1; ++k) {
                     ok = __all_sync(0xffffffffu, wait_bar(bar_scales + 8 * slot, phase, w));      // operands and scales are there
                     if (!ok) break;
@@ -307,9 +319,9 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     const uint64_t a_desc = ptx::umma_desc_k_sw128(a), b_desc = ptx::umma_desc_k_sw128(a + kABytes);
                     const int halves = min(2, p.kblocks - 2 * k);      // the last step may hold one 128-K block only
                     for (int h = 0; h < halves; ++h) {
-                        const uint32_t sfa = scales + F::kScaleCols * h, sfb = sfa + 4;
-                        mma_mxf4_pair(d, a_desc + 4 * h, b_desc + 4 * h, idesc_mxf4(kTileM, BN, 0), sfa, sfb, (k > k0 || h > 0) ? 1u : 0u);
-                        mma_mxf4_pair(d, a_desc + 4 * h + 2, b_desc + 4 * h + 2, idesc_mxf4(kTileM, BN, 2), sfa, sfb, 1u);
+                        const uint32_t sfa = scales + F::kScaleCols * h, sfb = sfa + sfb_at;
+                        mma_mxf4_pair(d, a_desc + 4 * h, b_desc + 4 * h, id0, sfa, sfb, (k > k0 || h > 0) ? 1u : 0u);
+                        mma_mxf4_pair(d, a_desc + 4 * h + 2, b_desc + 4 * h + 2, id2, sfa, sfb, 1u);
                     }
                     commit_pair(bar_empty + 8 * slot, pair_mask);
                     if (++slot == kStages) slot = 0, phase ^= 1u;
@@ -349,11 +361,12 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         for (int32_t t = cluster; t < tiles; t += stride) {
             if (!__all_sync(0xffffffffu, wait_bar(bar_tfull + 8 * acc, phase, w))) break;
             ptx::tc_fence_after();
-            int32_t mt, nt;
-            tile_of(t, p, mt, nt);
+            int32_t mt, nt, part;
+            tile_of(t, p, mt, nt, part);
+            const int cols = part >= 0 ? kCols / 2 : kCols;      // of this warp, in this tile
             uint32_t r[kChunks][32];
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + half * kCols + c * 32, r[c]);
+            for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_32x32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN + half * cols + c * 32, r[c]);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) ptx::tmem_ld_wait(r[c]);
             ptx::tc_fence_before();
@@ -364,7 +377,8 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             if (row0 >= p.M || *abort_flag != 0) continue;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                const int32_t n0 = nt * BN + half * kCols + c * 32;
+                if (c * 32 >= cols) break;
+                const int32_t n0 = nt * BN + max(part, 0) * (BN / 2) + half * cols + c * 32;
                 float f[32];
 #pragma unroll
                 for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(r[c][q]);
@@ -394,8 +408,8 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     }
 
     if (SPLIT) {
-        int32_t mt, nt;
-        tile_of(cluster, p, mt, nt);
+        int32_t mt, nt, half_tile;
+        tile_of(cluster, p, mt, nt, half_tile);
         const int32_t row0 = mt * kTileM + (int32_t)pr * 128;
         const int32_t live = max(0, min(p.M - row0, 128));
         __syncwarp();
@@ -568,12 +582,13 @@ static int max_clusters(int size) {
 
 template <int BN, bool SPLIT>
 static int launch(const void* A, const void* sfa, const void* B, const void* sfb, int64_t K, const GemmArgs& p, unsigned clusters, cudaStream_t st) {
-    CUtensorMap a, b, sa, sb, c;
+    CUtensorMap a, b, sa, sb, c, bh;
     int rc;
     if ((rc = code_map(&a, A, p.M, K, 128, false)) != KBN_OK || (rc = code_map(&b, B, p.N, K, BN / 2, true)) != KBN_OK ||
         (rc = scale_map(&sa, sfa, p.M, p.kblocks)) != KBN_OK || (rc = scale_map(&sb, sfb, p.N, p.kblocks)) != KBN_OK)
         return rc;
-    c = a;                               // never read without tiled_out
+    c = bh = a;                          // never read without tiled_out, without halved tiles
+    if (p.whole < p.m_tiles * p.n_tiles && (rc = code_map(&bh, B, p.N, K, BN / 4, true)) != KBN_OK) return rc;
     if (p.tiled_out && (rc = out_map(&c, p.C, p.M, p.N, p.ldc)) != KBN_OK) return rc;
     const unsigned size = SPLIT ? 2u * (unsigned)p.S : 2u;
     cudaLaunchConfig_t cfg = {};
@@ -589,7 +604,7 @@ static int launch(const void* A, const void* sfa, const void* B, const void* sfb
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    KBN_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BN, SPLIT>, a, b, sa, sb, c, p));
+    KBN_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BN, SPLIT>, a, b, sa, sb, c, bh, p));
     KBN_CHECK_LAUNCH();
     return KBN_OK;
 }
@@ -599,7 +614,14 @@ static int launch_persistent(const void* A, const void* sfa, const void* B, cons
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     const int pairs = max_clusters<BN, false>(2);
     KBN_REQUIRE(pairs > 0, KBN_ERR_UNSUPPORTED, "kbn_mxfp4_gemm_nt: no CTA pair fits this device");
-    return launch<BN, false>(A, sfa, B, sfb, K, p, (unsigned)std::min<int64_t>(tiles, pairs), st);
+    // A last round that at most half of the pairs have a tile in is worked on in halves, by twice as many (with the quantiser):
+    // 1280 x 4096 x 2048 (80 tiles on 74 pairs) 14.9 -> 13.8 us, x 7168 32.8 -> 30.8, 8192 x 7168 x 1024 (896) 51.7 -> 48.6,
+    // x 7168 180 either way, where power is the bound.  As a launch of their own the halves cost more than they saved.
+    GemmArgs q = p;
+    q.whole = (int32_t)tiles;
+    const int64_t rest = tiles % pairs;
+    if (BN == 256 && tiles > pairs && rest > 0 && 2 * rest <= pairs) q.whole = (int32_t)(tiles - rest);
+    return launch<BN, false>(A, sfa, B, sfb, K, q, (unsigned)std::min<int64_t>(tiles, pairs), st);
 }
 
 }  // namespace mxfp4
@@ -642,6 +664,7 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const vo
         const int per = (p.steps + S - 1) / S;
         if (2 * S * wide > sm_count() || (S - 1) * per >= p.steps || p.steps - per < kSplitGain || wide > max_clusters<256, true>(2 * S)) continue;
         p.S = S;
+        p.whole = (int32_t)wide;
         return launch<256, true>(A, sfa_packed, B, sfb_packed, K, p, (unsigned)wide, st);
     }
     const int64_t pairs = sm_count() / 2;

@@ -443,3 +443,22 @@ def test_gemm_with_k_split_over_a_cluster(cuda_dev, m, n, k):
         ops.mxfp4_gemm_nt(aq, asf, bq, bsf, again, bb)
         assert torch.equal(out[:, :n], again)
     assert ops.gemm_status(cuda_dev) == 0
+
+
+@pytest.mark.parametrize("m,n,k,pad", [(1280, 4096, 512, 8), (1270, 4200, 544, 8), (1270, 4200, 544, 3), (2304, 2309, 96, 0), (300, 12800, 2080, 8)])
+def test_gemm_with_a_halved_last_round(cuda_dev, m, n, k, pad):
+    """A few tiles more than pairs: the last round's tiles in halves, of which the outer may lie behind the last column."""
+    from kb_nano_b200 import ops
+    gen = torch.Generator(device=cuda_dev).manual_seed(m + n + k + pad)
+    aq, asc = operand(m, k, gen, cuda_dev)
+    bq, bsc = operand(n, k, gen, cuda_dev)
+    bias = torch.randn(n, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    asf, bsf = ops.pack_mxfp4_scales(asc, k), ops.pack_mxfp4_scales(bsc, k)
+    a, b = ref.values(aq, asc), ref.values(bq, bsc)
+    for bb in (None, bias):
+        buf = torch.full((m + 1, n + pad), 7.0, dtype=torch.bfloat16, device=cuda_dev)
+        out = buf[:m, :n]
+        ops.mxfp4_gemm_nt(aq, asf, bq, bsf, out, bb)
+        check(out, a, b, bb)
+        assert (buf[m] == 7).all() and (buf[:, n:] == 7).all()
+    assert ops.gemm_status(cuda_dev) == 0
