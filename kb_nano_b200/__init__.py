@@ -4,7 +4,7 @@
   torch_ops  the same calls registered as opaque torch.library ops (for torch.compile)
   candidate  drop-in modules for kb-nano's tasks/candidate + infra/kernel_swapper interface
   inputs     seeded synthetic inputs of the benchmark configurations
-  build      in-tree nvcc build of the library
+  build      in-tree build of the library (nvcc) and of the native call path _calls.so (g++)
 """
 from . import _lib, ops  # noqa: F401
 
