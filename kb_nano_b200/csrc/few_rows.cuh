@@ -11,12 +11,18 @@
 //   product    mma.sync.m16n8k16, f16 x f16 -> fp32: the 16 weight rows are its M, the tokens its N.  (tcgen05 would spend a
 //              128-row tile on them and needs its operands in fp8 or fp4; at this intensity the legacy instruction is far
 //              from being the bound.)  e4m3 and e2m1 codes are converted to f16 exactly, two per instruction.
-//   tokens     held in shared memory as f16, each 128 K-values of a row multiplied by a power of two that brings their
-//              largest magnitude into [2^14, 2^15); the power is taken out of the chunk's partial sum.  bf16 has 8 significant
-//              bits and f16 has 11, so a value is kept exactly down to 2^-32 of its chunk's largest, and below that to within
-//              2^-40 of it.  One power per chunk, not per row, so that a row is converted in one pass, without a barrier.
-//   scales     FP8: one fp32 factor per 128 x 128 block, applied to each 128-K partial sum.  MXFP4: one power of two per row
-//              and 32 K-values, applied to each 32-K partial sum.  Both in fp32, so any scale works.
+//   tokens     held in shared memory as f16, every block of a row (the K-values that share a weight scale: 128 with FP8, 32 with
+//              MXFP4) multiplied by a power of two that brings its largest magnitude into [2^14, 2^15); the power is taken out
+//              of the block's partial sum.  bf16 has 8 significant bits and f16 has 11, so a value is kept exactly down to
+//              2^-32 of its block's largest, and below that to within 2^-39 of it.  One power per block, not per row, so that a
+//              row is converted in one pass, without a barrier, and values that the weights' scales make up for are kept.
+//   scales     FP8: one fp32 factor per 128 x 128 block.  MXFP4: one power of two per row and 32 K-values.  A block's partial
+//              sum is multiplied first by the tokens' power, then by the weights' scale, both in fp32.  So that neither step
+//              leaves fp32's range where the result does not, the tokens' power lacks a constant factor 2^kLift, which the
+//              sums get back at the end: partial sum times power stays below 2^128 (2^31 * 2^(113 - 16) with FP8, 2^23 *
+//              2^(113 - 9) with MXFP4), powers go down to fp32's smallest.  Nothing overflows before 2^128, and a zero sum stays
+//              zero under any scale.  For MXFP4 that is four multiplications a tile and block more than one power per 128 values
+//              behind the blocks' scales, which overflowed from scales of 2^101 on.
 //   K order    a dot product does not care: lane t of a quad takes 16 consecutive K-values of a row per load (FP8) or
 //              eight (MXFP4), and reads the same K-values of its token.
 //   sums       fp32; the warps' partial results meet in shared memory, where two finisher warps (one per buffer, every other
@@ -56,14 +62,19 @@ template <>
 struct Fmt<kFp8> {
     static constexpr int kTiles = 1;                      // 16-row tiles of the matrix instruction per unit
     static constexpr int kChunkBytes = 128, kScaleBytes = 512, kTokenPad = 16;
+    static constexpr int kBlock = 128, kLift = 16;        // K-values that share a weight scale; sums are held times 2^-kLift
 };
 template <>
 struct Fmt<kMxfp4> {
     static constexpr int kTiles = 2;                      // half the bytes a row: two tiles share a warp's token loads and waits
     static constexpr int kChunkBytes = 64, kScaleBytes = 1024, kTokenPad = 64;
+    static constexpr int kBlock = 32, kLift = 9;
 };
 template <int FMT>
 constexpr int kBoxRows = 8 * Fmt<FMT>::kTiles;            // rows of each of a unit's two boxes
+// Bytes of a token row's powers: an fp32 per block.  MXFP4 reads four at once; 16 bytes more keep a warp's rows on different banks.
+template <int FMT>
+__host__ __device__ constexpr int64_t power_bytes(int64_t K) { return K / Fmt<FMT>::kBlock * 4 + (FMT == kMxfp4 ? 16 : 0); }
 template <int FMT>
 constexpr int kRedBytes = kFinishers * kConsumerWarps * 128 * Fmt<FMT>::kTiles * 4;
 
@@ -83,7 +94,7 @@ struct Smem {
     uint8_t* ring;         // stages, 1024-byte aligned
     uint8_t* scales;       // one area per stage
     uint8_t* tokens;       // f16 rows, stride token_stride
-    float* token_scales;   // [rows, K / 128]: what a chunk's partial sum is multiplied by
+    float* token_scales;   // a row of power_bytes each: what the blocks' partial sums are multiplied by
     float* red;            // 32 x 128 partial sums (times tiles): two buffers of 16 warps or four of 8
     uint64_t* bars;        // full[stages], empty[stages], partials full[kBuffers], partials empty[kBuffers]
     int32_t stages;
@@ -236,16 +247,16 @@ __device__ __forceinline__ void produce_unit(const Smem& s, RingPos& pos, const 
     }
 }
 
-// What a consumer lane reads of the tokens: the f16 row of column g, the chunk scales of columns 2t and 2t + 1 (shared-memory
+// What a consumer lane reads of the tokens: the f16 row of column g, the powers of columns 2t and 2t + 1 (shared-memory
 // addresses).  Columns without a token repeat the last one's; nothing reads their results.
 struct TokenColumns {
     uint32_t row, scale0, scale1;
 };
-template <typename RowOf>
+template <int FMT, typename RowOf>
 __device__ __forceinline__ TokenColumns token_columns(const Smem& s, uint32_t stride, int32_t KC, int count, int lane, RowOf row_of) {
     const int g = min(lane >> 2, count - 1), t0 = min(2 * (lane & 3), count - 1), t1 = min(2 * (lane & 3) + 1, count - 1);
-    return TokenColumns{ptx::smem_u32(s.tokens) + (uint32_t)row_of(g) * stride, ptx::smem_u32(s.token_scales) + (uint32_t)(row_of(t0) * KC) * 4u,
-                        ptx::smem_u32(s.token_scales) + (uint32_t)(row_of(t1) * KC) * 4u};
+    const uint32_t powers = ptx::smem_u32(s.token_scales), row_bytes = (uint32_t)power_bytes<FMT>(128 * (int64_t)KC);
+    return TokenColumns{ptx::smem_u32(s.tokens) + (uint32_t)row_of(g) * stride, powers + (uint32_t)row_of(t0) * row_bytes, powers + (uint32_t)row_of(t1) * row_bytes};
 }
 
 // Consumer warp: its chunks of one unit, added to acc.  acc[i][0..1]: row 8 i + g of box 0 with tokens 2t, 2t + 1; acc[i][2..3]:
@@ -265,8 +276,8 @@ __device__ __forceinline__ void consume_unit(const Smem& s, OwnPos& here, int32_
             const uint32_t box0 = ptx::smem_u32(s.ring) + here.slot * kStageBytes + (uint32_t)(cw * kBoxRows<FMT> + g) * F::kChunkBytes;
             const uint32_t box1 = box0 + kStageBytes / 2;
             const uint32_t sdst = ptx::smem_u32(s.scales) + here.slot * F::kScaleBytes;
-            const float x0s = __uint_as_float(lds32(tc.scale0 + (uint32_t)c * 4u)), x1s = __uint_as_float(lds32(tc.scale1 + (uint32_t)c * 4u));
             if constexpr (FMT == kFp8) {
+                const float x0s = __uint_as_float(lds32(tc.scale0 + (uint32_t)c * 4u)), x1s = __uint_as_float(lds32(tc.scale1 + (uint32_t)c * 4u));
                 float p[4], q[4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -299,7 +310,8 @@ __device__ __forceinline__ void consume_unit(const Smem& s, OwnPos& here, int32_
                 for (int i = 0; i < F::kTiles; ++i)
 #pragma unroll
                     for (int box = 0; box < 2; ++box) sw[i][box] = lds32(sdst + scale_word(8 * i + g, cw) + box * 512);
-                float q[F::kTiles][4] = {};
+                const uint4 v0 = lds128(tc.scale0 + (uint32_t)c * 16u), v1 = lds128(tc.scale1 + (uint32_t)c * 16u);
+                const uint32_t x0s[4] = {v0.x, v0.y, v0.z, v0.w}, x1s[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                 for (int pair = 0; pair < 2; ++pair) {
                     uint32_t e[F::kTiles][2];
@@ -324,19 +336,13 @@ __device__ __forceinline__ void consume_unit(const Smem& s, OwnPos& here, int32_
                             mma_f16_m16n8k16(p, ha[2], hb[2], ha[3], hb[3], x.z, x.w);
                             const float s0 = b & 1 ? bf16_hi(e[i][0]) : bf16_lo(e[i][0]);
                             const float s1 = b & 1 ? bf16_hi(e[i][1]) : bf16_lo(e[i][1]);
-                            q[i][0] = fmaf(p[0], s0, q[i][0]);
-                            q[i][1] = fmaf(p[1], s0, q[i][1]);
-                            q[i][2] = fmaf(p[2], s1, q[i][2]);
-                            q[i][3] = fmaf(p[3], s1, q[i][3]);
+                            const float t0 = __uint_as_float(x0s[2 * pair + b]), t1 = __uint_as_float(x1s[2 * pair + b]);
+                            acc[i][0] = fmaf(p[0] * t0, s0, acc[i][0]);
+                            acc[i][1] = fmaf(p[1] * t1, s0, acc[i][1]);
+                            acc[i][2] = fmaf(p[2] * t0, s1, acc[i][2]);
+                            acc[i][3] = fmaf(p[3] * t1, s1, acc[i][3]);
                         }
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < F::kTiles; ++i) {
-                    acc[i][0] = fmaf(q[i][0], x0s, acc[i][0]);
-                    acc[i][1] = fmaf(q[i][1], x1s, acc[i][1]);
-                    acc[i][2] = fmaf(q[i][2], x0s, acc[i][2]);
-                    acc[i][3] = fmaf(q[i][3], x1s, acc[i][3]);
                 }
             }
         }
@@ -365,8 +371,10 @@ __device__ __forceinline__ void hand_over(const Smem& s, uint32_t n, int warp, i
 // HALVES: whose unit is the one at this ring slot (0: warps 0-7, 1: warps 8-15).  The finishers follow the ring with a RingPos.
 __device__ __forceinline__ int half_of(const RingPos& pos) { return (int)(pos.slot & 1u); }
 // Finisher: the sums of its n-th unit.  Lane l receives, of each tile, row l / 2, tokens 4 (l % 2) .. + 3.
-template <bool HALVES = false, int TILES>
-__device__ __forceinline__ void take_over(const Smem& s, int finisher, uint32_t n, int lane, float (&v)[TILES][4], const WaitCtx& w) {
+template <int FMT, bool HALVES = false>
+__device__ __forceinline__ void take_over(const Smem& s, int finisher, uint32_t n, int lane, float (&v)[Fmt<FMT>::kTiles][4], const WaitCtx& w) {
+    constexpr int TILES = Fmt<FMT>::kTiles;
+    constexpr float kUnlift = (float)(1 << Fmt<FMT>::kLift);
     constexpr int kPartials = HALVES ? 8 : kConsumerWarps;
     const int buf = HALVES ? 2 * finisher + (int)(n & 1u) : finisher;
     wait_ring(ptx::smem_u32(s.bars + 2 * s.stages + buf), (HALVES ? n >> 1 : n) & 1u, w);
@@ -379,6 +387,8 @@ __device__ __forceinline__ void take_over(const Smem& s, int finisher, uint32_t 
             const float4 p = r[(j * TILES + i) * 32];
             v[i][0] += p.x; v[i][1] += p.y; v[i][2] += p.z; v[i][3] += p.w;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] *= kUnlift;
     }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(s.bars + 2 * s.stages + kBuffers + buf));
@@ -403,14 +413,17 @@ __device__ __forceinline__ int token_exponent(uint32_t amax_bits) {
     return 14 - e;
 }
 
-// Rows of K values -> f16 rows and chunk scales in shared memory, normalised as described above, by NT threads.  T: fp32 or
+// Rows of K values -> f16 rows and the blocks' powers in shared memory, normalised as described above, by NT threads.  T: fp32 or
 // bf16.  row_ptr(i): row i < n, 16-byte aligned.  No barrier inside: the caller sees to it that nobody reads the rows that
 // are replaced, and publishes the new ones.  BATCH loads are under way at once in every thread.
-template <typename T, int NT, typename RowPtr>
+template <int FMT, typename T, int NT, typename RowPtr>
 __device__ __forceinline__ void load_tokens(const Smem& s, uint32_t stride, int n, int K, RowPtr row_ptr, int tid) {
+    constexpr int kTeam = Fmt<FMT>::kBlock / 8;   // consecutive threads that share a block of a row: K % 128 == 0
+    constexpr int kMaxExponent = 149 - Fmt<FMT>::kLift;      // so that a power is never below fp32's smallest value
+    const uint32_t row_powers = (uint32_t)power_bytes<FMT>(K) / 4u;
     constexpr int W = sizeof(T) / 2;              // 16-byte loads per eight values
     constexpr int BATCH = 8 / W;
-    const uint32_t vecs = (uint32_t)K / 8u;       // K % 128 == 0: sixteen consecutive threads share a chunk of a row
+    const uint32_t vecs = (uint32_t)K / 8u;
     const uint32_t total = (uint32_t)n * vecs;
     const uint32_t magic = 0xffffffffu / vecs + 1u;      // i / vecs == umulhi(i, magic): i * vecs < 2^32 here
     for (uint32_t i0 = 0; i0 < total; i0 += BATCH * NT) {
@@ -445,9 +458,9 @@ __device__ __forceinline__ void load_tokens(const Smem& s, uint32_t stride, int 
                 m = max(m, b < 0x7f800000u ? b : 0u);         // infinities and NaNs keep their place, the finite values set the scale
             }
 #pragma unroll
-            for (int o = 8; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = kTeam / 2; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (i < total) {
-                const int e = token_exponent(m);
+                const int e = min(token_exponent(m), kMaxExponent);
                 uint32_t h[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -455,7 +468,7 @@ __device__ __forceinline__ void load_tokens(const Smem& s, uint32_t stride, int 
                     h[j] = *reinterpret_cast<const uint32_t*>(&p);
                 }
                 *reinterpret_cast<uint4*>(s.tokens + (size_t)row * stride + (size_t)v * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-                if ((tid & 15) == 0) s.token_scales[row * (vecs >> 4) + (v >> 4)] = scale_pow2(1.0f, -e);
+                if ((tid & (kTeam - 1)) == 0) s.token_scales[row * row_powers + v / kTeam] = scale_pow2(1.0f, -e - Fmt<FMT>::kLift);
             }
         }
     }

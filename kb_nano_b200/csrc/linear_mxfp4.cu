@@ -2,8 +2,7 @@
 //
 // At most eight rows (a decode step): one launch.  Every CTA quantises the rows itself -- a few thousand values, under a
 // microsecond a row -- into f16 rows in shared memory and streams its share of the weight rows (few_rows.cuh).  The values are
-// the ones the quantiser would have stored: a code times 2^(b - b_max), b_max the largest of the scale bytes of 128 values, is
-// exact in f16 down to 2^-36 of the largest block, and the power is taken out of the 128 values' partial sum.
+// the ones the quantiser would have stored: the codes, exact in f16, and each block's power of two beside them.
 // More rows, or K no multiple of 128: the quantiser and the tensor-core GEMM.
 // Measured, one row, 4096 x 7168 (15.6 MB, 2.4 us at a copy's rate): 6.3 us, against
 // 14.9 for quantiser and GEMM; 7168 x 2048, one to eight rows, 5.2 to 6.5 and 8.7 to 9.4.  Every row adds what its quantisation
@@ -33,10 +32,12 @@ struct LinearArgs {
     int32_t M, N, K, stages, token_stride;
 };
 
-// x rows -> MXFP4 values as f16 and their chunk scales, by all consumer threads.
+// x rows -> MXFP4 codes as f16 (times 2^-kLift, see few_rows.cuh) and their blocks' powers, by all consumer threads.
 __device__ __forceinline__ void quantise_tokens(const Smem& s, const LinearArgs& a, bool vec, int tid) {
     constexpr int NT = 32 * kConsumerWarps, BATCH = 4;
-    const uint32_t vecs = (uint32_t)a.K / 8u, total = (uint32_t)a.M * vecs;      // sixteen consecutive threads share a chunk, four a block
+    const uint32_t vecs = (uint32_t)a.K / 8u, total = (uint32_t)a.M * vecs;      // four consecutive threads share a block
+    const uint32_t row_powers = (uint32_t)power_bytes<kMxfp4>(a.K) / 4u;
+    const __half2 lift = __float2half2_rn(1.0f / (1 << Fmt<kMxfp4>::kLift));
     const uint32_t magic = 0xffffffffu / vecs + 1u;      // i / vecs == umulhi(i, magic): i * vecs < 2^32 here
     for (uint32_t i0 = 0; i0 < total; i0 += BATCH * NT) {
         uint32_t w[BATCH][4];
@@ -65,22 +66,16 @@ __device__ __forceinline__ void quantise_tokens(const Smem& s, const LinearArgs&
             m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = mxfp4::max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const uint32_t b = mxfp4::scale_byte(max(m & 0xffffu, m >> 16));
-            int top = b == 255u ? 0 : (int)b;
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
             uint32_t h[4];
             mxfp4::unpack_e2m1x8(mxfp4::quant8(w[k], mxfp4::inv_scale(b), b == 255u), h);
             if (i < total) {
-                // 2^(b - top + 13): the largest code, 6, becomes 49152
-                const float f = b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(max((int)b - top + 13, -126) + 127) << 23);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const __half2 c = *reinterpret_cast<const __half2*>(&h[j]);
-                    const __half2 r = __floats2half2_rn(__low2float(c) * f, __high2float(c) * f);
-                    h[j] = *reinterpret_cast<const uint32_t*>(&r);
+                    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h[j]), lift);
+                    h[j] = b == 255u ? 0x7e007e00u : *reinterpret_cast<const uint32_t*>(&r);      // a block with an infinity or a NaN is all NaN
                 }
                 *reinterpret_cast<uint4*>(s.tokens + (size_t)row * (uint32_t)a.token_stride + (size_t)v * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-                if ((tid & 15) == 0) s.token_scales[row * (vecs >> 4) + (v >> 4)] = scale_pow2(1.0f, top - 127 - 13);
+                if ((tid & 3) == 0) s.token_scales[row * row_powers + v / 4] = mxfp4::scale_value(b);
             }
         }
     }
@@ -125,7 +120,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
         OwnPos pos(warp);
         quantise_tokens(s, a, vec != 0, tid);
         consumer_sync();
-        const TokenColumns columns = token_columns(s, (uint32_t)a.token_stride, KC, a.M, lane, [](int col) { return col; });
+        const TokenColumns columns = token_columns<kMxfp4>(s, (uint32_t)a.token_stride, KC, a.M, lane, [](int col) { return col; });
         for (int32_t u = u0; u < u1; ++u) {
             float acc[Fmt<kMxfp4>::kTiles][4] = {};
             consume_unit<kMxfp4>(s, pos, KC, warp, lane, columns, acc, w);
@@ -135,7 +130,7 @@ mxfp4_linear_few_kernel(const __grid_constant__ CUtensorMap tm, const LinearArgs
         const WaitCtx w{abort_flag, a.status, 21};
         for (int32_t u = u0 + warp - kFirstFinisher; u < u1; u += kFinishers) {
             float v[Fmt<kMxfp4>::kTiles][4];
-            take_over(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
+            take_over<kMxfp4>(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
             const int tok0 = 4 * (lane & 1);
 #pragma unroll
             for (int tile = 0; tile < Fmt<kMxfp4>::kTiles; ++tile) {
@@ -174,7 +169,7 @@ static int linear_few(const void* x, int64_t ld_x, int64_t M, int64_t K, const v
     if (rc != KBN_OK) return rc;
     const int64_t units = (N + kUnitRows - 1) / kUnitRows;
     const unsigned grid = (unsigned)std::min<int64_t>(units, sm_count());
-    const size_t smem = (size_t)(kLinearFixed + M * (a.token_stride + K / 32) + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));
+    const size_t smem = (size_t)(kLinearFixed + M * (a.token_stride + power_bytes<kMxfp4>(K)) + stages * (kStageBytes + Fmt<kMxfp4>::kScaleBytes));
     const int vec = (ld_x % 8 == 0 || M == 1) && aligned16(x);
     KBN_CUDA(launch_pdl(mxfp4_linear_few_kernel, dim3(grid), dim3(kThreads), smem, st, tm, a, vec));
     KBN_CHECK_LAUNCH();
@@ -210,7 +205,7 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
     KBN_REQUIRE(!rows_overlap(x, ld_x, K, C, ldc, N, M), KBN_ERR_ARG, "kbn_mxfp4_linear: x and the output overlap");
     // The weight stream serves up to eight rows, as long as their f16 values leave room for the ring.
     if (M <= kMaxGroup && K % 128 == 0 && K < (1ll << 17) && N < (1ll << 27)) {
-        const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad + K / 32);
+        const int64_t left = kSmemMax - kLinearFixed - M * (K * 2 + Fmt<kMxfp4>::kTokenPad + power_bytes<kMxfp4>(K));
         const int64_t stages = std::min<int64_t>(left / (kStageBytes + Fmt<kMxfp4>::kScaleBytes), kMaxStages);
         if (stages >= kLinearMinStages) return linear_few(x, ld_x, M, K, B, sfb_packed, bias, C, ldc, N, (int)stages, static_cast<cudaStream_t>(stream));
     }

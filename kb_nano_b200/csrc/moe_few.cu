@@ -10,7 +10,7 @@
 // grouped GEMMs, activation and reduction (tasks/baseline/L2/qwen3_moe.py:161-188, tasks/baseline/L2/fused_experts.py:208-283).
 // The activations are not quantised here: with a few tokens that saves no bytes (the weights are everything), so the result
 // is closer to the real-number one than the W8A8 pipeline's.  Roundings: the tokens and the activated rows to 11 bits
-// beside a power of two per 128 values (few_rows.cuh), the result to bf16; everything between is fp32.
+// beside a power of two per block of 128 or 32 values (few_rows.cuh), the result to bf16; everything between is fp32.
 //
 // Bound: the chosen experts' weights, once.  A CTA's range of units is contiguous over (job, row block), so the tokens of
 // a job are loaded into shared memory once or twice per CTA and the ring keeps filling meanwhile.  What a small call takes
@@ -167,14 +167,14 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
             }
         }
     }
-    if (at_once && warp < kConsumerWarps / 2) load_tokens<__nv_bfloat16, 16 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
+    if (at_once && warp < kConsumerWarps / 2) load_tokens<FMT, __nv_bfloat16, 16 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
     __syncthreads();
     // The producer groups the pairs and starts on the weights at once; the others join as soon as the jobs are there.
     if (warp == kProducerWarp) {
         build_jobs(sc, a.T, a.topk, a.group, lane);
         asm volatile("bar.arrive %0, %1;" ::"n"(kJobsBarrier), "n"(kThreads) : "memory");
     } else {
-        if (resident && !at_once && warp < kConsumerWarps) load_tokens<__nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
+        if (resident && !at_once && warp < kConsumerWarps) load_tokens<FMT, __nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
         asm volatile("bar.sync %0, %1;" ::"n"(kJobsBarrier), "n"(kThreads) : "memory");
         if (blockIdx.x == 0) {            // for the second kernel
             const uint32_t* src = reinterpret_cast<const uint32_t*>(&sc.jobs);
@@ -208,12 +208,12 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
             if (job != loaded) {
                 if (!resident) {
                     consumer_sync();          // everybody is done with the last job's tokens
-                    load_tokens<__nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, a.H,
+                    load_tokens<FMT, __nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, a.H,
                                                                     [&](int i) { return token(sc.jobs.pair[job][i] / a.topk); }, tid);
                     consumer_sync();
                 }
                 loaded = job;
-                columns = token_columns(s, (uint32_t)a.token_stride, KC, count, lane, [&](int col) { return resident ? sc.jobs.pair[job][col] / a.topk : col; });
+                columns = token_columns<FMT>(s, (uint32_t)a.token_stride, KC, count, lane, [&](int col) { return resident ? sc.jobs.pair[job][col] / a.topk : col; });
             }
             float acc[Fmt<FMT>::kTiles][4] = {};
             consume_unit<FMT>(s, pos, KC, warp, lane, columns, acc, w);
@@ -225,7 +225,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         for (int64_t u = u0; u < u1; ++u) {
             if ((u - u0) % kFinishers == warp - kFirstFinisher) {
                 float v[Fmt<FMT>::kTiles][4];
-                take_over(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
+                take_over<FMT>(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
                 const int count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -330,11 +330,11 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                 const int32_t c0 = first_chunk(part);
                 kc = first_chunk(part + 1) - c0;
                 consumer_sync();
-                load_tokens<float, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, 128 * kc,
+                load_tokens<FMT, float, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, count, 128 * kc,
                                                         [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I + 128 * c0; }, tid);
                 consumer_sync();
                 loaded = vj;
-                columns = token_columns(s, (uint32_t)a.token_stride, kc, count, lane, [](int col) { return col; });
+                columns = token_columns<FMT>(s, (uint32_t)a.token_stride, kc, count, lane, [](int col) { return col; });
             }
             float acc[Fmt<FMT>::kTiles][4] = {};
             const bool part = !HALVES || pos.ahead == 0;      // a unit is one stage
@@ -351,7 +351,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         for (int64_t u = u0; u < u1; ++u) {
             if ((HALVES ? half_of(pos) : (int)((u - u0) % kFinishers)) == finisher) {
                 float v[Fmt<FMT>::kTiles][4];
-                take_over<HALVES>(s, finisher, taken++, lane, v, w);
+                take_over<FMT, HALVES>(s, finisher, taken++, lane, v, w);
                 const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -387,15 +387,15 @@ struct Plan {
 };
 
 template <int FMT>
-static int64_t row_bytes(int64_t K) {      // of a token row with its chunk scales
-    return K * 2 + Fmt<FMT>::kTokenPad + K / 32;
+static int64_t row_bytes(int64_t K) {      // of a token row with its powers
+    return K * 2 + Fmt<FMT>::kTokenPad + power_bytes<FMT>(K);
 }
 template <int FMT>
 static int64_t fixed_bytes() {
     return 1024 + kRedBytes<FMT> + scratch_bytes() + kBarBytes;
 }
 
-// As many token rows of K values (with their chunk scales), up to `want`, as leave room for a ring of at least kMinStages.
+// As many token rows of K values (with their powers), up to `want`, as leave room for a ring of at least kMinStages.
 template <int FMT>
 static bool plan(int64_t K, int want, Plan* p) {
     const int64_t row = row_bytes<FMT>(K), per_stage = kStageBytes + Fmt<FMT>::kScaleBytes, fixed = fixed_bytes<FMT>();
@@ -403,7 +403,7 @@ static bool plan(int64_t K, int want, Plan* p) {
         const int64_t left = kSmemMax - fixed - g * row;
         if (left < kMinStages * per_stage) continue;
         p->rows = g;
-        p->token_stride = (int)(row - K / 32);
+        p->token_stride = (int)(row - power_bytes<FMT>(K));
         p->stages = (int)std::min<int64_t>(left / per_stage, kMaxStages);
         p->smem = (size_t)(fixed + g * row + p->stages * per_stage);
         return true;
