@@ -337,11 +337,12 @@ int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t K, void* a_
  *     All contiguous.
  *   out [T,H] bf16, row stride ld_out; out_w fp32 [T,topk] and out_ids int32 [T,topk] (both or neither): the routing.
  * The activations are not quantised (a few tokens cost no bytes): out = bf16(sum_s w_s * W2 (silu(W1 x) * (W3 x))), summed
- * in fp32 in slot order, tokens and activated rows rounded to 11 bits beside a power of two per 128 (MXFP4: 32) values.  A NaN logit
- * makes all of a softmax router's scores NaN, and only its own expert's score of a sigmoid router; a NaN score is never
- * chosen.  A token without a single choice gets ids -1 and a row of NaNs.  out may be x.  workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents
- * irrelevant; calls that may overlap need one each.  KBN_ERR_UNSUPPORTED when a row of H values does not fit the
- * shared memory of an SM (about 55,000).  Waits inside are bounded and report through kbn_gemm_status.
+ * in fp32 in slot order; tokens exactly (a value 2^-32 below the largest of its 128, MXFP4 32, to f16's smallest step), activated
+ * rows to 22 bits.  A NaN logit makes all of a softmax router's scores NaN, and only its own expert's score of a sigmoid
+ * router; a NaN score is never chosen.  A token without a single choice gets ids -1 and a row of NaNs.  out may be x.
+ * workspace: kbn_moe_few_tokens_workspace_bytes bytes of device scratch, contents irrelevant; calls that may overlap need one
+ * each.  KBN_ERR_UNSUPPORTED when a row of H values does not fit the shared memory of an SM (H above 74,624, MXFP4 62,848).
+ * Waits inside are bounded and report through kbn_gemm_status.
  */
 int64_t kbn_moe_few_tokens_workspace_bytes(int64_t T, int64_t topk, int64_t H, int64_t I);
 int kbn_moe_few_tokens(const void* x, int64_t ld_x, int64_t T, const void* logits, int logits_bf16, int64_t ld, int64_t E,

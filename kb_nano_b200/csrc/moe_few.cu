@@ -3,14 +3,19 @@
 //   few_gate_up   every CTA routes all tokens (one warp each, moe_route.cuh) and groups the chosen (token, slot) pairs into
 //                 jobs of one expert and at most eight tokens; then streams the gate and up rows of the jobs' experts and
 //                 writes silu(gate) * up, fp32, for every pair
-//   few_down      streams the down rows and adds up each token's rows with the router weights, in slot order, where the
-//                 last of an output column block's jobs ends
+//   few_down      streams the down rows, for at most four tokens at a time (their rows take two columns each, see below), and
+//                 adds up each token's rows with the router weights, in slot order, where the last of an output column block's
+//                 jobs ends
 //
 // out[t] = sum_s w[t, s] * W2_e (silu(W1_e x_t) * (W3_e x_t)), e = e[t, s]; kb-nano runs it as routing, permutation, two
 // grouped GEMMs, activation and reduction (tasks/baseline/L2/qwen3_moe.py:161-188, tasks/baseline/L2/fused_experts.py:208-283).
 // The activations are not quantised here: with a few tokens that saves no bytes (the weights are everything), so the result
-// is closer to the real-number one than the W8A8 pipeline's.  Roundings: the tokens and the activated rows to 11 bits
-// beside a power of two per block of 128 or 32 values (few_rows.cuh), the result to bf16; everything between is fp32.
+// is closer to the real-number one than the W8A8 pipeline's.  Roundings: the activated rows to 22 bits beside a power of two per
+// block of 128 or 32 values (few_rows.cuh; the bf16 tokens are exact there), the result to bf16; everything between is fp32.
+// 22 bits, in two f16 pieces side by side in the product's columns, and not 11: with 11 the layer's error against 64 bits was 1 %
+// above that of fp32 arithmetic.  An expert of more than four tokens then has its down rows streamed twice, by CTAs that run side by
+// side, mostly from L2 (I 14336, 8 experts, 16 tokens: MXFP4 228 -> 232 us, FP8 286 -> 299); products of their own for the second
+// pieces needed twice the shared memory (300 and 349).
 //
 // Bound: the chosen experts' weights, once.  A CTA's range of units is contiguous over (job, row block), so the tokens of
 // a job are loaded into shared memory once or twice per CTA and the ring keeps filling meanwhile.  What a small call takes
@@ -39,7 +44,7 @@ struct Jobs {
 struct MoeArgs {
     const __nv_bfloat16* x;
     int64_t ld_x;
-    int32_t T, topk, H, I, E, group;
+    int32_t T, topk, H, I, E, group;      // group: most tokens of a job of the first kernel
     const void *s13, *s2;          // weight scales
     int32_t tiled13, tiled2;       // their loads are tiled (MXFP4, K % 512 == 0)
     float* y;                      // [pairs, I]
@@ -121,6 +126,29 @@ __device__ __forceinline__ void build_jobs(Scratch& sc, int T, int topk, int gro
 }
 constexpr int kJobsBarrier = 3;
 
+// The second kernel's jobs, by one warp: those of more than kPieceGroup tokens in two halves.
+__device__ __forceinline__ void write_down_jobs(const Jobs& jobs, Jobs* out, int lane) {
+    static_assert(kMaxGroup <= 2 * kPieceGroup, "a job has two halves at most");
+    const unsigned before = (1u << lane) - 1u;
+    int n = 0;
+    for (int base = 0; base < jobs.n_jobs; base += 32) {
+        const int job = base + lane, count = job < jobs.n_jobs ? jobs.count[job] : 0;
+        const unsigned any = __ballot_sync(0xffffffffu, count > 0), split = __ballot_sync(0xffffffffu, count > kPieceGroup);
+        const int at = n + __popc(any & before) + __popc(split & before), first = count > kPieceGroup ? (count + 1) / 2 : count;
+        for (int k = 0; k < count; ++k) out->pair[k < first ? at : at + 1][k < first ? k : k - first] = jobs.pair[job][k];
+        if (count > 0) {
+            out->expert[at] = jobs.expert[job];
+            out->count[at] = first;
+        }
+        if (count > first) {
+            out->expert[at + 1] = jobs.expert[job];
+            out->count[at + 1] = count - first;
+        }
+        n += __popc(any) + __popc(split);
+    }
+    if (lane == 0) out->n_jobs = n;
+}
+
 // A copy that was asked for may still be on its way when a bounded wait has run out: give it time to land before the
 // shared memory is given back.
 __device__ __forceinline__ void drain_after_abort(const volatile int* abort_flag) {
@@ -177,23 +205,22 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         if (resident && !at_once && warp < kConsumerWarps) load_tokens<FMT, __nv_bfloat16, 32 * kConsumerWarps>(s, (uint32_t)a.token_stride, a.T, a.H, token, tid);
         asm volatile("bar.sync %0, %1;" ::"n"(kJobsBarrier), "n"(kThreads) : "memory");
         if (blockIdx.x == 0) {            // for the second kernel
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(&sc.jobs);
-            uint32_t* dst = reinterpret_cast<uint32_t*>(a.jobs);
             const int i0 = tid - (warp > kProducerWarp ? 32 : 0);      // the producer is not here
-            for (int i = i0; i < (int)(sizeof(Jobs) / 4); i += kThreads - 32) dst[i] = src[i];
+            for (int i = i0; i < a.T * a.topk; i += kThreads - 32) a.jobs->weight[i] = sc.jobs.weight[i];
             for (int i = i0; i < a.H / (2 * kBoxRows<FMT>); i += kThreads - 32) a.counters[i] = 0;
+            if (warp == kFirstFinisher) write_down_jobs(sc.jobs, a.jobs, lane);
         }
     }
 
     constexpr int kRows = kBoxRows<FMT>;      // gate rows, and as many up rows, of a unit
     const int32_t blocks = a.I / kRows, KC = a.H / 128;
-    const int64_t units = (int64_t)sc.jobs.n_jobs * blocks;
-    const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    int32_t job = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)job * blocks);
+    const int64_t units = (int64_t)sc.jobs.n_jobs * blocks;      // below 2^31: at most 16 E jobs, E * 2 I rows below 2^31
+    const int32_t u0 = (int32_t)(units * blockIdx.x / gridDim.x), u1 = (int32_t)(units * (blockIdx.x + 1) / gridDim.x);
+    int32_t job = u0 / blocks, rb = u0 - job * blocks;
     if (warp == kProducerWarp) {
         const WaitCtx w{&sc.abort_flag, a.status, 8};
         RingPos pos;
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[job] * 2 * a.I + kRows * rb;
             produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s13, a.tiled13 ? &tm_scales : nullptr}, row, row + a.I, 2 * a.I * a.E, KC, 0, KC, lane, w);
             if (++rb == blocks) rb = 0, ++job;
@@ -203,7 +230,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         OwnPos pos(warp);
         int32_t loaded = -1;
         TokenColumns columns{};
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             const int count = sc.jobs.count[job];
             if (job != loaded) {
                 if (!resident) {
@@ -222,7 +249,7 @@ few_gate_up_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         }
     } else {
         const WaitCtx w{&sc.abort_flag, a.status, 19};
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             if ((u - u0) % kFinishers == warp - kFirstFinisher) {
                 float v[Fmt<FMT>::kTiles][4];
                 take_over<FMT>(s, warp - kFirstFinisher, (uint32_t)(u - u0) / kFinishers, lane, v, w);
@@ -307,13 +334,13 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
     // A job's K is worked on in parts of whole stages; vj = (job << log_parts) + part.
     const int32_t lp = MODE == kParts ? a.log_parts : 0, n_parts = n_jobs << lp, k_stages = (KC + kChunks - 1) / kChunks;
     auto first_chunk = [&](int32_t part) { return min(KC, (k_stages * part >> lp) * kChunks); };
-    const int64_t units = (int64_t)n_parts * blocks;
-    const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-    int32_t vj = (int32_t)(u0 / blocks), rb = (int32_t)(u0 - (int64_t)vj * blocks);
+    const int64_t units = (int64_t)n_parts * blocks;      // below 2^31: each has 64 bytes of workspace or more
+    const int32_t u0 = (int32_t)(units * blockIdx.x / gridDim.x), u1 = (int32_t)(units * (blockIdx.x + 1) / gridDim.x);
+    int32_t vj = u0 / blocks, rb = u0 - vj * blocks;
     if (warp == kProducerWarp) {
         const WaitCtx w{&sc.abort_flag, a.status, 10};
         RingPos pos;
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             const int32_t row = sc.jobs.expert[vj >> lp] * a.H + kRows * rb, part = vj & ((1 << lp) - 1);
             produce_unit<FMT>(s, pos, &tm, ScaleSource{a.s2, a.tiled2 ? &tm_scales : nullptr}, row, row + kRows / 2, a.H * a.E, KC, first_chunk(part), first_chunk(part + 1), lane, w);
             if (++rb == blocks) rb = 0, ++vj;
@@ -324,7 +351,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         int32_t loaded = -1, kc = 0;
         uint32_t handed = 0;
         TokenColumns columns{};
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             if (vj != loaded) {
                 const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job];
                 const int32_t c0 = first_chunk(part);
@@ -334,7 +361,7 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
                                                         [&](int i) { return a.y + (int64_t)sc.jobs.pair[job][i] * a.I + 128 * c0; }, tid);
                 consumer_sync();
                 loaded = vj;
-                columns = token_columns<FMT>(s, (uint32_t)a.token_stride, kc, count, lane, [](int col) { return col; });
+                columns = piece_columns<FMT>(s, (uint32_t)a.token_stride, kc, count, lane);
             }
             float acc[Fmt<FMT>::kTiles][4] = {};
             const bool part = !HALVES || pos.ahead == 0;      // a unit is one stage
@@ -348,16 +375,20 @@ few_down_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ 
         uint32_t taken = 0;
         RingPos pos;
         int pending = 0, mine = 0;            // column blocks stored but not yet counted; lane i holds the i-th
-        for (int64_t u = u0; u < u1; ++u) {
+        for (int32_t u = u0; u < u1; ++u) {
             if ((HALVES ? half_of(pos) : (int)((u - u0) % kFinishers)) == finisher) {
                 float v[Fmt<FMT>::kTiles][4];
                 take_over<FMT, HALVES>(s, finisher, taken++, lane, v, w);
-                const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job], tok0 = 4 * (lane & 1);
+                const int job = vj >> lp, part = vj & ((1 << lp) - 1), count = sc.jobs.count[job];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int tile = 0; tile < Fmt<FMT>::kTiles; ++tile)
+#pragma unroll
+                    for (int i = 0; i < kPieceGroup; ++i) v[tile][i] += __shfl_down_sync(0xffffffffu, v[tile][i], 1);      // the odd lanes hold the second pieces' sums
+#pragma unroll
+                for (int i = 0; i < kPieceGroup; ++i)
 #pragma unroll
                     for (int tile = 0; tile < Fmt<FMT>::kTiles; ++tile)
-                        if (tok0 + i < count) a.rows[(((int64_t)sc.jobs.pair[job][tok0 + i] << lp) + part) * a.H + kRows * rb + row_of_lane<FMT>(tile, lane)] = v[tile][i];
+                        if ((lane & 1) == 0 && i < count) a.rows[(((int64_t)sc.jobs.pair[job][i] << lp) + part) * a.H + kRows * rb + row_of_lane<FMT>(tile, lane)] = v[tile][i];
                 if (lane == pending) mine = rb;
                 ++pending;
             }
@@ -387,23 +418,24 @@ struct Plan {
 };
 
 template <int FMT>
-static int64_t row_bytes(int64_t K) {      // of a token row with its powers
-    return K * 2 + Fmt<FMT>::kTokenPad + power_bytes<FMT>(K);
+static int64_t row_bytes(int64_t K, int pieces) {      // of a token with its powers; the second kernel's in two pieces
+    return pieces * (K * 2 + Fmt<FMT>::kTokenPad) + power_bytes<FMT>(K);
 }
 template <int FMT>
 static int64_t fixed_bytes() {
     return 1024 + kRedBytes<FMT> + scratch_bytes() + kBarBytes;
 }
 
-// As many token rows of K values (with their powers), up to `want`, as leave room for a ring of at least kMinStages.
+// As many tokens of K values (with their powers), up to `want`, as leave room for a ring of at least kMinStages; a single token
+// whose row does not, at least three.
 template <int FMT>
-static bool plan(int64_t K, int want, Plan* p) {
-    const int64_t row = row_bytes<FMT>(K), per_stage = kStageBytes + Fmt<FMT>::kScaleBytes, fixed = fixed_bytes<FMT>();
+static bool plan(int64_t K, int want, int pieces, Plan* p) {
+    const int64_t row = row_bytes<FMT>(K, pieces), per_stage = kStageBytes + Fmt<FMT>::kScaleBytes, fixed = fixed_bytes<FMT>();
     for (int g = want; g >= 1; --g) {
         const int64_t left = kSmemMax - fixed - g * row;
-        if (left < kMinStages * per_stage) continue;
+        if (left < kMinStages * per_stage && (g > 1 || left < 3 * per_stage)) continue;
         p->rows = g;
-        p->token_stride = (int)(row - power_bytes<FMT>(K));
+        p->token_stride = (int)(K * 2 + Fmt<FMT>::kTokenPad);
         p->stages = (int)std::min<int64_t>(left / per_stage, kMaxStages);
         p->smem = (size_t)(fixed + g * row + p->stages * per_stage);
         return true;
@@ -412,18 +444,19 @@ static bool plan(int64_t K, int want, Plan* p) {
 }
 
 // Parts of K per job of the second kernel, as a power of two, and the longest part's length.  The rows of a job's tokens
-// share the shared memory with the ring: with long rows whole, a job holds fewer tokens, and an expert with more is streamed
-// again.  So: one part if that leaves a ring beside a full job, else the fewest parts, of three stages or more, that leave a
-// ring of seven.  I 14336, 8 experts, whole / two / four parts: MXFP4, 16 tokens 319 / 260 / 223 us, 5 tokens 161.5 / 161.5 /
-// 157.5; FP8, 5 tokens 209 / 211 / 215, where the rule takes two.  Where a full job fits parts only cost: MXFP4, I 7168, 5
-// tokens 90.3 / 95.3.
+// share the shared memory with the ring.  So: one part if that leaves a ring beside a full job, else the fewest parts, of three
+// stages or more, that leave a ring of seven, else the fewest, of a stage or more, that leave a ring.  8 experts, two / four / eight
+// parts (whole rows do not fit): I 14336, MXFP4, 5 tokens - / 157 / 173 us, 16 tokens - / 232 / 253; FP8, 5 tokens 207 / 208 / 225, 16
+// tokens 306 / 299 / 331; I 7168, MXFP4, 5 tokens 96 / 93 / 112, where the rule takes two.  Where a full job fits whole, parts cost:
+// I 6144, FP8, 5 tokens 100 / 106 with two.
 template <int FMT>
 static int log_parts(int64_t T, int64_t I, int64_t* longest) {
     const int64_t S = (I / 128 + kChunks - 1) / kChunks;
     for (int lp = 0;; ++lp) {
         *longest = std::min(I, ((S + ((int64_t)1 << lp) - 1) >> lp) * kChunks * 128);
-        const int64_t ring = kSmemMax - fixed_bytes<FMT>() - std::min<int64_t>(T, kMaxGroup) * row_bytes<FMT>(*longest);
-        if (ring >= (lp == 0 ? kMinStages : 7) * (kStageBytes + Fmt<FMT>::kScaleBytes) || (S >> (lp + 1)) < 3) return lp;
+        const int64_t ring = (kSmemMax - fixed_bytes<FMT>() - std::min<int64_t>(T, kPieceGroup) * row_bytes<FMT>(*longest, 2)) / (kStageBytes + Fmt<FMT>::kScaleBytes);
+        const int64_t shorter = S >> (lp + 1);      // stages of a part with twice as many
+        if (ring >= (lp == 0 ? kMinStages : 7) || shorter < 1 || (shorter < 3 && ring >= kMinStages)) return lp;
     }
 }
 
@@ -445,18 +478,15 @@ static WorkspaceLayout workspace_layout(int64_t T, int64_t topk, int64_t H, int6
 
 template <int FMT>
 static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& ra, int logits_bf16, cudaStream_t st) {
-    // One grouping of the pairs for both kernels: as many rows as either can hold.  The first keeps all tokens if it can.
+    // The first kernel keeps all tokens in shared memory if it can, else those of one job at a time.
     Plan p1, p2;
-    const int most = std::min(a.T, kMaxGroup);
     int64_t longest;
     a.log_parts = log_parts<FMT>(a.T, a.I, &longest);
-    KBN_REQUIRE(plan<FMT>(a.H, most, &p1) && plan<FMT>(longest, most, &p2), KBN_ERR_UNSUPPORTED,
+    KBN_REQUIRE(plan<FMT>(a.H, a.T, 1, &p1) && plan<FMT>(longest, std::min(a.T, kPieceGroup), 2, &p2), KBN_ERR_UNSUPPORTED,
                 "kbn_moe_few_tokens: a row of %d values does not fit the shared memory", std::max(a.H, a.I));
-    a.group = std::min(p1.rows, p2.rows);
-    Plan all;
-    KBN_REQUIRE(plan<FMT>(a.H, a.T, &all) && plan<FMT>(longest, a.group, &p2), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
-    if (all.rows < a.T) plan<FMT>(a.H, a.group, &all);
-    p1 = all;
+    KBN_REQUIRE(p2.rows == std::min(a.T, kPieceGroup), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: shared memory");
+    a.group = std::min(p1.rows, kMaxGroup);
+    if (p1.rows < a.T) plan<FMT>(a.H, a.group, 1, &p1);
     CUtensorMap t13, t2;
     int rc = weight_map<FMT>(&t13, w13, (int64_t)a.E * 2 * a.I, a.H);
     if (rc != KBN_OK) return rc;
@@ -486,7 +516,7 @@ static int run_moe(const void* w13, const void* w2, MoeArgs a, const RouteArgs& 
     KBN_CUDA(launch_pdl(up_kernel, dim3(grid), dim3(kThreads), p1.smem, st, t13, t13s, ra, logits_bf16, a));
     KBN_CHECK_LAUNCH();
     a.stages = p2.stages;
-    a.token_rows = p2.rows;
+    a.token_rows = 2 * p2.rows;
     a.token_stride = p2.token_stride;
     KBN_CUDA(launch_pdl(down_kernel, dim3(grid), dim3(kThreads), p2.smem, st, t2, t2s, a));
     KBN_CHECK_LAUNCH();

@@ -155,7 +155,8 @@ def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13
     Returns out bf16 [T,H]; out_w fp32 [T,top_k] and out_ids int32 [T,top_k], given together, receive the routing.
 
     The activations are not quantised (with a few tokens that saves no bytes), so results differ from fused_experts_fp8 by
-    that pipeline's FP8 rounding of its activations.  Scratch comes from the caching allocator with every call: calls on
+    that pipeline's FP8 rounding of its activations: the tokens are taken as they are, the activated rows keep 22 bits beside a power
+    of two per weight-scale block, everything else is fp32, and the result is rounded to bf16 once.  Scratch comes from the caching allocator with every call: calls on
     several streams, and captured graphs, do not share any."""
     done = _lib.calls().few_tokens_moe(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, scoring, bias, n_group, topk_group, renormalize,
                                        renorm_floor, scale, round_bf16, out, out_w, out_ids)

@@ -143,3 +143,49 @@ def test_moe_small_values_beside_large_ones(cuda_dev, fmt):
     x[:, 1::2] *= 2.0**-25
     lg = torch.randn(6, 4, generator=gen, device=cuda_dev)
     check_moe(cuda_dev, x.to(torch.bfloat16), lg, (w13, s13, w2, s2, f13, f2))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("t,e", [(1, 4), (3, 4), (4, 2), (5, 2), (8, 2), (16, 2)])
+@pytest.mark.parametrize("i", [256, 1280, 7424])
+def test_moe_activated_rows_keep_more_than_f16(cuda_dev, fmt, t, e, i):
+    """Neighbouring activated values that differ by 2^-13 and the down projection's difference of the two: what is left of
+    them is the result, and rounding them to 11 bits would be most of it.  One to eight tokens an expert and more."""
+    gen = torch.Generator(device=cuda_dev).manual_seed(700 + t)
+    h = 256
+    w13, s13, w2, s2, f13, f2 = shifted(fmt, e, h, i, cuda_dev, 44, 0, 17)
+    x = torch.zeros(t, h, device=cuda_dev)                              # two values a row, so that the sums round little
+    x[:, 0] = torch.randn(t, generator=gen, device=cuda_dev)
+    x[:, h - 1] = torch.randn(t, generator=gen, device=cuda_dev) * 2.0**-13
+    b13, b2 = w13.view(torch.uint8), w2.view(torch.uint8)
+    # gate rows 2j and 2j + 1 alike; up rows too but for the last value; four down columns, neighbours of opposite sign
+    b13[:, 1::2] = b13[:, 0::2]
+    if fmt == "fp8":
+        b13[:, :, h - 1] = 0
+        b13[:, i + 1::2, h - 1] = 0x74                                    # 192
+        b2[:, :, 2:i - 2] = 0
+        b2[:, :, 1::2] = b2[:, :, 0::2] ^ 0x80
+    else:
+        s13[:, 1::2] = s13[:, 0::2]
+        b13[:, :, h // 2 - 1] &= 0x0F
+        b13[:, i + 1::2, h // 2 - 1] |= 0x70                              # 6
+        b2[:, :, 1:i // 2 - 1] = 0
+        b2 &= 0x0F
+        b2 |= (b2 << 4) ^ 0x80
+    lg = torch.randn(t, e, generator=gen, device=cuda_dev)
+    check_moe(cuda_dev, x.to(torch.bfloat16), lg, (w13, s13, w2, s2, f13, f2), top=1 if t > 8 else 2, n13=2, n2=4, row=2.0**-22)
+
+
+@pytest.mark.parametrize("fmt,h", [("fp8", 74624), ("mxfp4", 62848)])
+@pytest.mark.parametrize("t", [1, 16])
+def test_moe_longest_token_rows(cuda_dev, fmt, h, t):
+    """The largest H that is taken: one token at a time beside a ring of three stages."""
+    from kb_nano_b200 import moe
+    gen = torch.Generator(device=cuda_dev).manual_seed(800 + t)
+    x = torch.randn(t, h, generator=gen, device=cuda_dev).to(torch.bfloat16)
+    lg = torch.randn(t, 2, generator=gen, device=cuda_dev)
+    ex = experts(fmt, 2, h, 128, cuda_dev, 45)
+    check_moe(cuda_dev, x, lg, ex, top=1)
+    with pytest.raises(RuntimeError, match="shared memory"):
+        longer = torch.cat([x, x[:, :128]], dim=1)
+        moe.few_tokens_moe(longer, lg, *experts(fmt, 2, h + 128, 128, cuda_dev, 46)[:4], 1)
