@@ -3,8 +3,10 @@ small operators, csrc/calls.cpp, which reads torch tensors itself) with g++.
 
     python -m kb_nano_b200.build [--force] [--verbose]
 
-Either is rebuilt only when a source or header is newer than it.  nvcc cross-compiles
-without a GPU, so this also serves as the "does it build" check on a CPU-only machine.
+Either is rebuilt only when a source or header is newer than it, _calls.so also when torch, Python or its command line are not
+the ones it was built with (build/_calls.stamp).  Each is linked beside its place and moved there whole, so that a process that
+loads it during a build finds the old or the new one.  nvcc cross-compiles without a GPU, so this also serves as the "does it
+build" check on a CPU-only machine.
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libkbn_fp8.so")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 CALLS_SRC = os.path.join(CSRC, "calls.cpp")
 CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
+CALLS_STAMP = os.path.join(OBJ_DIR, "_calls.stamp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -62,7 +65,20 @@ def _compile_one(nvcc: str, src: str, verbose: bool) -> tuple[str, str]:
     return obj, r.stderr if verbose else ""
 
 
-def _build_calls() -> None:
+def _link(cmd: list[str], path: str, what: str) -> None:
+    """Runs `cmd` + -o with a file beside `path`, then moves that file there."""
+    tmp = f"{path}.{os.getpid()}.tmp"
+    try:
+        r = subprocess.run([*cmd, "-o", tmp], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
+        os.replace(tmp, path)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+
+
+def _calls_command() -> list[str]:
     import sysconfig
 
     import torch
@@ -71,18 +87,40 @@ def _build_calls() -> None:
     include = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     lib = os.path.join(root, "lib")
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), CALLS_SRC, "-o", CALLS_PATH,
-           f"-L{PKG_DIR}", "-l:" + os.path.basename(LIB_PATH), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {CALLS_SRC}:\n{r.stdout}\n{r.stderr}")
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), CALLS_SRC,
+            f"-L{PKG_DIR}", "-l:" + os.path.basename(LIB_PATH), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
+
+
+def _calls_stamp() -> str:
+    """What _calls.so depends on beside its sources: torch's tensors and Python's objects have no layout of their own promised."""
+    import torch
+    return "\n".join([torch.__version__, sys.version, *_calls_command()])
+
+
+def _calls_need_build() -> bool:
+    if not os.path.exists(CALLS_PATH) or not os.path.exists(CALLS_STAMP):
+        return True
+    t = os.path.getmtime(CALLS_PATH)
+    if any(os.path.getmtime(f) > t for f in (CALLS_SRC, os.path.join(INCLUDE, "kbn_fp8.h"))):
+        return True
+    with open(CALLS_STAMP) as f:
+        return f.read() != _calls_stamp()
+
+
+def _build_calls() -> None:
+    os.makedirs(os.path.dirname(CALLS_STAMP), exist_ok=True)
+    if os.path.exists(CALLS_STAMP):
+        os.remove(CALLS_STAMP)           # an interrupted build is not taken for a finished one
+    _link(_calls_command(), CALLS_PATH, f"g++ on {CALLS_SRC}")
+    with open(CALLS_STAMP, "w") as f:
+        f.write(_calls_stamp())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     _build_lib(force, verbose)
-    if force or not os.path.exists(CALLS_PATH) or any(os.path.getmtime(f) > os.path.getmtime(CALLS_PATH) for f in (CALLS_SRC, os.path.join(INCLUDE, "kbn_fp8.h"))):
+    if force or _calls_need_build():
         _build_calls()
     return LIB_PATH
 
@@ -99,10 +137,7 @@ def _build_lib(force: bool, verbose: bool) -> str:
     if verbose:
         for _, log in results:
             sys.stderr.write(log)
-    cmd = [nvcc, "-shared", "-o", LIB_PATH, *objs, "-cudart", "static", "-Xcompiler", "-fPIC"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _link([nvcc, "-shared", *objs, "-cudart", "static", "-Xcompiler", "-fPIC"], LIB_PATH, "linking the library")
     return LIB_PATH
 
 
