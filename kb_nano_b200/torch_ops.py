@@ -63,6 +63,6 @@ def mxfp4_linear(input: torch.Tensor, a_fp4: torch.Tensor, a_packed: torch.Tenso
 @torch.library.custom_op("kbn_b200::few_tokens_moe", mutates_args=("output",))
 def few_tokens_moe(hidden_states: torch.Tensor, router_logits: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
                    w2_scale: torch.Tensor, output: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None,
-                   n_group: int = 1, topk_group: int = 1, renormalize: bool = True, renorm_floor: float = 0.0, scale: float = 1.0) -> None:
+                   n_group: int = 1, topk_group: int = 1, renormalize: bool = True, renorm_floor: float = 0.0, scale: float = 1.0, round_bf16: bool = False) -> None:
     moe.few_tokens_moe(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, scoring, bias, n_group, topk_group, renormalize,
-                       renorm_floor, scale, out=output)
+                       renorm_floor, scale, round_bf16, out=output)

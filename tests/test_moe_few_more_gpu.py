@@ -1,0 +1,24 @@
+"""The few-token MoE layer where other code reaches it: the registered op, the layer classes."""
+import pytest
+import torch
+
+from tests.test_moe_few_gpu import experts
+
+pytestmark = pytest.mark.gpu
+
+
+def test_registered_op_rounds_scores_as_deepseek_does(cuda_dev):
+    """bf16 logits scored and weighed in bf16 steps: the registered op gives what the function gives, and other than without."""
+    from kb_nano_b200 import moe, ops, torch_ops  # noqa: F401
+    e, h, i, top = 16, 512, 256, 4
+    w13, s13, w2, s2, _, _ = experts("fp8", e, h, i, cuda_dev, 50)
+    x, bias = torch.randn(7, h, device=cuda_dev).to(torch.bfloat16), torch.randn(e, device=cuda_dev) * 0.1
+    lg = torch.randn(7, e, device=cuda_dev).to(torch.bfloat16)
+    outs = [torch.empty_like(x) for _ in range(2)]
+    for rounds in (False, True):
+        torch.ops.kbn_b200.few_tokens_moe(x, lg, w13, s13, w2, s2, outs[rounds], top, "sigmoid", bias, 4, 2, True, 0.0, 1.0, rounds)
+        assert torch.equal(outs[rounds], moe.few_tokens_moe(x, lg, w13, s13, w2, s2, top, "sigmoid", bias, 4, 2, round_bf16=rounds))
+    assert not torch.equal(outs[0], outs[1])
+    by_default = torch.empty_like(x)
+    torch.ops.kbn_b200.few_tokens_moe(x, lg, w13, s13, w2, s2, by_default, top, "sigmoid", bias, 4, 2)
+    assert torch.equal(by_default, outs[0]) and ops.gemm_status(cuda_dev) == 0
