@@ -38,6 +38,7 @@ void set_error(const char* fmt, ...);   // thread-local message returned by kbn_
     } while (0)
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static inline bool aligned_to(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }      // a power of two; null is
 
 int sm_count();   // SMs of the current device (cached per device)
 

@@ -637,6 +637,7 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, const void* sfa_packed, const vo
     KBN_REQUIRE(K % 32 == 0, KBN_ERR_ARG, "kbn_mxfp4_gemm_nt: K=%lld must be a multiple of 32", (long long)K);
     KBN_REQUIRE(aligned16(A) && aligned16(B) && aligned16(sfa_packed) && aligned16(sfb_packed), KBN_ERR_ARG, "kbn_mxfp4_gemm_nt: pointers must be 16-byte aligned");
     KBN_REQUIRE((reinterpret_cast<uintptr_t>(C) & 1u) == 0 && (ldc >= N || M == 1), KBN_ERR_ARG, "kbn_mxfp4_gemm_nt: odd output pointer or row stride below N");
+    KBN_REQUIRE(aligned_to(bias, 2), KBN_ERR_ARG, "kbn_mxfp4_gemm_nt: odd bias pointer");
     const int64_t kblocks = (K + 127) / 128;
     // packed-scale rows and tile numbers are 32-bit in the kernel
     KBN_REQUIRE(K < (1ll << 31) && M < (1ll << 30) && N < (1ll << 30) && (M / 128 + 3) * kblocks * 2 < (1ll << 31) && (N / 128 + 3) * kblocks * 2 < (1ll << 31) &&

@@ -201,6 +201,7 @@ extern "C" int kbn_mxfp4_linear(const void* x, int64_t ld_x, int64_t M, int64_t 
     KBN_REQUIRE(aligned16(B) && aligned16(sfb_packed) && aligned16(a_q) && aligned16(a_sf), KBN_ERR_ARG, "kbn_mxfp4_linear: pointers must be 16-byte aligned");
     KBN_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1u) == 0 && (reinterpret_cast<uintptr_t>(C) & 1u) == 0 && ((ld_x >= K && ldc >= N) || M == 1), KBN_ERR_ARG,
                 "kbn_mxfp4_linear: odd pointer or a row stride too small");
+    KBN_REQUIRE(aligned_to(bias, 2), KBN_ERR_ARG, "kbn_mxfp4_linear: odd bias pointer");
     // the one-launch form still reads x where it already writes C
     KBN_REQUIRE(!rows_overlap(x, ld_x, K, C, ldc, N, M), KBN_ERR_ARG, "kbn_mxfp4_linear: x and the output overlap");
     // The weight stream serves up to eight rows, as long as their f16 values leave room for the ring.

@@ -555,6 +555,8 @@ extern "C" int kbn_moe_few_tokens(const void* x, int64_t ld_x, int64_t T, const 
     KBN_REQUIRE(aligned16(x) && (ld_x % 8 == 0 || T == 1), KBN_ERR_ARG, "kbn_moe_few_tokens: rows of x must start on 16-byte boundaries");
     KBN_REQUIRE(aligned16(w13) && aligned16(w2) && (reinterpret_cast<uintptr_t>(w13_s) & 3u) == 0 && (reinterpret_cast<uintptr_t>(w2_s) & 3u) == 0, KBN_ERR_ARG,
                 "kbn_moe_few_tokens: weights must be 16-byte aligned, their scales 4-byte aligned");
+    KBN_REQUIRE(aligned_to(logits, logits_bf16 ? 2 : 4) && aligned_to(bias, 4) && aligned_to(out, 2) && aligned_to(out_w, 4) && aligned_to(out_ids, 4), KBN_ERR_ARG,
+                "kbn_moe_few_tokens: logits, bias, out, out_w and out_ids must be aligned to their elements");
     KBN_REQUIRE(E * 2 * I < (1ll << 31) && E * H < (1ll << 31), KBN_ERR_UNSUPPORTED, "kbn_moe_few_tokens: more than 2^31 weight rows");
     const WorkspaceLayout wl = workspace_layout(T, topk, H, I);
     KBN_REQUIRE(workspace_bytes >= wl.total && aligned16(workspace), KBN_ERR_ARG, "kbn_moe_few_tokens: workspace of %lld bytes (16-byte aligned) needed, got %lld",
