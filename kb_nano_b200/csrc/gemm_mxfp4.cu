@@ -555,10 +555,11 @@ static int out_map(CUtensorMap* tm, const void* base, int64_t M, int64_t N, int6
 
 template <int BN, bool SPLIT>
 static int max_clusters(int size) {
-    static int cache[64][9] = {};
+    static std::atomic<int> cache[64][9];      // calls come from several threads at once, without the interpreter's lock
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (cache[dev][size] == 0) {
+    int known = cache[dev][size].load(std::memory_order_acquire);
+    if (known == 0) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(size * 16));
         cfg.blockDim = dim3(kGemmThreads);
@@ -575,9 +576,10 @@ static int max_clusters(int size) {
             cudaGetLastError();
             n = 0;
         }
-        cache[dev][size] = n > 0 ? n : -1;
+        known = n > 0 ? n : -1;
+        cache[dev][size].store(known, std::memory_order_release);
     }
-    return cache[dev][size] > 0 ? cache[dev][size] : 0;
+    return known > 0 ? known : 0;
 }
 
 template <int BN, bool SPLIT>
