@@ -149,6 +149,7 @@ class _MoeBlock(nn.Module):
         if self.ep_size == 1:
             if 0 < x.shape[0] <= self.few_tokens:
                 w13_s, w2_s = getattr(self, self._scale_names[0]), getattr(self, self._scale_names[1])
+                x = x.clone() if x.data_ptr() % 16 else x            # these kernels read 16 bytes at a time, the pipeline's quantiser any rows
                 return _moe.few_tokens_moe(x, router_logits, self.w13, w13_s, self.w2, w2_s, self.top_k, **route)
             tw, ti = _ops.moe_route_topk(router_logits, self.top_k, **route)
             return self._run_experts(x, tw, ti)
