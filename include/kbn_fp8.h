@@ -299,8 +299,8 @@ int kbn_moe_route_topk(const void* logits, int logits_bf16, int64_t ld, int64_t 
  *     scale (may be null): row-major bytes [M,K/32], row stride s_row; sf_packed (may be null; one of the two is needed):
  *     the same bytes in the packed form kbn_mxfp4_gemm_nt reads, kbn_packed_mxfp4_bytes(M, K) bytes, 16-byte aligned;
  *     words of rows past M in the last 128-row block are left unwritten, blocks past K count as 2^0.
- *   kbn_silu_mul_quant_mxfp4: in [M, 2*N2] bf16 (gate | up) -> the same outputs for y = bf16(bf16(silu(gate)) * up), [M, N2].
- *     N2 % 32 == 0.  Enqueues the table fill of kbn_silu_mul_quant_1x128 on first use.
+ *   kbn_silu_mul_quant_mxfp4: in [M, 2*N2] bf16 (gate | up) -> the same outputs for y = bf16(bf16(silu(gate)) * up), [M, N2],
+ *     silu as in kbn_silu_mul_quant_1x128 (fp32's, rounded once: -0 below -88.7).  N2 % 32 == 0.  Enqueues the table fill of kbn_silu_mul_quant_1x128 on first use.
  *   kbn_dequant_mxfp4: codes and row-major scales -> bf16 [M,K], row stride ld_out.
  *   kbn_pack_mxfp4_scales: row-major scale bytes [rows,K/32] -> the packed form (rows past the last one: 2^0).
  * Strides of codes and scales are in bytes.

@@ -150,9 +150,11 @@ quant_mxfp4_kernel(const __nv_bfloat16* x, uint32_t K, int64_t ld_x, QuantOut o,
     store_scales<U>(word, valid, row, g0, j, G, K, o);
 }
 
-// Eight gates times eight ups -> four packed bf16x2 y = bf16(bf16(silu(g)) * up), silu exactly rounded.  For every bf16 gate
-// of at least -60 the five-instruction approximation lies on the right side of its rounding boundary (all 65,536 gates are
-// tested), so only gates below that, where the exponential overflows, come from the table of exactly rounded results.
+// Eight gates times eight ups -> four packed bf16x2 y = bf16(bf16(silu(g)) * up).  silu(g) is g / (1 + exp(-g)) in fp32 with an
+// exactly rounded exponential: the exactly rounded SiLU for gates from -60 on (of an odd subnormal gate, whose half is a tie,
+// the even neighbour), -0 below -88.7, where fp32's exponential overflows.  For every finite gate of at least -60 the
+// five-instruction approximation lies on the right side of its rounding boundary, so only gates below that come from the
+// table.  Every finite gate is tested against the definition, by itself and, beside one below -60, from the table.
 __device__ __forceinline__ void silu_mul_exact8(const uint32_t* g, const uint32_t* u, const uint16_t* __restrict__ table, uint32_t* y) {
     const uint32_t gm = min_bf16x2(min_bf16x2(g[0], g[1]), min_bf16x2(g[2], g[3]));
     uint32_t s[4];
@@ -166,7 +168,7 @@ __device__ __forceinline__ void silu_mul_exact8(const uint32_t* g, const uint32_
     for (int i = 0; i < 4; ++i) y[i] = mul_bf16x2(s[i], u[i]);
 }
 
-// bf16(bf16(silu(gate)) * up) with the exactly rounded SiLU of the FP8 activation kernel (silu_exact.cuh), then as above.
+// bf16(bf16(silu(gate)) * up) with the SiLU of the FP8 activation kernel (silu_exact.cuh), then as above.
 // The two roundings to bf16 are those of an unfused activation in the model's type, so that fused and unfused layers agree.
 template <int ALIGN, int U>
 __global__ void __launch_bounds__(256)
