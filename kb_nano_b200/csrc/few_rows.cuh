@@ -23,7 +23,7 @@
 //              leaves fp32's range where the result does not, the tokens' power lacks a constant factor 2^kLift, which the
 //              sums get back at the end: partial sum times power stays below 2^128 (2^31 * 2^(113 - 16) with FP8, 2^23 *
 //              2^(113 - 9) with MXFP4), powers go down to fp32's smallest.  Nothing overflows before 2^128, and a zero sum stays
-//              zero under any scale.  For MXFP4 that is four multiplications a tile and block more than one power per 128 values
+//              zero under any scale; sums below 2^-120 (FP8) and 2^-127 carry fp32's smallest step times 2^kLift.  For MXFP4 that is four multiplications a tile and block more than one power per 128 values
 //              behind the blocks' scales, which overflowed from scales of 2^101 on.
 //   K order    a dot product does not care: lane t of a quad takes 16 consecutive K-values of a row per load (FP8) or
 //              eight (MXFP4), and reads the same K-values of its token.
@@ -33,10 +33,11 @@
 //              eight warps): each half of the consumers has a finisher and two buffers of eight partial sums to itself.
 //
 // Bound: the weights' bytes, once, wherever there are enough units to keep 80 to 190 KB per SM in flight.  One token on 8 of
-// 256 experts (FP8, H 7168, I 2048): 352 MB in 77.2 us, 4.56 TB/s over the whole layer, 7.0 to 7.5 TB/s while the weights
-// stream; 16 tokens: 4.5 GB in 739 us, 93 % of a copy's 6.57 TB/s.  MXFP4 is bound by its conversions (a byte holds two codes, a
-// conversion yields two f16 values): 5 tokens on 8 experts (H 4096, I 14336) take 156 us at 55 to 60 % of all issue slots,
-// 3.65 TB/s.  Converting with integer shifts and masks instead of cvt was slower (175 -> 224 us, one tile per warp).
+// 256 experts (FP8, H 7168, I 2048): 352 MB in 76.4 us (all times inside a graph), 4.61 TB/s over the whole layer, 7.0 to 7.5 TB/s
+// while the weights stream; 16 tokens: 4.5 GB in 724 us, 95 % of a copy's 6.57 TB/s.  MXFP4 is bound by its conversions (a byte
+// holds two codes, a conversion yields two f16 values): 5 tokens on 8 experts (H 4096, I 14336) take 157 us at 52 to 54 % of all
+// issue slots, 3.6 TB/s.  Converting with integer shifts and masks instead of cvt was slower (175 -> 224 us, one tile per warp), and
+// so were packed fp32 multiplications for the tokens' powers (163.9 -> 166.7).
 #pragma once
 #include "gemm_common.cuh"
 #include "mxfp4.cuh"

@@ -23,11 +23,11 @@
 //               receives the other pairs' partial sums of them as one bulk copy each through the cluster's shared memory;
 //               partials are added in slice order, so results are reproducible.
 //
-// Measured: 8192 x 7168 x 7168 153 us, 5.5 PFLOP/s, 82 % of four times the measured bf16 rate of cuBLAS.  What is missing is
+// Measured inside a graph: 8192 x 7168 x 7168 153 us, 5.5 PFLOP/s, 82 % of four times the measured bf16 rate of cuBLAS.  What is missing is
 // the drain of the accumulator between two tiles (1 to 2 us of 11.8) and the last round (896 tiles on 74 pairs: 8 in the
 // thirteenth round, which run as 16 halves).  In a loop of seconds the
-// power cap sets the clock.  512 x 4096 x 7168: 17.1 us with the quantiser (3.2) in front, against 4.5 for the products
-// alone: one tile per pair has nothing to hide its first loads and its drain behind.
+// power cap sets the clock (calls in a row, with the quantiser: 203 to 211 us).  512 x 4096 x 7168: 17.5 us with the quantiser (3.2)
+// in front (calls in a row 19.2 to 20.2), against 4.5 for the products alone: one tile per pair has nothing to hide its first loads and its drain behind.
 #include <algorithm>
 
 #include "gemm_common.cuh"

@@ -4,9 +4,9 @@
 // microsecond a row -- into f16 rows in shared memory and streams its share of the weight rows (few_rows.cuh).  The values are
 // the ones the quantiser would have stored: the codes, exact in f16, and each block's power of two beside them.
 // More rows, or K no multiple of 128: the quantiser and the tensor-core GEMM.
-// Measured, one row, 4096 x 7168 (15.6 MB, 2.4 us at a copy's rate): 6.3 us, against
-// 14.9 for quantiser and GEMM; 7168 x 2048, one to eight rows, 5.2 to 6.5 and 8.7 to 9.4.  Every row adds what its quantisation
-// takes in every CTA: 4096 x 7168, four rows, 9.1 us.
+// Measured inside a graph, one row, 4096 x 7168 (15.6 MB, 2.4 us at a copy's rate): 6.5 us (a call among others 6.7), against
+// 14.9 for quantiser and GEMM; 7168 x 2048, one to eight rows, 5.3 to 6.5 and 8.4 to 8.5.  Every row adds what its quantisation
+// takes in every CTA: 4096 x 7168, four rows, 9.2 us, eight 11.9.
 #include <algorithm>
 
 #include "few_rows.cuh"
@@ -15,8 +15,8 @@ namespace kbn {
 namespace few {
 
 // Rows that leave a shorter ring go through the GEMM.  Weight stream against quantiser and GEMM, with four stages: 8 rows,
-// 4096 x 7168 12.2 and 14.8 us, 7 rows, 16384 x 8192 24.4 and 23.3; with three: 8 rows, 4096 x 8192 14.1 and 15.5, 16384 x 8192
-// 27.5 and 22.7; with two: 8 rows, 7168 x 9216 24.0 and 17.8.
+// 4096 x 7168 11.9 and 14.2 us, 7 rows, 4096 x 8192 12.4 and 15.2, 16384 x 8192 25.3 and 21.9; with three (measured while a power
+// served 128 values): 8 rows, 4096 x 8192 14.1 and 15.5, 16384 x 8192 27.5 and 22.7; with two: 8 rows, 7168 x 9216 24.0 and 17.8.
 constexpr int kLinearMinStages = 4;
 constexpr int kUnitRows = 2 * kBoxRows<kMxfp4>;
 constexpr int kLinearFixed = 1024 + kRedBytes<kMxfp4> + 256 + 128;      // alignment, partial sums, barriers, flag

@@ -19,7 +19,7 @@
 //
 // Bound: the chosen experts' weights, once.  A CTA's range of units is contiguous over (job, row block), so the tokens of
 // a job are loaded into shared memory once or twice per CTA and the ring keeps filling meanwhile.  What a small call takes
-// beyond its bytes is latency: one token, 8 of 128 experts, H 2048, I 768 (38 MB, 5.7 us at a copy's rate) takes 23 us, of which
+// beyond its bytes is latency: one token, 8 of 128 experts, H 2048, I 768 (38 MB, 5.7 us at a copy's rate) takes 22 to 24 us, of which
 // logits, routing and jobs 4, the first stages' way to the first sums 2, the streams themselves 8, the second kernel's start
 // behind the first's last block 2, its jobs, tokens and first stages 3, and the last sums' way through finisher, count and
 // weighted sum 3.  Both kernels on one SM at a time (shorter rings, the second filling its own under the first) was slower: 78 ->

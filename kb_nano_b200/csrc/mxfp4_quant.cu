@@ -5,7 +5,7 @@
 // All four are HBM-bound: 2 B in and 17/32 B out per element (4 B in with the activation), the inverse the other way round.
 // A lane takes 16 consecutive values (one 32-byte access), eight lanes 128 of a row: a block of 32 is two lanes, one shuffle
 // gives its largest magnitude, and the four scale bytes of the 128 values meet in one word, which is stored whole, both in
-// the row-major scales and in the packed layout.  Measured (share of a copy's 6.57 TB/s), 8192 x 7168: quantise 23.7 us (95 %),
+// the row-major scales and in the packed layout.  Measured inside a graph (share of a copy's 6.57 TB/s), 8192 x 7168: quantise 23.7 us (95 %),
 // dequantise 24.8 (91 %), activation and quantise (8192 x 2 * 7168 in) 44.4 (91 %); 16384 x 2048: 14.9, 13.6, 27.0; 512 x 7168:
 // 3.1, 2.6, 4.9, where the launch is most of it.  With 8 values a lane (16-byte accesses) the first were 33.9 and 34.4; the
 // activation took 73 with those and with every gate's SiLU from the table.
