@@ -3,7 +3,7 @@ small operators, csrc/calls.cpp, which reads torch tensors itself) with g++.
 
     python -m kb_nano_b200.build [--force] [--verbose]
 
-Either is rebuilt only when a source or header is newer than it, _calls.so also when torch, Python or its command line are not
+Either is rebuilt only when a source or header is newer than it, _calls.so also when torch, Python or its compiler flags are not
 the ones it was built with (build/_calls.stamp).  Each is linked beside its place and moved there whole, so that a process that
 loads it during a build finds the old or the new one.  nvcc cross-compiles without a GPU, so this also serves as the "does it
 build" check on a CPU-only machine.
@@ -25,6 +25,7 @@ OBJ_DIR = os.path.join(PKG_DIR, "build")
 CALLS_SRC = os.path.join(CSRC, "calls.cpp")
 CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
 CALLS_STAMP = os.path.join(OBJ_DIR, "_calls.stamp")
+CALLS_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -87,16 +88,16 @@ def _calls_command() -> list[str]:
     include = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     lib = os.path.join(root, "lib")
-    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+    return [shutil.which("g++") or "g++", *CALLS_FLAGS,
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), CALLS_SRC,
             f"-L{PKG_DIR}", "-l:" + os.path.basename(LIB_PATH), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
             "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
 
 
 def _calls_stamp() -> str:
-    """What _calls.so depends on beside its sources: torch's tensors and Python's objects have no layout of their own promised."""
+    """What _calls.so depends on beside its sources (torch and Python promise no binary layout), known without a compiler at hand."""
     import torch
-    return "\n".join([torch.__version__, sys.version, *_calls_command()])
+    return "\n".join([torch.__version__, torch.__file__, str(torch._C._GLIBCXX_USE_CXX11_ABI), sys.version, *CALLS_FLAGS])
 
 
 def _calls_need_build() -> bool:

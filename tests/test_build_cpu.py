@@ -75,3 +75,14 @@ def test_a_failed_build_leaves_the_old_file_and_is_tried_again(fake, tmp_path):
     fake.fail = False
     build.build()
     assert content() == "build 3"
+
+
+def test_an_up_to_date_build_needs_no_compiler(fake, monkeypatch):
+    build.build()
+
+    def missing():
+        raise RuntimeError("nvcc not found")
+
+    monkeypatch.setattr(build, "_nvcc", missing)
+    build.build()
+    assert len(fake.outputs) == 1
